@@ -2,6 +2,7 @@
 #pragma once
 
 #include "raggedroute/baseline_ops.h"
+#include "raggedroute/block.h"
 #include "raggedroute/chain.h"
 #include "raggedroute/dispatch.h"
 #include "raggedroute/operators.h"

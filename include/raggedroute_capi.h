@@ -426,6 +426,208 @@ rr_status rr_chain_graph_cache_launch(rr_chain_graph_cache* cache, int32_t entry
 void rr_chain_graph_cache_get_stats(const rr_chain_graph_cache* cache, rr_chain_graph_cache_stats* stats);
 void rr_chain_graph_cache_destroy(rr_chain_graph_cache* cache);
 
+/* ---- the expert block around the routing chain (no reference counterpart) ----
+ *
+ * The products a mixture-of-experts layer computes on the rows that
+ * token_permute placed (rows of expert e: [offsets[e], offsets[e + 1])), and the
+ * norms before and after it. Plain pointers to contiguous row-major tensors of
+ * any alignment their element type has; `dtype` is RR_DTYPE_FP16 or
+ * RR_DTYPE_BF16 (the norms and quantize_rows also RR_DTYPE_FP32). Sums are FP32
+ * (int32 for int8 products). Inputs and outputs must not overlap unless a field
+ * says so. Offsets are read on the device only: rising from 0, offsets[experts]
+ * <= rows; larger or negative ones are cut to [0, rows] and falling ones give
+ * empty experts. Rows past offsets[experts] are neither read nor written. The
+ * kernel families of the other operators apply: auto and optimized (id 950) run the gfx950 kernels, naive one thread per output. Entries allocate and
+ * synchronise nothing and may be captured into graphs.
+ */
+enum { RR_ACT_SILU = 0, RR_ACT_GELU_TANH = 1 };
+
+/* Largest hidden / inner / output width of these entries. */
+#define RR_MAX_BLOCK_WIDTH (1 << 20)
+
+/*
+ * Gated feed-forward block of every expert:
+ *   g = x Wg, u = x Wu, a = act(g) * u, y = a Wd.
+ * a is formed from the FP32 sums of g and u and rounded to `dtype` once, which
+ * the second product reads. gate / up (both or none) receive g and u for
+ * rr_gated_ffn_backward.
+ */
+typedef struct rr_gated_ffn_args {
+  const void* x;          /* [rows, hidden] */
+  const void* w_gate;     /* [experts, hidden, inner] */
+  const void* w_up;       /* [experts, hidden, inner] */
+  const void* w_down;     /* [experts, inner, output] */
+  const int32_t* offsets; /* [experts + 1] */
+  void* gate;             /* [rows, inner], optional */
+  void* up;               /* [rows, inner], optional */
+  void* act;              /* [rows, inner]: a */
+  void* y;                /* [rows, output], of y_dtype */
+  int32_t rows;
+  int32_t experts;
+  int32_t hidden;
+  int32_t inner;
+  int32_t output;
+  int32_t activation;
+  int32_t dtype;
+  int32_t y_dtype; /* dtype, or RR_DTYPE_FP32 (what unpermute reads) */
+  rr_kernel_selection kernel;
+} rr_gated_ffn_args;
+
+/*
+ * Gradients of the block, from gate, up and act as the forward call left them:
+ *   da = dy Wd^T, dg = da u act'(g), du = da act(g),
+ *   dx = dg Wg^T + du Wu^T, dWg = x^T dg, dWu = x^T du, dWd = a^T dy.
+ * dg and du are rounded to `dtype` once (workspace). An expert without rows gets
+ * weight gradients of zero. dx, dw_down and the pair dw_gate, dw_up may be NULL
+ * where they are not wanted. Every sum has a fixed order: equal calls give equal
+ * bits. Workspace: rr_gated_ffn_backward_workspace_size, 16-byte aligned.
+ */
+typedef struct rr_gated_ffn_backward_args {
+  const void* x;
+  const void* w_gate;
+  const void* w_up;
+  const void* w_down;
+  const int32_t* offsets;
+  const void* gate; /* [rows, inner] */
+  const void* up;   /* [rows, inner] */
+  const void* act;  /* [rows, inner] */
+  const void* dy;   /* [rows, output] */
+  void* dx;         /* [rows, hidden] */
+  void* dw_gate;    /* [experts, hidden, inner] */
+  void* dw_up;      /* [experts, hidden, inner] */
+  void* dw_down;    /* [experts, inner, output] */
+  int32_t rows;
+  int32_t experts;
+  int32_t hidden;
+  int32_t inner;
+  int32_t output;
+  int32_t activation;
+  int32_t dtype;
+  rr_kernel_selection kernel;
+} rr_gated_ffn_backward_args;
+
+/*
+ * Norm after a block, gated and scaled onto the residual stream, and norm before
+ * the next block:
+ *   h = x + residual_scale * gate * N(block; post_weight),  n = N(h; pre_weight),
+ *   N(v; w) = v / sqrt(mean(v^2) + eps) * w.
+ * n is formed from the FP32 values of h. block NULL: h = x (h may then be NULL
+ * too); post_weight NULL: the block is added without a norm; gate NULL: gate 1,
+ * else row t / gate_tokens of gate belongs to token t; n NULL (pre_weight is
+ * then not read): h alone. h may be x.
+ */
+typedef struct rr_block_norm_args {
+  const void* x;           /* [tokens, hidden] */
+  const void* block;       /* [tokens, hidden] of block_dtype, optional */
+  const void* post_weight; /* [hidden], optional */
+  const void* gate;        /* [ceil(tokens / gate_tokens), hidden], optional */
+  const void* pre_weight;  /* [hidden] */
+  void* h;                 /* [tokens, hidden] */
+  void* n;                 /* [tokens, hidden], optional */
+  float residual_scale;
+  float eps; /* > 0 */
+  int32_t gate_tokens;
+  int32_t tokens;
+  int32_t hidden;
+  int32_t dtype;       /* of everything but block */
+  int32_t block_dtype; /* dtype, or RR_DTYPE_FP32 (what unpermute writes) */
+  rr_kernel_selection kernel;
+} rr_block_norm_args;
+
+/*
+ * Gradients of rr_block_norm from its h (as written) and the gradients of h (dh,
+ * NULL: none) and n (dn, NULL: none; not both):
+ *   dx = dh + dN(h)^T dn,  db = residual_scale * gate * dx,  dblock = dN(block)^T db,
+ *   dgate = sum over the gate row's tokens of residual_scale * N(block) * dx,
+ *   dpre_weight = sum dn * h / rms(h),  dpost_weight = sum db * block / rms(block).
+ * dblock, dgate, dpre_weight and dpost_weight may be NULL where they are not
+ * wanted. dx may be dh, dblock may be block where their types agree. Sums over
+ * tokens go by fixed parts in a fixed order: equal calls give equal bits.
+ * Workspace: rr_block_norm_backward_workspace_size, 16-byte aligned.
+ */
+typedef struct rr_block_norm_backward_args {
+  const void* h;           /* [tokens, hidden] */
+  const void* block;       /* as in the forward call */
+  const void* post_weight;
+  const void* gate;
+  const void* pre_weight;
+  const void* dh;     /* [tokens, hidden], optional */
+  const void* dn;     /* [tokens, hidden], optional */
+  void* dx;           /* [tokens, hidden] */
+  void* dblock;       /* [tokens, hidden] of block_dtype, optional */
+  void* dgate;        /* as gate, optional */
+  void* dpre_weight;  /* [hidden], optional */
+  void* dpost_weight; /* [hidden], optional */
+  float residual_scale;
+  float eps;
+  int32_t gate_tokens;
+  int32_t tokens;
+  int32_t hidden;
+  int32_t dtype;
+  int32_t block_dtype;
+  rr_kernel_selection kernel;
+} rr_block_norm_backward_args;
+
+/*
+ * Rows to 8-bit integers with a scale each: scale = max|x| / 127 and q =
+ * round(x / scale), both divisions in FP32, halves to even; a row of zeros has
+ * scale 0 and q 0. A row with an infinity or a NaN has that scale and q 0, so that
+ * its products are NaN. Also lays weights out for rr_int8_grouped_gemm: one row
+ * per expert and output channel.
+ */
+typedef struct rr_quantize_rows_args {
+  const void* x; /* [rows, hidden] of dtype (FP32, FP16 or BF16) */
+  int8_t* q;     /* [rows, hidden] */
+  float* scale;  /* [rows] */
+  int32_t rows;
+  int32_t hidden;
+  int32_t dtype;
+  rr_kernel_selection kernel;
+} rr_quantize_rows_args;
+
+/*
+ * Expert products of quantised rows and weights, exact in int32:
+ *   p(w)[r, n] = (sum_k q[r, k] w[e, n, k]) * q_scale[r] * w_scale[e, n];
+ * y = p(w), or with w_up the gated form y = act(p(w)) * p(w_up). hidden <= 131072
+ * keeps the sums inside int32.
+ */
+typedef struct rr_int8_grouped_gemm_args {
+  const int8_t* q;         /* [rows, hidden] */
+  const float* q_scale;    /* [rows] */
+  const int8_t* w;         /* [experts, output, hidden] */
+  const float* w_scale;    /* [experts, output] */
+  const int8_t* w_up;      /* [experts, output, hidden], optional */
+  const float* w_up_scale; /* [experts, output], with w_up */
+  const int32_t* offsets;  /* [experts + 1] */
+  void* y;                 /* [rows, output] of dtype (FP32, FP16 or BF16) */
+  int32_t rows;
+  int32_t experts;
+  int32_t hidden;
+  int32_t output;
+  int32_t activation; /* with w_up */
+  int32_t dtype;
+  rr_kernel_selection kernel;
+} rr_int8_grouped_gemm_args;
+
+size_t rr_gated_ffn_workspace_size(const rr_gated_ffn_args* args);
+/* d gate and d up: 2 * rows * inner values, each part rounded up to 16 bytes */
+size_t rr_gated_ffn_backward_workspace_size(const rr_gated_ffn_backward_args* args);
+size_t rr_block_norm_workspace_size(const rr_block_norm_args* args);
+/* FP32 column sums of every part of the tokens */
+size_t rr_block_norm_backward_workspace_size(const rr_block_norm_backward_args* args);
+size_t rr_quantize_rows_workspace_size(const rr_quantize_rows_args* args);
+size_t rr_int8_grouped_gemm_workspace_size(const rr_int8_grouped_gemm_args* args);
+
+rr_status rr_gated_ffn(const rr_gated_ffn_args* args, const rr_runtime_context* context);
+rr_status rr_gated_ffn_backward(const rr_gated_ffn_backward_args* args,
+                                const rr_runtime_context* context);
+rr_status rr_block_norm(const rr_block_norm_args* args, const rr_runtime_context* context);
+rr_status rr_block_norm_backward(const rr_block_norm_backward_args* args,
+                                 const rr_runtime_context* context);
+rr_status rr_quantize_rows(const rr_quantize_rows_args* args, const rr_runtime_context* context);
+rr_status rr_int8_grouped_gemm(const rr_int8_grouped_gemm_args* args,
+                               const rr_runtime_context* context);
+
 /* Static device scratch of rr_chain_from_tokens_noalloc: one copy per GPU,
  * held until the process ends. */
 #define RR_CHAIN_NOALLOC_SCRATCH_BYTES (1u << 20)

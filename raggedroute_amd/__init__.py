@@ -34,6 +34,9 @@ from ._capi import (  # noqa: F401  (re-exported vocabulary)
     CHAIN_FROM_LOGITS,
     CHAIN_FROM_ROUTE_IDS,
     CHAIN_FROM_TOKENS,
+    Activation,
+    BlockNormArgs,
+    BlockNormBackwardArgs,
     ChainArgs,
     ChainGraphCacheStats,
     ConstTensorView,
@@ -42,14 +45,18 @@ from ._capi import (  # noqa: F401  (re-exported vocabulary)
     DispatchDecision,
     DispatchRequest,
     ExclusiveScanArgs,
+    GatedFfnArgs,
+    GatedFfnBackwardArgs,
     GroupedGemmArgs,
     HistogramArgs,
     HistogramExclusiveScanArgs,
+    Int8GroupedGemmArgs,
     KernelFamily,
     KernelSelection,
     MutableTensorView,
     OperatorKind,
     OperatorSignature,
+    QuantizeRowsArgs,
     RouteChainArgs,
     RouteTraceInfo,
     RuntimeContext,
@@ -157,6 +164,39 @@ def chain_fused_launch_names(args: ChainArgs, from_tokens: bool) -> list[str]:
         if name is None:
             return names
         names.append(name.decode())
+
+
+# ---- the expert block around the chain (no reference counterpart) ----
+
+def gated_ffn(args: GatedFfnArgs, context: RuntimeContext | None = None) -> Status:
+    """Gated feed-forward block of every expert over its routed rows."""
+    return lib.rr_gated_ffn(byref(args), byref(_ctx(context)))
+
+
+def gated_ffn_backward(args: GatedFfnBackwardArgs, context: RuntimeContext | None = None) -> Status:
+    """Gradients of gated_ffn, from the gate, up and act rows it kept."""
+    return lib.rr_gated_ffn_backward(byref(args), byref(_ctx(context)))
+
+
+def block_norm(args: BlockNormArgs, context: RuntimeContext | None = None) -> Status:
+    """h = x + residual_scale * gate * N(block), n = N(h): the norms after a block and before the next."""
+    return lib.rr_block_norm(byref(args), byref(_ctx(context)))
+
+
+def block_norm_backward(args: BlockNormBackwardArgs,
+                        context: RuntimeContext | None = None) -> Status:
+    """Gradients of block_norm, from the h it wrote."""
+    return lib.rr_block_norm_backward(byref(args), byref(_ctx(context)))
+
+
+def quantize_rows(args: QuantizeRowsArgs, context: RuntimeContext | None = None) -> Status:
+    """Rows to 8-bit integers, each with an FP32 scale."""
+    return lib.rr_quantize_rows(byref(args), byref(_ctx(context)))
+
+
+def int8_grouped_gemm(args: Int8GroupedGemmArgs, context: RuntimeContext | None = None) -> Status:
+    """Expert products of 8-bit rows and weights with scales per row and output channel."""
+    return lib.rr_int8_grouped_gemm(byref(args), byref(_ctx(context)))
 
 
 # ---- chain graphs (rr_chain_graph_*, rr_chain_graph_cache_*) ----
@@ -279,6 +319,30 @@ def get_unpermute_workspace_size(args: UnpermuteArgs) -> int:
 
 def get_chain_workspace_size(args: ChainArgs) -> int:
     return lib.rr_chain_workspace_size(byref(args))
+
+
+def get_gated_ffn_workspace_size(args: GatedFfnArgs) -> int:
+    return lib.rr_gated_ffn_workspace_size(byref(args))
+
+
+def get_gated_ffn_backward_workspace_size(args: GatedFfnBackwardArgs) -> int:
+    return lib.rr_gated_ffn_backward_workspace_size(byref(args))
+
+
+def get_block_norm_workspace_size(args: BlockNormArgs) -> int:
+    return lib.rr_block_norm_workspace_size(byref(args))
+
+
+def get_block_norm_backward_workspace_size(args: BlockNormBackwardArgs) -> int:
+    return lib.rr_block_norm_backward_workspace_size(byref(args))
+
+
+def get_quantize_rows_workspace_size(args: QuantizeRowsArgs) -> int:
+    return lib.rr_quantize_rows_workspace_size(byref(args))
+
+
+def get_int8_grouped_gemm_workspace_size(args: Int8GroupedGemmArgs) -> int:
+    return lib.rr_int8_grouped_gemm_workspace_size(byref(args))
 
 
 # ---- dispatch (reference include/raggedroute/dispatch.h:32-46) ----

@@ -67,6 +67,11 @@ class StatusCode(enum.IntEnum):
     kDeviceError = 7
 
 
+class Activation(enum.IntEnum):
+    kSilu = 0
+    kGeluTanh = 1
+
+
 GFX950_NATIVE = 950
 MAX_EXPERTS = 1024
 
@@ -296,6 +301,163 @@ class ChainArgs(ctypes.Structure):
         super().__init__(**kw)
 
 
+class GatedFfnArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", c_void_p),
+        ("w_gate", c_void_p),
+        ("w_up", c_void_p),
+        ("w_down", c_void_p),
+        ("offsets", c_void_p),
+        ("gate", c_void_p),
+        ("up", c_void_p),
+        ("act", c_void_p),
+        ("y", c_void_p),
+        ("rows", c_int32),
+        ("experts", c_int32),
+        ("hidden", c_int32),
+        ("inner", c_int32),
+        ("output", c_int32),
+        ("activation", c_int32),
+        ("dtype", c_int32),
+        ("y_dtype", c_int32),
+        ("kernel", KernelSelection),
+    ]
+
+    def __init__(self, **kw):
+        kw.setdefault("dtype", ScalarType.kBf16)
+        kw.setdefault("y_dtype", kw["dtype"])
+        super().__init__(**kw)
+
+
+class GatedFfnBackwardArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", c_void_p),
+        ("w_gate", c_void_p),
+        ("w_up", c_void_p),
+        ("w_down", c_void_p),
+        ("offsets", c_void_p),
+        ("gate", c_void_p),
+        ("up", c_void_p),
+        ("act", c_void_p),
+        ("dy", c_void_p),
+        ("dx", c_void_p),
+        ("dw_gate", c_void_p),
+        ("dw_up", c_void_p),
+        ("dw_down", c_void_p),
+        ("rows", c_int32),
+        ("experts", c_int32),
+        ("hidden", c_int32),
+        ("inner", c_int32),
+        ("output", c_int32),
+        ("activation", c_int32),
+        ("dtype", c_int32),
+        ("kernel", KernelSelection),
+    ]
+
+    def __init__(self, **kw):
+        kw.setdefault("dtype", ScalarType.kBf16)
+        super().__init__(**kw)
+
+
+class BlockNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", c_void_p),
+        ("block", c_void_p),
+        ("post_weight", c_void_p),
+        ("gate", c_void_p),
+        ("pre_weight", c_void_p),
+        ("h", c_void_p),
+        ("n", c_void_p),
+        ("residual_scale", c_float),
+        ("eps", c_float),
+        ("gate_tokens", c_int32),
+        ("tokens", c_int32),
+        ("hidden", c_int32),
+        ("dtype", c_int32),
+        ("block_dtype", c_int32),
+        ("kernel", KernelSelection),
+    ]
+
+    def __init__(self, **kw):
+        kw.setdefault("dtype", ScalarType.kBf16)
+        kw.setdefault("block_dtype", kw["dtype"])
+        kw.setdefault("residual_scale", 1.0)
+        kw.setdefault("eps", 1e-6)
+        super().__init__(**kw)
+
+
+class BlockNormBackwardArgs(ctypes.Structure):
+    _fields_ = [
+        ("h", c_void_p),
+        ("block", c_void_p),
+        ("post_weight", c_void_p),
+        ("gate", c_void_p),
+        ("pre_weight", c_void_p),
+        ("dh", c_void_p),
+        ("dn", c_void_p),
+        ("dx", c_void_p),
+        ("dblock", c_void_p),
+        ("dgate", c_void_p),
+        ("dpre_weight", c_void_p),
+        ("dpost_weight", c_void_p),
+        ("residual_scale", c_float),
+        ("eps", c_float),
+        ("gate_tokens", c_int32),
+        ("tokens", c_int32),
+        ("hidden", c_int32),
+        ("dtype", c_int32),
+        ("block_dtype", c_int32),
+        ("kernel", KernelSelection),
+    ]
+
+    def __init__(self, **kw):
+        kw.setdefault("dtype", ScalarType.kBf16)
+        kw.setdefault("block_dtype", kw["dtype"])
+        kw.setdefault("residual_scale", 1.0)
+        kw.setdefault("eps", 1e-6)
+        super().__init__(**kw)
+
+
+class QuantizeRowsArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", c_void_p),
+        ("q", c_void_p),
+        ("scale", c_void_p),
+        ("rows", c_int32),
+        ("hidden", c_int32),
+        ("dtype", c_int32),
+        ("kernel", KernelSelection),
+    ]
+
+    def __init__(self, **kw):
+        kw.setdefault("dtype", ScalarType.kBf16)
+        super().__init__(**kw)
+
+
+class Int8GroupedGemmArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", c_void_p),
+        ("q_scale", c_void_p),
+        ("w", c_void_p),
+        ("w_scale", c_void_p),
+        ("w_up", c_void_p),
+        ("w_up_scale", c_void_p),
+        ("offsets", c_void_p),
+        ("y", c_void_p),
+        ("rows", c_int32),
+        ("experts", c_int32),
+        ("hidden", c_int32),
+        ("output", c_int32),
+        ("activation", c_int32),
+        ("dtype", c_int32),
+        ("kernel", KernelSelection),
+    ]
+
+    def __init__(self, **kw):
+        kw.setdefault("dtype", ScalarType.kBf16)
+        super().__init__(**kw)
+
+
 class OperatorSignature(ctypes.Structure):
     _fields_ = [
         ("has_input", c_int32),
@@ -336,6 +498,12 @@ _OP_ENTRIES = [
     ("token_permute", TokenPermuteArgs),
     ("grouped_gemm", GroupedGemmArgs),
     ("unpermute", UnpermuteArgs),
+    ("gated_ffn", GatedFfnArgs),
+    ("gated_ffn_backward", GatedFfnBackwardArgs),
+    ("block_norm", BlockNormArgs),
+    ("block_norm_backward", BlockNormBackwardArgs),
+    ("quantize_rows", QuantizeRowsArgs),
+    ("int8_grouped_gemm", Int8GroupedGemmArgs),
 ]
 
 PROTOTYPES: list[tuple[str, object, list]] = []

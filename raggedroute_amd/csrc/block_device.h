@@ -1,0 +1,49 @@
+// Element types, activations and segment lookups shared by the expert block's kernels.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+
+#include "raggedroute_capi.h"
+
+namespace rr::dev {
+
+typedef __bf16 bf16;
+typedef _Float16 f16;
+
+// 1 / (1 + e^-v): v_exp_f32 takes powers of two. e^-v past FP32 gives 0, NaN stays.
+__device__ __forceinline__ float sigmoid(float v) {
+  return __builtin_amdgcn_rcpf(1.0F + __builtin_amdgcn_exp2f(-1.44269504088896341F * v));
+}
+
+// act(g) = g sigmoid(t(g)): t(g) = g for SiLU, and for the tanh form of GELU
+// (1 + tanh z) / 2 = sigmoid(2 z) with z = sqrt(2 / pi) (g + 0.044715 g^3).
+constexpr float kGelu = 1.59576912160573071F;  // 2 sqrt(2 / pi)
+constexpr float kGeluCube = 0.044715F;
+
+__device__ __forceinline__ float activation(int kind, float g) {
+  const float t = kind == RR_ACT_SILU ? g : kGelu * (g + kGeluCube * g * g * g);
+  return g * sigmoid(t);
+}
+
+// act(g) and act'(g) = s + g t'(g) s (1 - s), s = sigmoid(t(g)). The second term is
+// below FP32's last bit of the sum from |g| = 40 on and is formed there from 40, where no
+// square or cube overflows against 1 - s = 0.
+__device__ __forceinline__ void activation_grad(int kind, float g, float* act, float* grad) {
+  const float t = kind == RR_ACT_SILU ? g : kGelu * (g + kGeluCube * g * g * g);
+  const float s = sigmoid(t);
+  const float b = g > 40.0F ? 40.0F : g < -40.0F ? -40.0F : g;
+  const float slope = kind == RR_ACT_SILU ? 1.0F : kGelu * (1.0F + 3.0F * kGeluCube * b * b);
+  *act = g * s;
+  *grad = s + b * slope * (s * (1.0F - s));
+}
+
+// offsets[e] cut to [0, rows]
+__device__ __forceinline__ int offset_at(const int32_t* offsets, int e, int rows) {
+  const int o = offsets[e];
+  return o < 0 ? 0 : o > rows ? rows : o;
+}
+
+}  // namespace rr::dev
