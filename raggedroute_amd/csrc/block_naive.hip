@@ -203,8 +203,4 @@ hipError_t int8_grouped_gemm_naive(const Int8Params& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-hipError_t gated_ffn(const FfnParams& p, hipStream_t stream) { return gated_ffn_naive(p, stream); }
-hipError_t gated_ffn_backward(const FfnParams& p, hipStream_t stream) { return gated_ffn_backward_naive(p, stream); }
-hipError_t int8_grouped_gemm(const Int8Params& p, hipStream_t stream) { return int8_grouped_gemm_naive(p, stream); }
-
 }  // namespace rr::kern

@@ -1,0 +1,680 @@
+// Grouped products of the expert block: 256-column tiles of 256 rows on the 16-bit and
+// int8 matrix instructions (v_mfma_f32_16x16x32_bf16 / _f16, v_mfma_i32_16x16x64_i8).
+//
+// One workgroup of eight waves a CU walks over output tiles; a k slice is 128 bytes of
+// every row (64 16-bit or 128 int8 elements). Both operands' slices go straight from
+// memory into one of two LDS stages of 64 KB (buffer loads, 16 bytes a lane), two slices
+// ahead of the products and across the end of a tile: the stream of slices does not
+// stop for an epilogue.
+//  - Left operand and right operand may each have k along rows (KC: 128-byte rows in
+//    LDS, read with ds_read_b128) or down columns (KS: rows of 128 columns, read with
+//    ds_read_b64_tr_b16, which hands each lane four k of one column), so that no product
+//    of the block, forward or backward, needs a transposed copy.
+//  - 16-byte chunks are placed at chunk ^ f(row) by loading permuted chunks: the lanes
+//    that read together then reach all 64 banks.
+//  - What lies past a row's, segment's or expert's end is cut off by the buffer's record
+//    count (reads past it give zeros), what lies past the sum's length inside a row by
+//    an offset past it.
+//  - Wave (wm, wn) sums 128 rows x 64 columns (dual products: 32 columns of each right
+//    operand, so that gate and up of an element meet in one lane). The right operand is
+//    the instruction's first one and its columns are dealt so that a lane ends with 16 (8
+//    and 8) adjacent columns of a row: wide stores, no exchange.
+//  - The waves of wm = 0 and wm = 1 share the SIMDs pairwise and run a phase apart: while
+//    one reads its operands and issues loads, the other has the matrix pipe.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstddef>
+#include <cstdint>
+#include <initializer_list>
+#include <type_traits>
+
+#include "expert_gemm.h"
+#include "tiles.h"
+#include "wave.h"
+
+namespace rr::kern {
+namespace {
+
+using rr::dev::bf16;
+using rr::dev::f16;
+
+#define RR_LDS __attribute__((address_space(3)))
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef int i4 __attribute__((ext_vector_type(4)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+
+constexpr int kBufferFlags = 0x00027000;  // raw 32-bit buffer
+constexpr uint32_t kPast = 0x80000000U;   // an offset past every record count
+constexpr int kTileRows = 256;
+constexpr int kTileCols = 256;
+constexpr int kSliceBytes = 128;              // of every row
+constexpr int kOperandBytes = 256 * kSliceBytes;  // one operand's slice
+constexpr int kHalfBytes = kOperandBytes / 2;
+constexpr int kStageBytes = 2 * kOperandBytes;
+constexpr int kThreads = 512;
+
+template <typename T>
+struct Matrix;
+template <>
+struct Matrix<bf16> {
+  typedef bf16 frag __attribute__((ext_vector_type(8)));
+  typedef f4 acc;
+  static __device__ __forceinline__ acc mul(i4 a, i4 b, acc c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(frag, a), __builtin_bit_cast(frag, b), c, 0, 0, 0);
+  }
+};
+template <>
+struct Matrix<f16> {
+  typedef f16 frag __attribute__((ext_vector_type(8)));
+  typedef f4 acc;
+  static __device__ __forceinline__ acc mul(i4 a, i4 b, acc c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(frag, a), __builtin_bit_cast(frag, b), c, 0, 0, 0);
+  }
+};
+template <>
+struct Matrix<int8_t> {
+  typedef i4 acc;
+  static __device__ __forceinline__ acc mul(i4 a, i4 b, acc c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+  }
+};
+
+// A kernel: element type, whether A and B have k along rows (KC), weight gradients or row
+// products, epilogue.
+template <typename T_, bool A_KC, bool B_KC, bool WEIGHTS, class Epi_>
+struct Kind {
+  using T = T_;
+  using Epi = Epi_;
+  static constexpr bool kAKC = A_KC, kBKC = B_KC, kWeights = WEIGHTS, kDual = Epi_::kDual;
+  static constexpr int kSlice = kSliceBytes / sizeof(T_);  // k of a slice
+  static constexpr int kCols = kDual ? kTileCols / 2 : kTileCols;
+  static_assert(A_KC || sizeof(T_) == 2, "transposing reads are 16-bit");
+  static_assert(B_KC || sizeof(T_) == 2, "transposing reads are 16-bit");
+};
+
+// The chunk permutations f(row): KC by eight chunks of a 128-byte row, KS by 16 of a
+// 256-byte row (k). The rows (and pieces) that 16 lanes read together differ in the bits
+// used: KC A rows 16 i + 0..15; KC B columns 4 J a + 4 j + b (a, b in 0..3); KS k 8 g + 4 q + 0..3.
+template <bool DUAL>
+__device__ __forceinline__ int swizzle_b_row(int r) {
+  return (r & 3) | ((r >> (DUAL ? 3 : 4)) & 1) << 2;
+}
+__device__ __forceinline__ int swizzle_a_k(int k) { return (k & 3) << 1 | ((k >> 3) & 1) << 3; }
+template <bool DUAL>
+__device__ __forceinline__ int swizzle_b_k(int k) {
+  return DUAL ? (k & 3) << 2 : (k & 1) | ((k >> 1) & 1) << 3;
+}
+
+// Barriers and waits of the pipeline. The loads into LDS are written in assembly: they
+// have no register results, and the compiler, which would wait for all of them before
+// any LDS read, does not see them; every wait for them is one of these.
+__device__ __forceinline__ void phase_barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_barrier" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+template <int LOADS>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
+}
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// 64 lanes x 16 bytes from `rsrc` (a byte offset per lane) to LDS at `to`.
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t rsrc, uint32_t offset, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(rsrc)
+               : "memory");
+}
+
+__device__ __forceinline__ i4 read16(uint32_t at) { return *reinterpret_cast<RR_LDS const i4*>(at); }
+// Two transposing reads: eight k of one column, `at` and four rows further.
+__device__ __forceinline__ i4 read_columns(uint32_t at) {
+  const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<RR_LDS s4*>(at));
+  const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<RR_LDS s4*>(at + 4 * 256));
+  typedef int i2 __attribute__((ext_vector_type(2)));
+  const i2 l = __builtin_bit_cast(i2, lo), h = __builtin_bit_cast(i2, hi);
+  return i4{l[0], l[1], h[0], h[1]};
+}
+
+// An output tile (uniform).
+struct Tile {
+  int e;           // expert
+  int first;       // its first row
+  int row0, rows;  // row products: first row and rows; weight gradients: first row of the result and rows there
+  int n0;          // first column
+  int slices;      // k slices, of all parts
+};
+
+template <class P>
+__global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm) {
+  using T = typename P::T;
+  using M = Matrix<T>;
+  using Acc = typename M::acc;
+  constexpr int S = sizeof(T);
+  extern __shared__ __align__(16) char smem[];
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((RR_LDS char*)smem));
+  int32_t* s_off = reinterpret_cast<int32_t*>(smem + 2 * kStageBytes);  // [E + 1]
+  int32_t* s_pre = s_off + prm.experts + 1;                             // [E + 1] full row tiles before expert e
+  int32_t* s_pre2 = s_pre + prm.experts + 1;                            // [E + 1] short row tiles before expert e
+  const int tid = static_cast<int>(threadIdx.x);
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave >> 2, wn = wave & 3;
+  const int li = lane & 15, g = lane >> 4;
+  const int experts = prm.experts;
+
+  for (int e = tid; e <= experts; e += kThreads) s_off[e] = rr::dev::offset_at(prm.offsets, e, prm.rows);
+  __syncthreads();
+  if constexpr (!P::kWeights) {
+    if (wave == 0) build_tile_prefix<kTileRows, true>(s_off, s_pre, s_pre2, experts, lane);
+    __syncthreads();
+  }
+  const int col_tiles = (prm.N + P::kCols - 1) / P::kCols;
+  const int m_tiles = P::kWeights ? (prm.M + kTileRows - 1) / kTileRows : 0;
+  const int full_rows = P::kWeights ? 0 : __builtin_amdgcn_readfirstlane(s_pre[experts]);
+  const int short_rows = P::kWeights ? 0 : __builtin_amdgcn_readfirstlane(s_pre2[experts]);
+  const int total_full = full_rows * col_tiles;
+  const int total = P::kWeights ? experts * m_tiles * col_tiles : total_full + short_rows * col_tiles;
+  const int grid = static_cast<int>(gridDim.x);
+  const int worker = tile_worker(static_cast<int>(blockIdx.x), grid);
+  const int part_slices = P::kWeights ? 0 : (prm.K + P::kSlice - 1) / P::kSlice;
+  const int parts = P::kWeights || prm.a2 == nullptr || S == 1 ? 1 : 2;
+
+  // the workgroup's tile of a round (the last, partial round goes to the workgroups in
+  // dispatch order, over all XCDs); false past the last
+  auto decode = [&](int dealt, Tile& tl) {
+    const int mine = total - dealt >= grid ? worker : static_cast<int>(blockIdx.x);
+    const int t = dealt + mine;
+    if (t >= total) return false;
+    int rt, ct;
+    if constexpr (P::kWeights) {
+      tl.e = t / (m_tiles * col_tiles);
+      decode_tile(t - tl.e * m_tiles * col_tiles, m_tiles, col_tiles, &rt, &ct);
+      tl.first = __builtin_amdgcn_readfirstlane(s_off[tl.e]);
+      const int count = __builtin_amdgcn_readfirstlane(s_off[tl.e + 1]) - tl.first;
+      tl.row0 = rt * kTileRows;
+      tl.rows = min(prm.M - tl.row0, kTileRows);
+      // (an expert without rows takes one slice of zeros)
+      tl.slices = count > P::kSlice ? (count + P::kSlice - 1) / P::kSlice : 1;
+    } else {
+      const bool is_short = t >= total_full;
+      decode_tile(is_short ? t - total_full : t, is_short ? short_rows : full_rows, col_tiles, &rt, &ct);
+      tl.e = __builtin_amdgcn_readfirstlane(tile_expert(is_short ? s_pre2 : s_pre, experts, rt));
+      tl.first = __builtin_amdgcn_readfirstlane(s_off[tl.e]);
+      const int end = __builtin_amdgcn_readfirstlane(s_off[tl.e + 1]);
+      tl.row0 = tl.first +
+                (is_short ? (end - tl.first) / kTileRows : rt - __builtin_amdgcn_readfirstlane(s_pre[tl.e])) * kTileRows;
+      tl.rows = min(end - tl.row0, kTileRows);
+      tl.slices = part_slices * parts;
+    }
+    tl.n0 = ct * P::kCols;
+    return true;
+  };
+
+  // ---- the stream of slices into LDS ----
+  // Wave w brings rows 32 w .. + 31 (KC) or k rows 16 (w % 4) .. + 15 of half w / 4 (KS) of
+  // each operand in four loads; half w / 4 is the columns (of KS A: rows of the result)
+  // from 128 on, or in a dual product the right operand b_up.
+  const int half = wave >> 2;
+  // (lane offsets carry everything that varies: a range check must see the whole offset)
+  uint32_t a_lane[4], b_lane[4], a_chunk = 0, b_chunk[2] = {};
+  constexpr int b_bit = P::kDual ? 0 : 1;  // the bit of q that B's chunk depends on (KC)
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if constexpr (P::kAKC) {
+      const int r = 32 * wave + 8 * q + (lane >> 3);
+      a_chunk = static_cast<uint32_t>((lane & 7) ^ (r & 7)) << 4;
+      a_lane[q] = static_cast<uint32_t>(r) * static_cast<uint32_t>(prm.lda) * S + a_chunk;
+    } else {
+      const int k = 16 * wn + 4 * q + (lane >> 4);
+      a_lane[q] = static_cast<uint32_t>(k) * static_cast<uint32_t>(prm.lda) * S +
+                  (static_cast<uint32_t>((lane & 15) ^ swizzle_a_k(k)) << 4);
+    }
+    if constexpr (P::kBKC) {
+      const int r = 32 * wn + 8 * q + (lane >> 3);
+      const uint32_t chunk = static_cast<uint32_t>((lane & 7) ^ swizzle_b_row<P::kDual>(r)) << 4;
+      b_chunk[(q >> b_bit) & 1] = chunk;
+      b_lane[q] = static_cast<uint32_t>(r) * static_cast<uint32_t>(prm.ldb) * S + chunk;
+    } else {
+      const int k = 16 * wn + 4 * q + (lane >> 4);
+      b_lane[q] = static_cast<uint32_t>(k) * static_cast<uint32_t>(prm.ldb) * S +
+                  (static_cast<uint32_t>((lane & 15) ^ swizzle_b_k<P::kDual>(k)) << 4);
+    }
+  }
+  // bytes between slices
+  const int64_t a_slice = P::kAKC ? kSliceBytes : static_cast<int64_t>(P::kSlice) * prm.lda * S;
+  const int64_t b_slice = P::kBKC ? kSliceBytes : static_cast<int64_t>(P::kSlice) * prm.ldb * S;
+  const uint32_t to_a = lds0 + wave * (kOperandBytes / 8);
+  const uint32_t to_b = to_a + kOperandBytes;
+
+  Tile next;               // the tile whose slices are being loaded
+  int dealt = 0;           // its round
+  bool open;               // there is one
+  int slice = 0;           // its slice to be loaded
+  const char *a_at, *b_at;  // the slice of each operand, and the bytes to the operand's end from there
+  int64_t a_left, b_left;
+  int k_left;  // bytes of a row's sum from the slice on
+  auto start_part = [&](int part) {
+    const char* a = static_cast<const char*>(part == 0 ? prm.a : prm.a2);
+    const char* b = static_cast<const char*>(P::kDual ? (half == 0 ? prm.b : prm.b_up) : part == 0 ? prm.b : prm.b_up);
+    const int n = next.n0 + (P::kDual ? 0 : half * 128);
+    if constexpr (P::kWeights) {
+      const int count = s_off[next.e + 1] - next.first;
+      const int64_t rows = __builtin_amdgcn_readfirstlane(count > 0 ? count : 0);
+      const int m = next.row0 + half * 128;
+      a_at = a + (static_cast<int64_t>(next.first) * prm.lda + m) * S;
+      a_left = m < prm.M ? (rows * prm.lda - m) * S : 0;
+      b_at = b + (static_cast<int64_t>(next.first) * prm.ldb + n) * S;
+      b_left = n < prm.N ? (rows * prm.ldb - n) * S : 0;
+    } else {
+      a_at = a + static_cast<int64_t>(next.row0) * prm.lda * S;
+      a_left = static_cast<int64_t>(next.rows) * prm.lda * S;
+      if constexpr (P::kBKC) {
+        b_at = b + (static_cast<int64_t>(next.e) * prm.N + n) * prm.ldb * S;
+        b_left = static_cast<int64_t>(min(prm.N - n, 128)) * prm.ldb * S;
+      } else {
+        b_at = b + (static_cast<int64_t>(next.e) * prm.K * prm.ldb + n) * S;
+        b_left = n < prm.N ? (static_cast<int64_t>(prm.K) * prm.ldb - n) * S : 0;
+      }
+      k_left = prm.K * S;
+    }
+  };
+  auto start_tile = [&]() {
+    open = decode(dealt, next);
+    slice = 0;
+    if (open) {
+      start_part(0);
+    } else {
+      a_left = b_left = 0;
+    }
+  };
+  auto records = [](int64_t left) { return static_cast<int>(left <= 0 ? 0 : left < 0x7FFFFFFF ? left : 0x7FFFFFFF); };
+  auto cut = [&](uint32_t offset, uint32_t chunk) { return static_cast<int>(chunk) < k_left ? offset : kPast; };
+  auto load_b = [&](int stage) {
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(b_at), 0, records(b_left), kBufferFlags);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint32_t at = P::kBKC ? cut(b_lane[q], b_chunk[(q >> b_bit) & 1]) : b_lane[q];
+      load_to_lds(rsrc, at, to_b + stage * kStageBytes + q * 1024);
+    }
+  };
+  auto load_a = [&](int stage) {  // and on to the next slice
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(a_at), 0, records(a_left), kBufferFlags);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint32_t at = P::kAKC ? cut(a_lane[q], a_chunk) : a_lane[q];
+      load_to_lds(rsrc, at, to_a + stage * kStageBytes + q * 1024);
+    }
+    if (!open) return;
+    a_at += a_slice;
+    a_left -= a_slice;
+    b_at += b_slice;
+    b_left -= b_slice;
+    k_left -= kSliceBytes;
+    ++slice;
+    if (slice == next.slices) {
+      dealt += grid;
+      start_tile();
+    } else if (!P::kWeights && parts == 2 && slice == part_slices) {
+      start_part(1);
+    }
+  };
+
+  // ---- operand reads ----
+  uint32_t b_read[2];  // per k half (KC), per fragment pair (KS)
+  if constexpr (P::kBKC) {
+    const int r = (P::kDual ? 32 * wn + 8 * (li >> 2) : 64 * (wn & 1) + 16 * (li >> 2)) + (li & 3);
+    const uint32_t base = lds0 + kOperandBytes + (P::kDual ? 0 : (wn >> 1) * kHalfBytes) + r * kSliceBytes;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) b_read[h] = base + (static_cast<uint32_t>((4 * h + g) ^ swizzle_b_row<P::kDual>(r)) << 4);
+  } else {
+    const int k = 8 * g + (li >> 2);
+    const uint32_t base = lds0 + kOperandBytes + (P::kDual ? 0 : (wn >> 1) * kHalfBytes) + k * 256;
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      const int chunk = P::kDual ? 4 * wn + (li & 3) : 8 * (wn & 1) + 2 * (li & 3) + v;
+      b_read[v] = base + (static_cast<uint32_t>(chunk ^ swizzle_b_k<P::kDual>(k)) << 4);
+    }
+  }
+  // fragment j (0..3; dual: gate 0, 1, up 2, 3) of k half h
+  auto read_b = [&](uint32_t stage, int j, int h) -> i4 {
+    if constexpr (P::kBKC) {
+      return read16(b_read[h] + stage + (P::kDual ? (j >> 1) * kHalfBytes + (j & 1) * 4 * kSliceBytes : j * 4 * kSliceBytes));
+    } else if constexpr (P::kDual) {
+      return read_columns(b_read[0] + stage + (j >> 1) * kHalfBytes + (j & 1) * 8 + h * 32 * 256);
+    } else {
+      return read_columns(b_read[j >> 1] + stage + (j & 1) * 8 + h * 32 * 256);
+    }
+  };
+
+  start_tile();
+  if (!open) return;
+  Tile tl = next;
+  load_b(0);
+  load_a(0);
+  load_b(1);
+  load_a(1);
+  wait_loads<8>();
+  phase_barrier();
+  i4 b0[2][2], b1[2][2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) b0[j][h] = read_b(0, j, h);
+  }
+  // the second half of the waves runs a phase behind
+  if (wm == 1) phase_barrier();
+  int step = 0;  // slices multiplied: the stage is step & 1
+  int round = 0;
+
+  auto run_tile = [&](auto mi) {
+    constexpr int MI = decltype(mi)::value;  // 16-row fragments of a wave
+    constexpr int MA = MI < 4 ? MI : 4;      // of them in one operand set
+    Acc acc[MI][4] = {};
+    const int wrow = wm * 16 * MI;
+    uint32_t a_read[P::kAKC ? 2 : MI];
+    if constexpr (P::kAKC) {
+      const uint32_t base = lds0 + (wrow + li) * kSliceBytes;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) a_read[h] = base + (static_cast<uint32_t>((4 * h + g) ^ (li & 7)) << 4);
+    } else {
+      const int k = 8 * g + (li >> 2);
+      const uint32_t base = lds0 + (wrow >> 7) * kHalfBytes + k * 256 + (li & 1) * 8;
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        const int chunk = ((wrow & 127) >> 3) + 2 * i + ((li & 3) >> 1);
+        a_read[i] = base + (static_cast<uint32_t>(chunk ^ swizzle_a_k(k)) << 4);
+      }
+    }
+    auto read_a = [&](uint32_t stage, int i, int h) -> i4 {
+      if constexpr (P::kAKC) {
+        return read16(a_read[h] + stage + i * 16 * kSliceBytes);
+      } else {
+        return read_columns(a_read[i] + stage + h * 32 * 256);
+      }
+    };
+    i4 a[MA][2];
+    auto fetch_a = [&](uint32_t stage, int i0) {
+#pragma unroll
+      for (int i = 0; i < MA; ++i) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) a[i][h] = read_a(stage, i0 + i, h);
+      }
+    };
+    auto fetch_b = [&](uint32_t stage, int j0, i4 (&b)[2][2]) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) b[j][h] = read_b(stage, j0 + j, h);
+      }
+    };
+    auto multiply = [&](int i0, int j0, const i4 (&b)[2][2]) {
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int i = 0; i < MA; ++i) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) acc[i0 + i][j0 + j] = M::mul(b[j][h], a[i][h], acc[i0 + i][j0 + j]);
+        }
+      }
+      __builtin_amdgcn_s_setprio(0);
+    };
+    // A slice takes four phases of a fetch and a product. Its B half of the stage is read
+    // by the end of the second fetch of the waves behind, its A half by the end of the
+    // third: the loads of slice + 2 into them are issued by the third and fourth fetch.
+    // At the end of each, the loads of the same operand of slice + 1, issued a slice ago,
+    // have landed but for the eight issued since.
+#pragma unroll 1
+    for (int kt = 0; kt < tl.slices; ++kt, ++step) {
+      const int st = step & 1;
+      const uint32_t stage = st * kStageBytes;
+      fetch_a(stage, 0);
+      wait_lds();
+      phase_barrier();
+      multiply(0, 0, b0);
+      phase_barrier();
+      fetch_b(stage, 2, b1);
+      wait_lds();
+      phase_barrier();
+      multiply(0, 2, b1);
+      phase_barrier();
+      if constexpr (MI == 8) fetch_a(stage, 4);
+      load_b(st);
+      wait_loads<8>();
+      wait_lds();
+      phase_barrier();
+      if constexpr (MI == 8) multiply(4, 0, b0);
+      phase_barrier();
+      fetch_b(stage ^ kStageBytes, 0, b0);  // of the next slice
+      load_a(st);
+      wait_loads<8>();
+      wait_lds();
+      phase_barrier();
+      if constexpr (MI == 8) multiply(4, 2, b1);
+      phase_barrier();
+    }
+    // lane: rows wrow + 16 i + li, 16 columns from 16 g (dual: 8 from 8 g) of the wave's
+    const std::size_t row0 = (P::kWeights ? static_cast<std::size_t>(tl.e) * prm.M : 0) + tl.row0;
+    const int n = tl.n0 + (P::kDual ? 32 * wn + 8 * g : 64 * wn + 16 * g);
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const int r = wrow + 16 * i + li;
+      if (r >= tl.rows) continue;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = static_cast<float>(acc[i][2 * c + (q >> 2)][q & 3]);
+        if constexpr (P::kDual) {
+          float u[8];
+#pragma unroll
+          for (int q = 0; q < 8; ++q) u[q] = static_cast<float>(acc[i][2 + (q >> 2)][q & 3]);
+          if (c == 0 && n < prm.N) P::Epi::template emit<8>(prm, tl.e, row0 + r, n, prm.N - n, v, u);
+        } else {
+          if (n + 8 * c < prm.N) P::Epi::template emit<8>(prm, tl.e, row0 + r, n + 8 * c, prm.N - n - 8 * c, v);
+        }
+      }
+    }
+  };
+
+#pragma unroll 1
+  for (;;) {
+    if (tl.rows > 128) {
+      run_tile(std::integral_constant<int, 8>{});
+    } else if (tl.rows > 64) {
+      run_tile(std::integral_constant<int, 4>{});
+    } else {
+      run_tile(std::integral_constant<int, 2>{});
+    }
+    round += grid;
+    if (!decode(round, tl)) break;
+  }
+  if (wm == 0) phase_barrier();
+  wait_loads<0>();  // (the stream's last loads bring nothing, but they write LDS)
+}
+
+int cu_count() {
+  static const int cus = [] {
+    int device = 0, count = 0;
+    if (hipGetDevice(&device) != hipSuccess ||
+        hipDeviceGetAttribute(&count, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || count <= 0) {
+      return 256;
+    }
+    return count;
+  }();
+  return cus;
+}
+
+template <class P>
+hipError_t launch(const Product& prm, hipStream_t stream) {
+  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(rr_expert_gemm_kernel<P>),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+  if (attr != hipSuccess) return attr;
+  const long cols = (prm.N + P::kCols - 1) / P::kCols;
+  const long rows = P::kWeights ? static_cast<long>(prm.experts) * ((prm.M + kTileRows - 1) / kTileRows)
+                                : prm.rows / kTileRows + std::min<long>(prm.experts, prm.rows);
+  long grid = std::min<long>(cols * rows, cu_count());
+  if (grid >= kXcds) grid = grid / kXcds * kXcds;
+  const std::size_t lds = 2 * kStageBytes + 3 * static_cast<std::size_t>(prm.experts + 1) * sizeof(int32_t);
+  rr_expert_gemm_kernel<P><<<dim3(static_cast<unsigned>(grid)), kThreads, lds, stream>>>(prm);
+  return hipGetLastError();
+}
+
+template <typename T>
+using GateUp = Kind<T, true, false, false, EpiGate<T>>;  // x [Wg | Wu]
+template <typename T>
+using Down = Kind<T, true, false, false, EpiStore<T>>;  // a Wd
+template <typename T>
+using DGateUp = Kind<T, true, true, false, EpiDGate<T>>;  // dy Wd^T
+template <typename T>
+using Dx = Kind<T, true, true, false, EpiStore<T>>;  // dg Wg^T + du Wu^T
+template <typename T>
+using DwPair = Kind<T, false, false, true, EpiPair<T>>;  // x^T [dg | du]
+template <typename T>
+using Dw = Kind<T, false, false, true, EpiStore<T>>;  // a^T dy
+
+// 16-byte loads need every row of every operand on a 16-byte boundary.
+bool aligned16(std::initializer_list<const void*> pointers) {
+  for (const void* p : pointers) {
+    if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return false;
+  }
+  return true;
+}
+
+Product base_of(const FfnParams& f) {
+  Product p{};
+  p.offsets = f.offsets;
+  p.experts = f.experts;
+  p.rows = f.rows;
+  p.activation = f.activation;
+  return p;
+}
+
+template <typename T>
+hipError_t forward(const FfnParams& f, hipStream_t stream) {
+  Product p = base_of(f);
+  p.a = f.x;
+  p.b = f.w_gate;
+  p.b_up = f.w_up;
+  p.out = f.gate;
+  p.out_up = f.up;
+  p.out_act = f.act;
+  p.N = f.inner;
+  p.K = f.hidden;
+  p.lda = f.hidden;
+  p.ldb = f.inner;
+  hipError_t error = launch<GateUp<T>>(p, stream);
+  if (error != hipSuccess) return error;
+  p = base_of(f);
+  p.a = f.act;
+  p.b = f.w_down;
+  p.out = f.y;
+  p.out_f32 = f.y_f32;
+  p.N = f.output;
+  p.K = f.inner;
+  p.lda = f.inner;
+  p.ldb = f.output;
+  return launch<Down<T>>(p, stream);
+}
+
+template <typename T>
+hipError_t backward(const FfnParams& f, hipStream_t stream) {
+  hipError_t error = hipSuccess;
+  if (f.rows != 0) {
+    Product p = base_of(f);
+    p.a = f.dy;
+    p.b = f.w_down;
+    p.in = f.gate;
+    p.in_up = f.up;
+    p.out = f.d_gate;
+    p.out_up = f.d_up;
+    p.N = f.inner;
+    p.K = f.output;
+    p.lda = p.ldb = f.output;
+    error = launch<DGateUp<T>>(p, stream);
+  }
+  if (error == hipSuccess && f.rows != 0 && f.dx != nullptr) {
+    Product p = base_of(f);
+    p.a = f.d_gate;
+    p.a2 = f.d_up;
+    p.b = f.w_gate;
+    p.b_up = f.w_up;
+    p.out = f.dx;
+    p.N = f.hidden;
+    p.K = f.inner;
+    p.lda = p.ldb = f.inner;
+    error = launch<Dx<T>>(p, stream);
+  }
+  if (error == hipSuccess && f.dw_gate != nullptr) {
+    Product p = base_of(f);
+    p.a = f.x;
+    p.b = f.d_gate;
+    p.b_up = f.d_up;
+    p.out = f.dw_gate;
+    p.out_up = f.dw_up;
+    p.M = f.hidden;
+    p.N = f.inner;
+    p.lda = f.hidden;
+    p.ldb = f.inner;
+    error = launch<DwPair<T>>(p, stream);
+  }
+  if (error == hipSuccess && f.dw_down != nullptr) {
+    Product p = base_of(f);
+    p.a = f.act;
+    p.b = f.dy;
+    p.out = f.dw_down;
+    p.M = f.inner;
+    p.N = f.output;
+    p.lda = f.inner;
+    p.ldb = f.output;
+    error = launch<Dw<T>>(p, stream);
+  }
+  return error;
+}
+
+template <typename T>
+hipError_t int8_product(const Int8Params& f, hipStream_t stream) {
+  Product p{};
+  p.offsets = f.offsets;
+  p.experts = f.experts;
+  p.rows = f.rows;
+  p.activation = f.activation;
+  p.a = f.q;
+  p.a2 = f.q_scale;
+  p.b = f.w;
+  p.b_up = f.w_up;
+  p.in = f.w_scale;
+  p.in_up = f.w_up_scale;
+  p.out = f.y;
+  p.N = f.output;
+  p.K = f.hidden;
+  p.lda = p.ldb = f.hidden;
+  return f.w_up != nullptr ? launch<Kind<int8_t, true, true, false, EpiInt8Gate<T>>>(p, stream)
+                           : launch<Kind<int8_t, true, true, false, EpiInt8<T>>>(p, stream);
+}
+
+}  // namespace
+
+hipError_t gated_ffn(const FfnParams& f, hipStream_t stream) {
+  if (f.hidden % 8 != 0 || f.inner % 8 != 0 || f.output % 8 != 0 || !aligned16({f.x, f.w_gate, f.w_up, f.w_down, f.act})) {
+    return gated_ffn_naive(f, stream);
+  }
+  return f.bf16 ? forward<bf16>(f, stream) : forward<f16>(f, stream);
+}
+
+hipError_t gated_ffn_backward(const FfnParams& f, hipStream_t stream) {
+  if (f.hidden % 8 != 0 || f.inner % 8 != 0 || f.output % 8 != 0 ||
+      !aligned16({f.x, f.w_gate, f.w_up, f.w_down, f.act, f.dy, f.d_gate, f.d_up})) {
+    return gated_ffn_backward_naive(f, stream);
+  }
+  return f.bf16 ? backward<bf16>(f, stream) : backward<f16>(f, stream);
+}
+
+hipError_t int8_grouped_gemm(const Int8Params& f, hipStream_t stream) {
+  if (f.hidden % 16 != 0 || !aligned16({f.q, f.w, f.w_up})) return int8_grouped_gemm_naive(f, stream);
+  if (f.dtype == RR_DTYPE_FP32) return int8_product<float>(f, stream);
+  return f.dtype == RR_DTYPE_BF16 ? int8_product<bf16>(f, stream) : int8_product<f16>(f, stream);
+}
+
+}  // namespace rr::kern
