@@ -19,8 +19,8 @@
 //    operand, so that gate and up of an element meet in one lane). The right operand is
 //    the instruction's first one and its columns are dealt so that a lane ends with 16 (8
 //    and 8) adjacent columns of a row: wide stores, no exchange.
-//  - The waves of wm = 0 and wm = 1 share the SIMDs pairwise and run a phase apart: while
-//    one reads its operands and issues loads, the other has the matrix pipe.
+//  - A wave fetches the operands of its next 16 products while it issues the present
+//    ones; the workgroup meets once a slice.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -109,7 +109,7 @@ __device__ __forceinline__ int swizzle_b_k(int k) {
 // Barriers and waits of the pipeline. The loads into LDS are written in assembly: they
 // have no register results, and the compiler, which would wait for all of them before
 // any LDS read, does not see them; every wait for them is one of these.
-__device__ __forceinline__ void phase_barrier() {
+__device__ __forceinline__ void wave_barrier() {
   __builtin_amdgcn_sched_barrier(0);
   asm volatile("s_barrier" ::: "memory");
   __builtin_amdgcn_sched_barrier(0);
@@ -290,21 +290,24 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
   };
   auto records = [](int64_t left) { return static_cast<int>(left <= 0 ? 0 : left < 0x7FFFFFFF ? left : 0x7FFFFFFF); };
   auto cut = [&](uint32_t offset, uint32_t chunk) { return static_cast<int>(chunk) < k_left ? offset : kPast; };
-  auto load_b = [&](int stage) {
+  // loads [q0, q1) of the wave's four of the slice
+  auto load_b = [&](int stage, int q0, int q1) {
     const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(b_at), 0, records(b_left), kBufferFlags);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = q0; q < q1; ++q) {
       const uint32_t at = P::kBKC ? cut(b_lane[q], b_chunk[(q >> b_bit) & 1]) : b_lane[q];
       load_to_lds(rsrc, at, to_b + stage * kStageBytes + q * 1024);
     }
   };
-  auto load_a = [&](int stage) {  // and on to the next slice
+  auto load_a = [&](int stage, int q0, int q1) {
     const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(a_at), 0, records(a_left), kBufferFlags);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = q0; q < q1; ++q) {
       const uint32_t at = P::kAKC ? cut(a_lane[q], a_chunk) : a_lane[q];
       load_to_lds(rsrc, at, to_a + stage * kStageBytes + q * 1024);
     }
+  };
+  auto advance = [&]() {  // to the next slice
     if (!open) return;
     a_at += a_slice;
     a_left -= a_slice;
@@ -350,26 +353,21 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
   start_tile();
   if (!open) return;
   Tile tl = next;
-  load_b(0);
-  load_a(0);
-  load_b(1);
-  load_a(1);
+  load_a(0, 0, 4);
+  load_b(0, 0, 4);
+  advance();
+  load_a(1, 0, 4);
+  load_b(1, 0, 4);
+  advance();
   wait_loads<8>();
-  phase_barrier();
-  i4 b0[2][2], b1[2][2];
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) b0[j][h] = read_b(0, j, h);
-  }
-  // the second half of the waves runs a phase behind
-  if (wm == 1) phase_barrier();
+  wave_barrier();
   int step = 0;  // slices multiplied: the stage is step & 1
   int round = 0;
 
   auto run_tile = [&](auto mi) {
     constexpr int MI = decltype(mi)::value;  // 16-row fragments of a wave
-    constexpr int MA = MI < 4 ? MI : 4;      // of them in one operand set
+    constexpr int MA = MI < 4 ? MI : 4;      // of them in a phase
+    constexpr int PH = 2 * MI / MA;          // phases of a slice: k half p / (PH / 2), fragments from MA (p % (PH / 2))
     Acc acc[MI][4] = {};
     const int wrow = wm * 16 * MI;
     uint32_t a_read[P::kAKC ? 2 : MI];
@@ -393,66 +391,58 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
         return read_columns(a_read[i] + stage + h * 32 * 256);
       }
     };
-    i4 a[MA][2];
-    auto fetch_a = [&](uint32_t stage, int i0) {
+    i4 a[2][MA], b[2][4];  // of this phase and the next, of both k halves
+    // the operands of phase p, in two parts
+    auto fetch = [&](uint32_t stage, int p, int part) {
+      const int h = p / (PH / 2), i0 = MA * (p % (PH / 2));
+      if (p % (PH / 2) == 0) {
 #pragma unroll
-      for (int i = 0; i < MA; ++i) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) a[i][h] = read_a(stage, i0 + i, h);
+        for (int j = 2 * part; j < 2 * part + 2; ++j) b[h][j] = read_b(stage, j, h);
       }
+#pragma unroll
+      for (int i = part * (MA / 2); i < (part + 1) * (MA / 2); ++i) a[p & 1][i] = read_a(stage, i0 + i, h);
     };
-    auto fetch_b = [&](uint32_t stage, int j0, i4 (&b)[2][2]) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) b[j][h] = read_b(stage, j0 + j, h);
-      }
-    };
-    auto multiply = [&](int i0, int j0, const i4 (&b)[2][2]) {
-      __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int i = 0; i < MA; ++i) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) acc[i0 + i][j0 + j] = M::mul(b[j][h], a[i][h], acc[i0 + i][j0 + j]);
-        }
-      }
-      __builtin_amdgcn_s_setprio(0);
-    };
-    // A slice takes four phases of a fetch and a product. Its B half of the stage is read
-    // by the end of the second fetch of the waves behind, its A half by the end of the
-    // third: the loads of slice + 2 into them are issued by the third and fourth fetch.
-    // At the end of each, the loads of the same operand of slice + 1, issued a slice ago,
-    // have landed but for the eight issued since.
+    uint32_t stage = (step & 1) * kStageBytes;
+    fetch(stage, 0, 0);
+    fetch(stage, 0, 1);
+    // A slice takes PH phases of MA x 4 products, each under the fetch of the next one's
+    // operands. Before its last phase the slice has been read whole by every wave and the
+    // next slice, loaded since that point of the slice before, has landed: one barrier,
+    // then the next slice's operands are fetched and the slice after it is loaded into
+    // the stage that came free.
 #pragma unroll 1
     for (int kt = 0; kt < tl.slices; ++kt, ++step) {
+      const bool last = kt + 1 == tl.slices;  // (the next tile fetches its own operands)
       const int st = step & 1;
-      const uint32_t stage = st * kStageBytes;
-      fetch_a(stage, 0);
-      wait_lds();
-      phase_barrier();
-      multiply(0, 0, b0);
-      phase_barrier();
-      fetch_b(stage, 2, b1);
-      wait_lds();
-      phase_barrier();
-      multiply(0, 2, b1);
-      phase_barrier();
-      if constexpr (MI == 8) fetch_a(stage, 4);
-      load_b(st);
-      wait_loads<8>();
-      wait_lds();
-      phase_barrier();
-      if constexpr (MI == 8) multiply(4, 0, b0);
-      phase_barrier();
-      fetch_b(stage ^ kStageBytes, 0, b0);  // of the next slice
-      load_a(st);
-      wait_loads<8>();
-      wait_lds();
-      phase_barrier();
-      if constexpr (MI == 8) multiply(4, 2, b1);
-      phase_barrier();
+#pragma unroll
+      for (int p = 0; p < PH; ++p) {
+        const int h = p / (PH / 2), i0 = MA * (p % (PH / 2));
+        if (p == PH - 1) {
+          wait_lds();
+          wait_loads<0>();
+          wave_barrier();
+          stage ^= kStageBytes;
+        }
+#pragma unroll
+        for (int i = 0; i < MA; ++i) {
+          if (i < 2) {
+            if (p < PH - 1) {
+              fetch(stage, p + 1, i);
+            } else if (!last) {
+              fetch(stage, 0, i);
+            }
+          }
+          if (p == PH - 1) {
+            load_a(st, i * 4 / MA, (i + 1) * 4 / MA);
+            load_b(st, i * 4 / MA, (i + 1) * 4 / MA);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i0 + i][j] = M::mul(b[h][j], a[p & 1][i], acc[i0 + i][j]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      advance();
     }
     // lane: rows wrow + 16 i + li, 16 columns from 16 g (dual: 8 from 8 g) of the wave's
     const std::size_t row0 = (P::kWeights ? static_cast<std::size_t>(tl.e) * prm.M : 0) + tl.row0;
@@ -490,7 +480,6 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
     round += grid;
     if (!decode(round, tl)) break;
   }
-  if (wm == 0) phase_barrier();
   wait_loads<0>();  // (the stream's last loads bring nothing, but they write LDS)
 }
 
