@@ -46,10 +46,9 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 
 constexpr int kBufferFlags = 0x00027000;  // raw 32-bit buffer
 constexpr uint32_t kPast = 0x80000000U;   // an offset past every record count
-constexpr int kTileRows = 256;
 constexpr int kTileCols = 256;
 constexpr int kSliceBytes = 128;              // of every row
-constexpr int kOperandBytes = 256 * kSliceBytes;  // one operand's slice
+constexpr int kOperandBytes = 256 * kSliceBytes;  // one operand's slice (A of 128-row tiles fills half)
 constexpr int kHalfBytes = kOperandBytes / 2;
 constexpr int kStageBytes = 2 * kOperandBytes;
 constexpr int kThreads = 512;
@@ -81,12 +80,13 @@ struct Matrix<int8_t> {
 };
 
 // A kernel: element type, whether A and B have k along rows (KC), weight gradients or row
-// products, epilogue.
-template <typename T_, bool A_KC, bool B_KC, bool WEIGHTS, class Epi_>
+// products, epilogue, and how slices come: DIRECT into LDS, or through registers.
+template <typename T_, bool A_KC, bool B_KC, bool WEIGHTS, class Epi_, bool DIRECT>
 struct Kind {
   using T = T_;
   using Epi = Epi_;
-  static constexpr bool kAKC = A_KC, kBKC = B_KC, kWeights = WEIGHTS, kDual = Epi_::kDual;
+  static constexpr bool kAKC = A_KC, kBKC = B_KC, kWeights = WEIGHTS, kDual = Epi_::kDual, kDirect = DIRECT;
+  static constexpr int kTileRows = DIRECT ? 256 : 128;
   static constexpr int kSlice = kSliceBytes / sizeof(T_);  // k of a slice
   static constexpr int kCols = kDual ? kTileCols / 2 : kTileCols;
   static_assert(A_KC || sizeof(T_) == 2, "transposing reads are 16-bit");
@@ -120,9 +120,18 @@ __device__ __forceinline__ void wait_loads() {
 }
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-// 64 lanes x 16 bytes from `rsrc` (a byte offset per lane) to LDS at `to`.
-__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t rsrc, uint32_t offset, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(rsrc)
+// A raw buffer from `at` to `left` bytes further (uniform).
+__device__ __forceinline__ i4 make_buffer(const char* at, int64_t left) {
+  const int64_t p = reinterpret_cast<int64_t>(at);
+  const int records = static_cast<int>(left <= 0 ? 0 : left < 0x7FFFFFFF ? left : 0x7FFFFFFF);
+  return i4{__builtin_amdgcn_readfirstlane(static_cast<int>(p)), __builtin_amdgcn_readfirstlane(static_cast<int>(p >> 32) & 0xFFFF),
+            __builtin_amdgcn_readfirstlane(records), kBufferFlags};
+}
+// 64 lanes x 16 bytes from `buffer` (a byte offset per lane) to LDS at `to` (uniform).
+__device__ __forceinline__ void load_to_lds(i4 buffer, uint32_t offset, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(
+                   __builtin_amdgcn_readfirstlane(static_cast<int>(to))),
+               "v"(offset), "s"(buffer)
                : "memory");
 }
 
@@ -166,11 +175,11 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
   for (int e = tid; e <= experts; e += kThreads) s_off[e] = rr::dev::offset_at(prm.offsets, e, prm.rows);
   __syncthreads();
   if constexpr (!P::kWeights) {
-    if (wave == 0) build_tile_prefix<kTileRows, true>(s_off, s_pre, s_pre2, experts, lane);
+    if (wave == 0) build_tile_prefix<P::kTileRows, true>(s_off, s_pre, s_pre2, experts, lane);
     __syncthreads();
   }
   const int col_tiles = (prm.N + P::kCols - 1) / P::kCols;
-  const int m_tiles = P::kWeights ? (prm.M + kTileRows - 1) / kTileRows : 0;
+  const int m_tiles = P::kWeights ? (prm.M + P::kTileRows - 1) / P::kTileRows : 0;
   const int full_rows = P::kWeights ? 0 : __builtin_amdgcn_readfirstlane(s_pre[experts]);
   const int short_rows = P::kWeights ? 0 : __builtin_amdgcn_readfirstlane(s_pre2[experts]);
   const int total_full = full_rows * col_tiles;
@@ -180,20 +189,29 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
   const int part_slices = P::kWeights ? 0 : (prm.K + P::kSlice - 1) / P::kSlice;
   const int parts = P::kWeights || prm.a2 == nullptr || S == 1 ? 1 : 2;
 
-  // the workgroup's tile of a round (the last, partial round goes to the workgroups in
-  // dispatch order, over all XCDs); false past the last
+  // The workgroup's tile of a round; false where there is none. The last, partial round
+  // goes to the workgroups in dispatch order, over all XCDs; its tiles are cut into two or
+  // four by their rows where that many workgroups are left (8192 rows of eight experts, K =
+  // 28672, N = 4096: 2.25 rounds).
   auto decode = [&](int dealt, Tile& tl) {
-    const int mine = total - dealt >= grid ? worker : static_cast<int>(blockIdx.x);
-    const int t = dealt + mine;
-    if (t >= total) return false;
+    const int left = total - dealt;
+    if (left <= 0) return false;
+    int t = dealt + worker, sub = 0, span = P::kTileRows;
+    if (left < grid) {
+      const int cuts = P::kDirect && 4 * left <= grid ? 4 : 2 * left <= grid ? 2 : 1;
+      sub = static_cast<int>(blockIdx.x) / left;
+      if (sub >= cuts) return false;
+      t = dealt + static_cast<int>(blockIdx.x) - sub * left;
+      span = P::kTileRows / cuts;
+    }
     int rt, ct;
     if constexpr (P::kWeights) {
       tl.e = t / (m_tiles * col_tiles);
       decode_tile(t - tl.e * m_tiles * col_tiles, m_tiles, col_tiles, &rt, &ct);
       tl.first = __builtin_amdgcn_readfirstlane(s_off[tl.e]);
       const int count = __builtin_amdgcn_readfirstlane(s_off[tl.e + 1]) - tl.first;
-      tl.row0 = rt * kTileRows;
-      tl.rows = min(prm.M - tl.row0, kTileRows);
+      tl.row0 = rt * P::kTileRows;
+      tl.rows = min(prm.M - tl.row0, P::kTileRows);
       // (an expert without rows takes one slice of zeros)
       tl.slices = count > P::kSlice ? (count + P::kSlice - 1) / P::kSlice : 1;
     } else {
@@ -203,49 +221,52 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
       tl.first = __builtin_amdgcn_readfirstlane(s_off[tl.e]);
       const int end = __builtin_amdgcn_readfirstlane(s_off[tl.e + 1]);
       tl.row0 = tl.first +
-                (is_short ? (end - tl.first) / kTileRows : rt - __builtin_amdgcn_readfirstlane(s_pre[tl.e])) * kTileRows;
-      tl.rows = min(end - tl.row0, kTileRows);
+                (is_short ? (end - tl.first) / P::kTileRows : rt - __builtin_amdgcn_readfirstlane(s_pre[tl.e])) * P::kTileRows;
+      tl.rows = min(end - tl.row0, P::kTileRows);
       tl.slices = part_slices * parts;
     }
     tl.n0 = ct * P::kCols;
-    return true;
+    tl.row0 += sub * span;
+    tl.rows = min(tl.rows - sub * span, span);
+    return tl.rows > 0;
   };
 
   // ---- the stream of slices into LDS ----
   // Wave w brings rows 32 w .. + 31 (KC) or k rows 16 (w % 4) .. + 15 of half w / 4 (KS) of
   // each operand in four loads; half w / 4 is the columns (of KS A: rows of the result)
-  // from 128 on, or in a dual product the right operand b_up.
+  // from 128 on, or in a dual product the right operand b_up. A of a 128-row tile is one
+  // half, brought by all waves in two loads.
+  constexpr int QA = P::kTileRows / 64;  // loads of A
   const int half = wave >> 2;
+  const int a_half = P::kTileRows == 256 ? half : 0;
+  const int a_share = P::kTileRows == 256 ? wn : wave;  // among the waves of a half
   // (lane offsets carry everything that varies: a range check must see the whole offset)
-  uint32_t a_lane[4], b_lane[4], a_chunk = 0, b_chunk[2] = {};
+  uint32_t a_lane[QA], b_lane[4], a_chunk = 0, b_chunk[2] = {};
   constexpr int b_bit = P::kDual ? 0 : 1;  // the bit of q that B's chunk depends on (KC)
+  auto a_row = [&](int q) {  // KC: row, KS: k
+    return P::kAKC ? 8 * QA * wave + 8 * q + (lane >> 3) : 4 * QA * a_share + 4 * q + (lane >> 4);
+  };
+  auto b_row = [&](int q) { return P::kBKC ? 32 * wn + 8 * q + (lane >> 3) : 16 * wn + 4 * q + (lane >> 4); };
+#pragma unroll
+  for (int q = 0; q < QA; ++q) {
+    const int r = a_row(q);
+    const uint32_t chunk = static_cast<uint32_t>(P::kAKC ? (lane & 7) ^ (r & 7) : (lane & 15) ^ swizzle_a_k(r)) << 4;
+    if (P::kAKC) a_chunk = chunk;
+    a_lane[q] = static_cast<uint32_t>(r) * static_cast<uint32_t>(prm.lda) * S + chunk;
+  }
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    if constexpr (P::kAKC) {
-      const int r = 32 * wave + 8 * q + (lane >> 3);
-      a_chunk = static_cast<uint32_t>((lane & 7) ^ (r & 7)) << 4;
-      a_lane[q] = static_cast<uint32_t>(r) * static_cast<uint32_t>(prm.lda) * S + a_chunk;
-    } else {
-      const int k = 16 * wn + 4 * q + (lane >> 4);
-      a_lane[q] = static_cast<uint32_t>(k) * static_cast<uint32_t>(prm.lda) * S +
-                  (static_cast<uint32_t>((lane & 15) ^ swizzle_a_k(k)) << 4);
-    }
-    if constexpr (P::kBKC) {
-      const int r = 32 * wn + 8 * q + (lane >> 3);
-      const uint32_t chunk = static_cast<uint32_t>((lane & 7) ^ swizzle_b_row<P::kDual>(r)) << 4;
-      b_chunk[(q >> b_bit) & 1] = chunk;
-      b_lane[q] = static_cast<uint32_t>(r) * static_cast<uint32_t>(prm.ldb) * S + chunk;
-    } else {
-      const int k = 16 * wn + 4 * q + (lane >> 4);
-      b_lane[q] = static_cast<uint32_t>(k) * static_cast<uint32_t>(prm.ldb) * S +
-                  (static_cast<uint32_t>((lane & 15) ^ swizzle_b_k<P::kDual>(k)) << 4);
-    }
+    const int r = b_row(q);
+    const uint32_t chunk = static_cast<uint32_t>(P::kBKC ? (lane & 7) ^ swizzle_b_row<P::kDual>(r)
+                                                         : (lane & 15) ^ swizzle_b_k<P::kDual>(r)) << 4;
+    if (P::kBKC) b_chunk[(q >> b_bit) & 1] = chunk;
+    b_lane[q] = static_cast<uint32_t>(r) * static_cast<uint32_t>(prm.ldb) * S + chunk;
   }
   // bytes between slices
   const int64_t a_slice = P::kAKC ? kSliceBytes : static_cast<int64_t>(P::kSlice) * prm.lda * S;
   const int64_t b_slice = P::kBKC ? kSliceBytes : static_cast<int64_t>(P::kSlice) * prm.ldb * S;
-  const uint32_t to_a = lds0 + wave * (kOperandBytes / 8);
-  const uint32_t to_b = to_a + kOperandBytes;
+  const uint32_t to_a = lds0 + wave * (QA * 1024);
+  const uint32_t to_b = lds0 + kOperandBytes + wave * 4096;
 
   Tile next;               // the tile whose slices are being loaded
   int dealt = 0;           // its round
@@ -254,6 +275,8 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
   const char *a_at, *b_at;  // the slice of each operand, and the bytes to the operand's end from there
   int64_t a_left, b_left;
   int k_left;  // bytes of a row's sum from the slice on
+  // through registers: rows (k rows) of each operand from the slice on, and bytes of them from its first column
+  int a_rows = 0, b_rows = 0, a_width = 0, b_width = 0;
   auto start_part = [&](int part) {
     const char* a = static_cast<const char*>(part == 0 ? prm.a : prm.a2);
     const char* b = static_cast<const char*>(P::kDual ? (half == 0 ? prm.b : prm.b_up) : part == 0 ? prm.b : prm.b_up);
@@ -261,11 +284,14 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
     if constexpr (P::kWeights) {
       const int count = s_off[next.e + 1] - next.first;
       const int64_t rows = __builtin_amdgcn_readfirstlane(count > 0 ? count : 0);
-      const int m = next.row0 + half * 128;
+      const int m = next.row0 + a_half * 128;
       a_at = a + (static_cast<int64_t>(next.first) * prm.lda + m) * S;
       a_left = m < prm.M ? (rows * prm.lda - m) * S : 0;
       b_at = b + (static_cast<int64_t>(next.first) * prm.ldb + n) * S;
       b_left = n < prm.N ? (rows * prm.ldb - n) * S : 0;
+      a_rows = b_rows = static_cast<int>(rows);
+      a_width = (prm.M - m) * S;
+      b_width = (prm.N - n) * S;
     } else {
       a_at = a + static_cast<int64_t>(next.row0) * prm.lda * S;
       a_left = static_cast<int64_t>(next.rows) * prm.lda * S;
@@ -277,6 +303,10 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
         b_left = n < prm.N ? (static_cast<int64_t>(prm.K) * prm.ldb - n) * S : 0;
       }
       k_left = prm.K * S;
+      a_rows = next.rows;
+      a_width = k_left;
+      b_rows = P::kBKC ? prm.N - n : prm.K;
+      b_width = P::kBKC ? k_left : (prm.N - n) * S;
     }
   };
   auto start_tile = [&]() {
@@ -286,26 +316,52 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
       start_part(0);
     } else {
       a_left = b_left = 0;
+      a_rows = b_rows = 0;
     }
   };
-  auto records = [](int64_t left) { return static_cast<int>(left <= 0 ? 0 : left < 0x7FFFFFFF ? left : 0x7FFFFFFF); };
   auto cut = [&](uint32_t offset, uint32_t chunk) { return static_cast<int>(chunk) < k_left ? offset : kPast; };
-  // loads [q0, q1) of the wave's four of the slice
-  auto load_b = [&](int stage, int q0, int q1) {
-    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(b_at), 0, records(b_left), kBufferFlags);
+  // The wave's load q of each operand's slice. Direct: into the stage. Through registers:
+  // `put` writes what the last `load` of the same q brought, 16 bytes of any alignment;
+  // chunks that a row's or the operand's end cuts are read element by element.
+  i4 a_held[P::kDirect ? 1 : QA], b_held[P::kDirect ? 1 : 4];
+  // 16 bytes at `at` + offset, of which the first `bytes` exist
+  auto read_cut = [&](const char* at, uint32_t offset, int bytes) -> i4 {
+    typedef T chunk __attribute__((ext_vector_type(16 / S), aligned(S)));
+    chunk v = {};
+    if (bytes >= 16) {
+      v = *reinterpret_cast<const chunk*>(at + offset);
+    } else {
 #pragma unroll
-    for (int q = q0; q < q1; ++q) {
-      const uint32_t at = P::kBKC ? cut(b_lane[q], b_chunk[(q >> b_bit) & 1]) : b_lane[q];
-      load_to_lds(rsrc, at, to_b + stage * kStageBytes + q * 1024);
+      for (int i = 0; i < 16 / S; ++i) {
+        if (i * S < bytes) v[i] = *reinterpret_cast<const T*>(at + offset + i * S);
+      }
+    }
+    return __builtin_bit_cast(i4, v);
+  };
+  auto load_a = [&](int stage, int q) {
+    if constexpr (P::kDirect) {
+      load_to_lds(make_buffer(a_at, a_left), P::kAKC ? cut(a_lane[q], a_chunk) : a_lane[q], to_a + stage * kStageBytes + q * 1024);
+    } else {
+      const int r = a_row(q);
+      const int at = static_cast<int>(a_lane[q] - static_cast<uint32_t>(r) * static_cast<uint32_t>(prm.lda) * S);  // chunk
+      a_held[q] = read_cut(a_at, a_lane[q], r < a_rows ? a_width - at : 0);
     }
   };
-  auto load_a = [&](int stage, int q0, int q1) {
-    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(a_at), 0, records(a_left), kBufferFlags);
-#pragma unroll
-    for (int q = q0; q < q1; ++q) {
-      const uint32_t at = P::kAKC ? cut(a_lane[q], a_chunk) : a_lane[q];
-      load_to_lds(rsrc, at, to_a + stage * kStageBytes + q * 1024);
+  auto load_b = [&](int stage, int q) {
+    if constexpr (P::kDirect) {
+      load_to_lds(make_buffer(b_at, b_left), P::kBKC ? cut(b_lane[q], b_chunk[(q >> b_bit) & 1]) : b_lane[q],
+                  to_b + stage * kStageBytes + q * 1024);
+    } else {
+      const int r = b_row(q);
+      const int at = static_cast<int>(b_lane[q] - static_cast<uint32_t>(r) * static_cast<uint32_t>(prm.ldb) * S);
+      b_held[q] = read_cut(b_at, b_lane[q], r < b_rows ? b_width - at : 0);
     }
+  };
+  auto put_a = [&](int stage, int q) {
+    if constexpr (!P::kDirect) *reinterpret_cast<RR_LDS i4*>(to_a + stage * kStageBytes + q * 1024 + lane * 16) = a_held[q];
+  };
+  auto put_b = [&](int stage, int q) {
+    if constexpr (!P::kDirect) *reinterpret_cast<RR_LDS i4*>(to_b + stage * kStageBytes + q * 1024 + lane * 16) = b_held[q];
   };
   auto advance = [&]() {  // to the next slice
     if (!open) return;
@@ -314,6 +370,8 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
     b_at += b_slice;
     b_left -= b_slice;
     k_left -= kSliceBytes;
+    if (P::kAKC) a_width -= kSliceBytes; else a_rows -= P::kSlice;
+    if (P::kBKC) b_width -= kSliceBytes; else b_rows -= P::kSlice;
     ++slice;
     if (slice == next.slices) {
       dealt += grid;
@@ -353,13 +411,31 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
   start_tile();
   if (!open) return;
   Tile tl = next;
-  load_a(0, 0, 4);
-  load_b(0, 0, 4);
-  advance();
-  load_a(1, 0, 4);
-  load_b(1, 0, 4);
-  advance();
-  wait_loads<8>();
+#pragma unroll
+  for (int st = 0; st < 2; ++st) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (q < QA) load_a(st, q);
+      load_b(st, q);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (q < QA) put_a(st, q);
+      put_b(st, q);
+    }
+    advance();
+  }
+  if constexpr (P::kDirect) {
+    wait_loads<8>();
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {  // (the third slice, on its way)
+      if (q < QA) load_a(0, q);
+      load_b(0, q);
+    }
+    advance();
+    wait_lds();
+  }
   wave_barrier();
   int step = 0;  // slices multiplied: the stage is step & 1
   int round = 0;
@@ -419,7 +495,7 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
         const int h = p / (PH / 2), i0 = MA * (p % (PH / 2));
         if (p == PH - 1) {
           wait_lds();
-          wait_loads<0>();
+          if constexpr (P::kDirect) wait_loads<0>();
           wave_barrier();
           stage ^= kStageBytes;
         }
@@ -433,8 +509,13 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
             }
           }
           if (p == PH - 1) {
-            load_a(st, i * 4 / MA, (i + 1) * 4 / MA);
-            load_b(st, i * 4 / MA, (i + 1) * 4 / MA);
+#pragma unroll
+            for (int q = i * 4 / MA; q < (i + 1) * 4 / MA; ++q) {
+              if (q < QA) put_a(st, q);
+              put_b(st, q);
+              if (q < QA) load_a(st, q);
+              load_b(st, q);
+            }
           }
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -447,22 +528,28 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
     // lane: rows wrow + 16 i + li, 16 columns from 16 g (dual: 8 from 8 g) of the wave's
     const std::size_t row0 = (P::kWeights ? static_cast<std::size_t>(tl.e) * prm.M : 0) + tl.row0;
     const int n = tl.n0 + (P::kDual ? 32 * wn + 8 * g : 64 * wn + 16 * g);
+    auto whole = [&](int col) { return S == 2 && P::kDirect ? 8 : prm.N - col; };  // (widths of 16-bit direct products are whole eights)
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
       const int r = wrow + 16 * i + li;
       if (r >= tl.rows) continue;
+      if constexpr (P::kDual) {
+        if (n >= prm.N) continue;
+        float v[8], u[8];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float v[8];
+        for (int q = 0; q < 8; ++q) {
+          v[q] = static_cast<float>(acc[i][q >> 2][q & 3]);
+          u[q] = static_cast<float>(acc[i][2 + (q >> 2)][q & 3]);
+        }
+        P::Epi::template emit<8>(prm, tl.e, row0 + r, n, whole(n), v, u);
+      } else {
 #pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] = static_cast<float>(acc[i][2 * c + (q >> 2)][q & 3]);
-        if constexpr (P::kDual) {
-          float u[8];
+        for (int c = 0; c < 2; ++c) {
+          if (n + 8 * c >= prm.N) continue;
+          float v[8];
 #pragma unroll
-          for (int q = 0; q < 8; ++q) u[q] = static_cast<float>(acc[i][2 + (q >> 2)][q & 3]);
-          if (c == 0 && n < prm.N) P::Epi::template emit<8>(prm, tl.e, row0 + r, n, prm.N - n, v, u);
-        } else {
-          if (n + 8 * c < prm.N) P::Epi::template emit<8>(prm, tl.e, row0 + r, n + 8 * c, prm.N - n - 8 * c, v);
+          for (int q = 0; q < 8; ++q) v[q] = static_cast<float>(acc[i][2 * c + (q >> 2)][q & 3]);
+          P::Epi::template emit<8>(prm, tl.e, row0 + r, n + 8 * c, whole(n + 8 * c), v);
         }
       }
     }
@@ -470,8 +557,8 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
 
 #pragma unroll 1
   for (;;) {
-    if (tl.rows > 128) {
-      run_tile(std::integral_constant<int, 8>{});
+    if (P::kDirect && tl.rows > 128) {
+      if constexpr (P::kDirect) run_tile(std::integral_constant<int, 8>{});
     } else if (tl.rows > 64) {
       run_tile(std::integral_constant<int, 4>{});
     } else {
@@ -480,7 +567,7 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
     round += grid;
     if (!decode(round, tl)) break;
   }
-  wait_loads<0>();  // (the stream's last loads bring nothing, but they write LDS)
+  if constexpr (P::kDirect) wait_loads<0>();  // (the stream's last loads bring nothing, but they write LDS)
 }
 
 int cu_count() {
@@ -501,8 +588,8 @@ hipError_t launch(const Product& prm, hipStream_t stream) {
                                                      hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
   if (attr != hipSuccess) return attr;
   const long cols = (prm.N + P::kCols - 1) / P::kCols;
-  const long rows = P::kWeights ? static_cast<long>(prm.experts) * ((prm.M + kTileRows - 1) / kTileRows)
-                                : prm.rows / kTileRows + std::min<long>(prm.experts, prm.rows);
+  const long rows = P::kWeights ? static_cast<long>(prm.experts) * ((prm.M + 63) / 64)
+                                : prm.rows / 64 + std::min<long>(prm.experts, prm.rows);
   long grid = std::min<long>(cols * rows, cu_count());
   if (grid >= kXcds) grid = grid / kXcds * kXcds;
   const std::size_t lds = 2 * kStageBytes + 3 * static_cast<std::size_t>(prm.experts + 1) * sizeof(int32_t);
@@ -510,20 +597,24 @@ hipError_t launch(const Product& prm, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <typename T>
-using GateUp = Kind<T, true, false, false, EpiGate<T>>;  // x [Wg | Wu]
-template <typename T>
-using Down = Kind<T, true, false, false, EpiStore<T>>;  // a Wd
-template <typename T>
-using DGateUp = Kind<T, true, true, false, EpiDGate<T>>;  // dy Wd^T
-template <typename T>
-using Dx = Kind<T, true, true, false, EpiStore<T>>;  // dg Wg^T + du Wu^T
-template <typename T>
-using DwPair = Kind<T, false, false, true, EpiPair<T>>;  // x^T [dg | du]
-template <typename T>
-using Dw = Kind<T, false, false, true, EpiStore<T>>;  // a^T dy
+template <typename T, bool DIRECT>
+using GateUp = Kind<T, true, false, false, EpiGate<T>, DIRECT>;  // x [Wg | Wu]
+template <typename T, bool DIRECT>
+using Down = Kind<T, true, false, false, EpiStore<T>, DIRECT>;  // a Wd
+template <typename T, bool DIRECT>
+using DGateUp = Kind<T, true, true, false, EpiDGate<T>, DIRECT>;  // dy Wd^T
+template <typename T, bool DIRECT>
+using Dx = Kind<T, true, true, false, EpiStore<T>, DIRECT>;  // dg Wg^T + du Wu^T
+template <typename T, bool DIRECT>
+using DwPair = Kind<T, false, false, true, EpiPair<T>, DIRECT>;  // x^T [dg | du]
+template <typename T, bool DIRECT>
+using Dw = Kind<T, false, false, true, EpiStore<T>, DIRECT>;  // a^T dy
+template <typename T, bool DIRECT>
+using Int8 = Kind<int8_t, true, true, false, EpiInt8<T>, DIRECT>;
+template <typename T, bool DIRECT>
+using Int8Gate = Kind<int8_t, true, true, false, EpiInt8Gate<T>, DIRECT>;
 
-// 16-byte loads need every row of every operand on a 16-byte boundary.
+// Loads straight into LDS need every row of every operand on a 16-byte boundary.
 bool aligned16(std::initializer_list<const void*> pointers) {
   for (const void* p : pointers) {
     if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return false;
@@ -540,7 +631,7 @@ Product base_of(const FfnParams& f) {
   return p;
 }
 
-template <typename T>
+template <typename T, bool DIRECT>
 hipError_t forward(const FfnParams& f, hipStream_t stream) {
   Product p = base_of(f);
   p.a = f.x;
@@ -553,7 +644,7 @@ hipError_t forward(const FfnParams& f, hipStream_t stream) {
   p.K = f.hidden;
   p.lda = f.hidden;
   p.ldb = f.inner;
-  hipError_t error = launch<GateUp<T>>(p, stream);
+  hipError_t error = launch<GateUp<T, DIRECT>>(p, stream);
   if (error != hipSuccess) return error;
   p = base_of(f);
   p.a = f.act;
@@ -564,10 +655,10 @@ hipError_t forward(const FfnParams& f, hipStream_t stream) {
   p.K = f.inner;
   p.lda = f.inner;
   p.ldb = f.output;
-  return launch<Down<T>>(p, stream);
+  return launch<Down<T, DIRECT>>(p, stream);
 }
 
-template <typename T>
+template <typename T, bool DIRECT>
 hipError_t backward(const FfnParams& f, hipStream_t stream) {
   hipError_t error = hipSuccess;
   if (f.rows != 0) {
@@ -581,7 +672,7 @@ hipError_t backward(const FfnParams& f, hipStream_t stream) {
     p.N = f.inner;
     p.K = f.output;
     p.lda = p.ldb = f.output;
-    error = launch<DGateUp<T>>(p, stream);
+    error = launch<DGateUp<T, DIRECT>>(p, stream);
   }
   if (error == hipSuccess && f.rows != 0 && f.dx != nullptr) {
     Product p = base_of(f);
@@ -593,7 +684,7 @@ hipError_t backward(const FfnParams& f, hipStream_t stream) {
     p.N = f.hidden;
     p.K = f.inner;
     p.lda = p.ldb = f.inner;
-    error = launch<Dx<T>>(p, stream);
+    error = launch<Dx<T, DIRECT>>(p, stream);
   }
   if (error == hipSuccess && f.dw_gate != nullptr) {
     Product p = base_of(f);
@@ -606,7 +697,7 @@ hipError_t backward(const FfnParams& f, hipStream_t stream) {
     p.N = f.inner;
     p.lda = f.hidden;
     p.ldb = f.inner;
-    error = launch<DwPair<T>>(p, stream);
+    error = launch<DwPair<T, DIRECT>>(p, stream);
   }
   if (error == hipSuccess && f.dw_down != nullptr) {
     Product p = base_of(f);
@@ -617,12 +708,12 @@ hipError_t backward(const FfnParams& f, hipStream_t stream) {
     p.N = f.output;
     p.lda = f.inner;
     p.ldb = f.output;
-    error = launch<Dw<T>>(p, stream);
+    error = launch<Dw<T, DIRECT>>(p, stream);
   }
   return error;
 }
 
-template <typename T>
+template <typename T, bool DIRECT>
 hipError_t int8_product(const Int8Params& f, hipStream_t stream) {
   Product p{};
   p.offsets = f.offsets;
@@ -639,31 +730,31 @@ hipError_t int8_product(const Int8Params& f, hipStream_t stream) {
   p.N = f.output;
   p.K = f.hidden;
   p.lda = p.ldb = f.hidden;
-  return f.w_up != nullptr ? launch<Kind<int8_t, true, true, false, EpiInt8Gate<T>>>(p, stream)
-                           : launch<Kind<int8_t, true, true, false, EpiInt8<T>>>(p, stream);
+  return f.w_up != nullptr ? launch<Int8Gate<T, DIRECT>>(p, stream)
+                           : launch<Int8<T, DIRECT>>(p, stream);
 }
 
 }  // namespace
 
 hipError_t gated_ffn(const FfnParams& f, hipStream_t stream) {
-  if (f.hidden % 8 != 0 || f.inner % 8 != 0 || f.output % 8 != 0 || !aligned16({f.x, f.w_gate, f.w_up, f.w_down, f.act})) {
-    return gated_ffn_naive(f, stream);
-  }
-  return f.bf16 ? forward<bf16>(f, stream) : forward<f16>(f, stream);
+  const bool direct =
+      f.hidden % 8 == 0 && f.inner % 8 == 0 && f.output % 8 == 0 && aligned16({f.x, f.w_gate, f.w_up, f.w_down, f.act});
+  if (f.bf16) return direct ? forward<bf16, true>(f, stream) : forward<bf16, false>(f, stream);
+  return direct ? forward<f16, true>(f, stream) : forward<f16, false>(f, stream);
 }
 
 hipError_t gated_ffn_backward(const FfnParams& f, hipStream_t stream) {
-  if (f.hidden % 8 != 0 || f.inner % 8 != 0 || f.output % 8 != 0 ||
-      !aligned16({f.x, f.w_gate, f.w_up, f.w_down, f.act, f.dy, f.d_gate, f.d_up})) {
-    return gated_ffn_backward_naive(f, stream);
-  }
-  return f.bf16 ? backward<bf16>(f, stream) : backward<f16>(f, stream);
+  const bool direct = f.hidden % 8 == 0 && f.inner % 8 == 0 && f.output % 8 == 0 &&
+                      aligned16({f.x, f.w_gate, f.w_up, f.w_down, f.act, f.dy, f.d_gate, f.d_up});
+  if (f.bf16) return direct ? backward<bf16, true>(f, stream) : backward<bf16, false>(f, stream);
+  return direct ? backward<f16, true>(f, stream) : backward<f16, false>(f, stream);
 }
 
 hipError_t int8_grouped_gemm(const Int8Params& f, hipStream_t stream) {
-  if (f.hidden % 16 != 0 || !aligned16({f.q, f.w, f.w_up})) return int8_grouped_gemm_naive(f, stream);
-  if (f.dtype == RR_DTYPE_FP32) return int8_product<float>(f, stream);
-  return f.dtype == RR_DTYPE_BF16 ? int8_product<bf16>(f, stream) : int8_product<f16>(f, stream);
+  const bool direct = f.hidden % 16 == 0 && aligned16({f.q, f.w, f.w_up});
+  if (f.dtype == RR_DTYPE_FP32) return direct ? int8_product<float, true>(f, stream) : int8_product<float, false>(f, stream);
+  if (f.dtype == RR_DTYPE_BF16) return direct ? int8_product<bf16, true>(f, stream) : int8_product<bf16, false>(f, stream);
+  return direct ? int8_product<f16, true>(f, stream) : int8_product<f16, false>(f, stream);
 }
 
 }  // namespace rr::kern
