@@ -450,7 +450,8 @@ enum { RR_ACT_SILU = 0, RR_ACT_GELU_TANH = 1 };
  *   g = x Wg, u = x Wu, a = act(g) * u, y = a Wd.
  * a is formed from the FP32 sums of g and u and rounded to `dtype` once, which
  * the second product reads. gate / up (both or none) receive g and u for
- * rr_gated_ffn_backward.
+ * rr_gated_ffn_backward. Workspace: rr_gated_ffn_workspace_size (0 but for few rows of
+ * few wide experts), 16-byte aligned.
  */
 typedef struct rr_gated_ffn_args {
   const void* x;          /* [rows, hidden] */
@@ -609,6 +610,7 @@ typedef struct rr_int8_grouped_gemm_args {
   rr_kernel_selection kernel;
 } rr_int8_grouped_gemm_args;
 
+/* FP32 parts of sums that are split over workgroups: few rows of few wide experts only, else 0 */
 size_t rr_gated_ffn_workspace_size(const rr_gated_ffn_args* args);
 /* d gate and d up: 2 * rows * inner values, each part rounded up to 16 bytes */
 size_t rr_gated_ffn_backward_workspace_size(const rr_gated_ffn_backward_args* args);

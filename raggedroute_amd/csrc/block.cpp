@@ -146,7 +146,13 @@ rr_status check_norm(const Args& a) noexcept {
 
 extern "C" {
 
-size_t rr_gated_ffn_workspace_size(const rr_gated_ffn_args*) { return 0; }
+size_t rr_gated_ffn_workspace_size(const rr_gated_ffn_args* args) {
+  if (args == nullptr || args->rows <= 0 || args->experts <= 0 || args->hidden <= 0 || args->inner <= 0 ||
+      args->output <= 0 || args->kernel.family == RR_FAMILY_NAIVE) {
+    return 0;
+  }
+  return rr::kern::gated_ffn_parts(args->rows, args->experts, args->hidden, args->inner, args->output) * sizeof(float);
+}
 size_t rr_gated_ffn_backward_workspace_size(const rr_gated_ffn_backward_args* args) {
   if (args == nullptr || args->rows <= 0 || args->inner <= 0) return 0;
   return 2 * rr::ffn_part_bytes(*args);
@@ -180,7 +186,7 @@ rr_status rr_gated_ffn(const rr_gated_ffn_args* args, const rr_runtime_context* 
                            "gated_ffn: dtype must be FP16 or BF16 and y_dtype the same or FP32");
   }
   bool naive = false;
-  const rr_status status = rr::choose_family(a.kernel, context->architecture, &naive);
+  rr_status status = rr::choose_family(a.kernel, context->architecture, &naive);
   if (status.code != RR_STATUS_SUCCESS) return status;
   if (a.rows == 0) return rr::ok_status();
   if (rr::any_null({a.x, a.w_gate, a.w_up, a.w_down, a.offsets, a.act, a.y})) {
@@ -190,7 +196,11 @@ rr_status rr_gated_ffn(const rr_gated_ffn_args* args, const rr_runtime_context* 
       !rr::is_aligned(a.y, rr::type_size(a.y_dtype)) || !rr::is_aligned(a.offsets, alignof(int32_t))) {
     return rr::invalid_argument("gated_ffn: every buffer must be aligned to its element type");
   }
+  status = rr::check_workspace(context, rr_gated_ffn_workspace_size(args),
+                               "gated_ffn: the workspace must hold the parts of split sums");
+  if (status.code != RR_STATUS_SUCCESS) return status;
   rr::kern::FfnParams p{};
+  p.parts = static_cast<float*>(context->workspace);
   p.x = a.x;
   p.w_gate = a.w_gate;
   p.w_up = a.w_up;

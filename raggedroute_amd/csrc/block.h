@@ -28,7 +28,8 @@ struct FfnParams {
   void* dw_gate;
   void* dw_up;
   void* dw_down;
-  void* d_gate;  // workspace [rows, inner]
+  float* parts;  // workspace, forward: gated_ffn_parts() floats
+  void* d_gate;  // workspace, backward: [rows, inner]
   void* d_up;
   int rows, experts, hidden, inner, output;
   int activation;
@@ -73,6 +74,8 @@ struct NormParams {
 };
 
 // ---- products on the matrix cores ----
+// FP32 values of workspace that the forward call needs.
+std::size_t gated_ffn_parts(int rows, int experts, int hidden, int inner, int output);
 hipError_t gated_ffn(const FfnParams& prm, hipStream_t stream);
 hipError_t gated_ffn_backward(const FfnParams& prm, hipStream_t stream);
 hipError_t int8_grouped_gemm(const Int8Params& prm, hipStream_t stream);

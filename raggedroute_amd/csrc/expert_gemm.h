@@ -171,4 +171,13 @@ struct EpiInt8Gate {
   }
 };
 
+// ---- few rows an expert (expert_rows.hip) ----
+// Whether the kernel for few rows takes a row product of this many rows.
+bool expert_rows_ok(int rows, int experts);
+// Workgroups that share an expert's sum of `length` (1: no parts are needed).
+int expert_rows_splits(int rows, int experts, int columns, int length);
+// parts: FP32 [1, dual products 2][splits][rows][N] where splits > 1 (16-bit products only).
+template <typename T, class Epi>
+hipError_t expert_rows(const Product& prm, float* parts, int splits, hipStream_t stream);
+
 }  // namespace rr::kern

@@ -644,7 +644,10 @@ hipError_t forward(const FfnParams& f, hipStream_t stream) {
   p.K = f.hidden;
   p.lda = f.hidden;
   p.ldb = f.inner;
-  hipError_t error = launch<GateUp<T, DIRECT>>(p, stream);
+  const bool few = expert_rows_ok(f.rows, f.experts);
+  int splits = expert_rows_splits(f.rows, f.experts, f.inner, f.hidden);
+  const hipError_t error = few ? expert_rows<T, EpiGate<T>>(p, splits > 1 ? f.parts : nullptr, splits, stream)
+                               : launch<GateUp<T, DIRECT>>(p, stream);
   if (error != hipSuccess) return error;
   p = base_of(f);
   p.a = f.act;
@@ -655,7 +658,9 @@ hipError_t forward(const FfnParams& f, hipStream_t stream) {
   p.K = f.inner;
   p.lda = f.inner;
   p.ldb = f.output;
-  return launch<Down<T, DIRECT>>(p, stream);
+  if (!few) return launch<Down<T, DIRECT>>(p, stream);
+  splits = expert_rows_splits(f.rows, f.experts, f.output, f.inner);
+  return expert_rows<T, EpiStore<T>>(p, splits > 1 ? f.parts : nullptr, splits, stream);
 }
 
 template <typename T, bool DIRECT>
@@ -730,11 +735,21 @@ hipError_t int8_product(const Int8Params& f, hipStream_t stream) {
   p.N = f.output;
   p.K = f.hidden;
   p.lda = p.ldb = f.hidden;
+  if (expert_rows_ok(f.rows, f.experts)) {
+    return f.w_up != nullptr ? expert_rows<int8_t, EpiInt8Gate<T>>(p, nullptr, 1, stream)
+                             : expert_rows<int8_t, EpiInt8<T>>(p, nullptr, 1, stream);
+  }
   return f.w_up != nullptr ? launch<Int8Gate<T, DIRECT>>(p, stream)
                            : launch<Int8<T, DIRECT>>(p, stream);
 }
 
 }  // namespace
+
+std::size_t gated_ffn_parts(int rows, int experts, int hidden, int inner, int output) {
+  const std::size_t up = static_cast<std::size_t>(expert_rows_splits(rows, experts, inner, hidden));
+  const std::size_t down = static_cast<std::size_t>(expert_rows_splits(rows, experts, output, inner));
+  return static_cast<std::size_t>(rows) * std::max(up > 1 ? 2 * up * inner : 0, down > 1 ? down * output : 0);
+}
 
 hipError_t gated_ffn(const FfnParams& f, hipStream_t stream) {
   const bool direct =

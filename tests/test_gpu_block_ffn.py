@@ -347,3 +347,12 @@ def test_other_stream_and_graph(device):
             assert rr.gated_ffn(args, ctx).ok()
         torch.cuda.synchronize()
         assert torch.equal(replayed, y) and (y != 0).any()
+
+
+@pytest.mark.parametrize("counts,k,f,n", [([1], 2048, 40, 24), ([2, 0, 1], 3000, 2100, 130), ([0, 3], 260, 4100, 17),
+                                          ([17], 2304, 8, 8), ([20, 0, 30], 2048, 2048, 48)])
+@pytest.mark.parametrize("dtype,y_dtype", [("bf16", "bf16"), ("f16", "f32")])
+def test_forward_split_sums(device, counts, k, f, n, dtype, y_dtype):
+    """Few rows of few wide experts: sums split over workgroups, parts in the workspace."""
+    v, b, rows = make(counts, k, f, n, dtype, seed=12)
+    check_forward(v, forward(b, counts, rows, k, f, n, dtype, y_dtype=y_dtype), counts, dtype, "silu", y_dtype=y_dtype)
