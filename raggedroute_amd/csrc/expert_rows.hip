@@ -1,7 +1,7 @@
 // Grouped products of the expert block for few rows an expert (decoding): the weights are
 // read once from memory, straight into registers in matrix-operand order.
 //
-// A workgroup of W waves takes 128 columns of one expert (of each right operand) and its
+// A workgroup of W waves takes 128 columns (int8: 64) of one expert (of each right operand) and its
 // rows in blocks of 16 MR; the waves share the sum's length and add up through LDS in a
 // fixed order. What bounds it is memory: a wave has 8 to 16 loads of 1 KB in flight and
 // never passes weights through LDS.
@@ -9,7 +9,8 @@
 //    of a 32-k step and turns that 8 x 8 block (32 byte permutes); register c then holds
 //    eight k of column 8 i + c, the operand of one v_mfma_f32_16x16x32: the order of the
 //    columns among the instruction's rows is free.
-//  - int8 weights lie [N, K]: a lane loads 16 k of one column.
+//  - int8 weights lie [N, K]: a lane loads 16 k of one column (64 columns a workgroup, 128 k
+//    a step, so that the two loads of a row's 128 bytes follow each other).
 //  - The weights are the instruction's first operand, so that a lane ends with adjacent
 //    columns of one row.
 // Where an expert's columns make fewer workgroups than the card has CUs, the sum is also
@@ -32,14 +33,26 @@ using rr::dev::f16;
 typedef int i4 __attribute__((ext_vector_type(4)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 
-constexpr int kCols = 128;
+constexpr int kBufferFlags = 0x00027000;  // raw 32-bit buffer
+// Policies of the weights' loads: past the caches where the weights are larger than the
+// caches keep from one call to the next (one token of E = 8, K = 4096, F = 14336 143 -> 125 us;
+// but E = 64, K = 256, F = 128 13.1 -> 15.2). int8 rows are loaded 64 bytes at a time, whose
+// lines the next load needs again (E = 128, K = 2048, N = 768, 128 rows: 46 us, past the
+// caches 59), 16-bit rows a whole line and more.
+constexpr int kStreamed = 2, kCached = 0;
+constexpr std::size_t kStreamedBytes = std::size_t{64} << 20;
+
 constexpr int kCus = 256;  // MI355X
 
+// A step: its k, the workgroup's columns, whether k runs along the weights' rows,
+// accumulator and product of the matrix instruction (int8 steps are two of them: 128 bytes
+// of every weight row).
 template <typename T>
-struct Step;  // one matrix instruction: k of it, accumulator, product
+struct Step;
 template <>
 struct Step<bf16> {
-  static constexpr int kK = 32;
+  static constexpr int kK = 32, kCols = 128;
+  static constexpr bool kKC = false;
   typedef f4 acc;
   typedef bf16 frag __attribute__((ext_vector_type(8)));
   static __device__ __forceinline__ acc mul(i4 a, i4 b, acc c) {
@@ -48,7 +61,8 @@ struct Step<bf16> {
 };
 template <>
 struct Step<f16> {
-  static constexpr int kK = 32;
+  static constexpr int kK = 32, kCols = 128;
+  static constexpr bool kKC = false;
   typedef f4 acc;
   typedef f16 frag __attribute__((ext_vector_type(8)));
   static __device__ __forceinline__ acc mul(i4 a, i4 b, acc c) {
@@ -57,23 +71,31 @@ struct Step<f16> {
 };
 template <>
 struct Step<int8_t> {
-  static constexpr int kK = 64;
+  static constexpr int kK = 128, kCols = 64;
+  static constexpr bool kKC = true;
   typedef i4 acc;
   static __device__ __forceinline__ acc mul(i4 a, i4 b, acc c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
 };
 
-// 16 bytes at p (of any alignment), of which the first `count` elements exist
-template <typename T>
-__device__ __forceinline__ i4 load16(const T* p, int count) {
+// 16 bytes at base (uniform) + offset + lane offset. `WHOLE`: all of them exist and lie on
+// a 4-byte boundary; else any alignment, the first `count` elements exist. POLICY:
+// of whole loads.
+template <bool WHOLE, int POLICY, typename T>
+__device__ __forceinline__ i4 load16(const T* base, uint32_t offset, uint32_t lane_offset, int count) {
+  if constexpr (WHOLE) {
+    const auto buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), 0, -1, kBufferFlags);
+    return __builtin_bit_cast(i4, __builtin_amdgcn_raw_buffer_load_b128(buffer, lane_offset, offset, POLICY));
+  }
   constexpr int V = 16 / sizeof(T);
   typedef T chunk __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+  const char* at = reinterpret_cast<const char*>(base) + offset + lane_offset;
   chunk v = {};
   if (count >= V) {
-    v = *reinterpret_cast<const chunk*>(p);
+    v = *reinterpret_cast<const chunk*>(at);
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      if (i < count) v[i] = p[i];
+      if (i < count) v[i] = reinterpret_cast<const T*>(at)[i];
     }
   }
   return __builtin_bit_cast(i4, v);
@@ -103,14 +125,18 @@ __device__ __forceinline__ int find_expert(const Product& p, int index, int* fir
   return -1;
 }
 
-template <typename T, class Epi, int MR, int W>
-__global__ __launch_bounds__(64 * W) void rr_expert_rows_kernel(Product prm, float* parts, int splits, int blocks) {
+// (waves a SIMD: what the accumulators and the two sets of weights leave room for)
+template <typename T, class Epi, int MR, int W, int POLICY>
+__global__ __launch_bounds__(64 * W, Epi::kDual ? 2 : 3) void rr_expert_rows_kernel(Product prm, float* parts, int splits, int blocks) {
   using M = Step<T>;
   using Acc = typename M::acc;
-  constexpr bool kKC = sizeof(T) == 1;  // k along the weights' rows
+  constexpr bool kKC = M::kKC;
   constexpr int B = Epi::kDual ? 2 : 1;
+  constexpr int C = kKC ? 4 : 8;       // accumulators of 16 columns
+  constexpr int X = kKC ? 2 : 1;       // matrix instructions of a step for each
+  constexpr int V = 16 / sizeof(T);    // elements of a load
   extern __shared__ __align__(16) char smem[];
-  i4* lds = reinterpret_cast<i4*>(smem);  // [W / 2][B * 8 * MR][64]
+  i4* lds = reinterpret_cast<i4*>(smem);  // [W / 2][B * C * MR][64]
   const int lane = static_cast<int>(threadIdx.x) & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int li = lane & 15, g = lane >> 4;
@@ -119,7 +145,7 @@ __global__ __launch_bounds__(64 * W) void rr_expert_rows_kernel(Product prm, flo
   int first, count;
   const int e = find_expert(prm, static_cast<int>(blockIdx.x) / blocks / splits, &first, &count);
   if (e < 0) return;
-  const int n0 = block * kCols;
+  const int n0 = block * M::kCols;
   const int K = prm.K, N = prm.N;
   // this wave's steps
   const int steps = (K + M::kK - 1) / M::kK;
@@ -128,91 +154,149 @@ __global__ __launch_bounds__(64 * W) void rr_expert_rows_kernel(Product prm, flo
   const int s1 = static_cast<int>(static_cast<int64_t>(steps) * (share + 1) / shares);
   const T* weights[2] = {static_cast<const T*>(prm.b) + static_cast<std::size_t>(e) * K * N,
                          static_cast<const T*>(Epi::kDual ? prm.b_up : prm.b) + static_cast<std::size_t>(e) * K * N};
+  // every row that is loaded starts on a 4-byte boundary
+  const bool aligned = ((reinterpret_cast<uintptr_t>(prm.a) | reinterpret_cast<uintptr_t>(weights[0]) |
+                         reinterpret_cast<uintptr_t>(weights[1]) | sizeof(T) * K | (kKC ? 0 : sizeof(T) * N)) & 3) == 0;
 
 #pragma unroll 1
   for (int r0 = 0; r0 < count; r0 += 16 * MR) {
-    Acc acc[B][8][MR] = {};
-    const T* x[MR];
+    Acc acc[B][C][MR] = {};
+    // byte offsets of the lane: of its rows (rows past the last repeat it: their results
+    // are not stored) and in the weights
+    constexpr uint32_t S = sizeof(T);
+    const T* x = static_cast<const T*>(prm.a) + static_cast<std::size_t>(first + r0) * K;
+    uint32_t x_at[MR];
 #pragma unroll
-    for (int i = 0; i < MR; ++i) x[i] = static_cast<const T*>(prm.a) + static_cast<std::size_t>(first + min(r0 + 16 * i + li, count - 1)) * K;
-    // One step: `whole` says that neither the columns nor the step are cut.
-    auto step = [&](int s, auto whole) {
-      constexpr bool kWhole = decltype(whole)::value;
-      const int k = s * M::kK + g * (16 / static_cast<int>(sizeof(T)));  // the lane's first k
-      i4 xv[MR];
+    for (int i = 0; i < MR; ++i) x_at[i] = S * (static_cast<uint32_t>(min(16 * i + li, count - 1 - r0)) * static_cast<uint32_t>(K) + g * V);
+    uint32_t w_at[kKC ? 4 : 1];
 #pragma unroll
-      for (int i = 0; i < MR; ++i) {
-        // (rows past the last repeat it: their results are not stored)
-        xv[i] = load16(x[i] + k, kWhole ? 16 : K - k);
-      }
-      if constexpr (kKC) {
-        i4 w[B][8];
+    for (int j = 0; j < (kKC ? 4 : 1); ++j) {
+      w_at[j] = kKC ? S * (static_cast<uint32_t>(min(16 * j + li, N - 1 - n0)) * static_cast<uint32_t>(K) + g * V)
+                    : S * (static_cast<uint32_t>(8 * g) * static_cast<uint32_t>(N) + 8 * li);
+    }
+    struct Rows {
+      i4 v[MR][X];
+    };
+    struct Weights {
+      i4 v[8];
+    };
+    // what a step multiplies; `whole`: neither the columns nor the step are cut
+    auto load_rows = [&](Rows& o, int s, auto whole) {
 #pragma unroll
-        for (int b = 0; b < B; ++b) {
+      for (int h = 0; h < X; ++h) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int n = n0 + 16 * j + li;
-            w[b][j] = load16(weights[b] + static_cast<std::size_t>(kWhole ? n : min(n, N - 1)) * K + k, kWhole ? 16 : K - k);
-          }
-        }
-#pragma unroll
-        for (int b = 0; b < B; ++b) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-#pragma unroll
-            for (int i = 0; i < MR; ++i) acc[b][j][i] = M::mul(w[b][j], xv[i], acc[b][j][i]);
-          }
-        }
-      } else {
-        i4 w[B][8];
-        const int n = n0 + 8 * li;
-#pragma unroll
-        for (int b = 0; b < B; ++b) {
-#pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const T* row = weights[b] + static_cast<std::size_t>(s * M::kK + q) * N;  // uniform
-            const std::size_t at = static_cast<std::size_t>(8 * g) * N + n;
-            w[b][q] = load16(row + at, kWhole ? 8 : k + q < K ? N - n : 0);
-          }
-        }
-#pragma unroll
-        for (int b = 0; b < B; ++b) {
-#pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            i4 column;
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-              column[m] = static_cast<int>(__builtin_amdgcn_perm(static_cast<uint32_t>(w[b][2 * m + 1][c >> 1]),
-                                                                 static_cast<uint32_t>(w[b][2 * m][c >> 1]),
-                                                                 (c & 1) != 0 ? 0x07060302U : 0x05040100U));
-            }
-#pragma unroll
-            for (int i = 0; i < MR; ++i) acc[b][c][i] = M::mul(column, xv[i], acc[b][c][i]);
-          }
+        for (int i = 0; i < MR; ++i) {
+          o.v[i][h] = load16<decltype(whole)::value, kCached>(x + s * M::kK, S * 4 * h * V, x_at[i], K - s * M::kK - (4 * h + g) * V);
         }
       }
     };
-    const bool cut = n0 + kCols > N;
-    const int whole_end = cut ? s0 : min(s1, K / M::kK);
+    auto load_weights = [&](Weights& o, int b, int s, auto whole) {
+      constexpr bool kWhole = decltype(whole)::value;
+      if constexpr (kKC) {  // [fragment][half]: columns 16 j + li, k of half h
+        const T* at = weights[b] + static_cast<std::size_t>(n0) * K + s * M::kK;  // (uniform, as below)
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          o.v[q] = load16<kWhole, POLICY>(at, S * 4 * (q & 1) * V, w_at[q >> 1], K - s * M::kK - (4 * (q & 1) + g) * V);
+          if (!kWhole) __builtin_amdgcn_sched_barrier(0);  // (the pieces of all eight at once would fill the registers)
+        }
+      } else {  // k 8 g + q: columns 8 li .. + 7
+        const T* at = weights[b] + static_cast<std::size_t>(s * M::kK) * N + n0;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          o.v[q] = load16<kWhole, POLICY>(at, S * static_cast<uint32_t>(q) * static_cast<uint32_t>(N), w_at[0],
+                                  s * M::kK + 8 * g + q < K ? N - n0 - 8 * li : 0);
+          if (!kWhole) __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    };
+    auto multiply = [&](const Weights& w, const Rows& r, int b) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        if constexpr (kKC) {
+#pragma unroll
+          for (int h = 0; h < X; ++h) {
+#pragma unroll
+            for (int i = 0; i < MR; ++i) acc[b][c][i] = M::mul(w.v[2 * c + h], r.v[i][h], acc[b][c][i]);
+          }
+        } else {
+          i4 column;
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            column[m] = static_cast<int>(__builtin_amdgcn_perm(static_cast<uint32_t>(w.v[2 * m + 1][c >> 1]),
+                                                               static_cast<uint32_t>(w.v[2 * m][c >> 1]),
+                                                               (c & 1) != 0 ? 0x07060302U : 0x05040100U));
+          }
+#pragma unroll
+          for (int i = 0; i < MR; ++i) acc[b][c][i] = M::mul(column, r.v[i][0], acc[b][c][i]);
+        }
+      }
+    };
+    // Two sets of weights in registers: while one is multiplied the other is on its way.
+    // Dual products hold one step's gate and up weights, others two steps.
+    const std::integral_constant<bool, true> whole;
+    const std::integral_constant<bool, false> cut;
+    int s = s0;
+    const int end = n0 + M::kCols > N || !aligned ? s0 : max(s0, min(s1, K / M::kK));  // of the whole steps
+    constexpr int D = Epi::kDual ? 1 : 2;                                 // steps in the two sets
+    if (s + D <= end) {
+      Weights w0, w1;
+      Rows r0v, r1v;
+      load_rows(r0v, s, whole);
+      load_weights(w0, 0, s, whole);
+      if constexpr (!Epi::kDual) load_rows(r1v, s + 1, whole);
+      load_weights(w1, B - 1, s + D - 1, whole);
 #pragma unroll 1
-    for (int s = s0; s < whole_end; ++s) step(s, std::integral_constant<bool, true>{});
+      for (; s + 2 * D <= end; s += D) {
+        __builtin_amdgcn_sched_barrier(0);
+        Rows next;
+        multiply(w0, r0v, 0);
+        __builtin_amdgcn_sched_barrier(0);  // (loads hoisted over the products would need registers of their own)
+        if constexpr (Epi::kDual) {
+          load_rows(next, s + 1, whole);
+        } else {
+          load_rows(r0v, s + 2, whole);
+        }
+        load_weights(w0, 0, s + D, whole);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(w1, Epi::kDual ? r0v : r1v, B - 1);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (Epi::kDual) {
+          r0v = next;
+        } else {
+          load_rows(r1v, s + 3, whole);
+        }
+        load_weights(w1, B - 1, s + 2 * D - 1, whole);
+      }
+      multiply(w0, r0v, 0);
+      multiply(w1, Epi::kDual ? r0v : r1v, B - 1);
+      s += D;
+    }
 #pragma unroll 1
-    for (int s = whole_end; s < s1; ++s) step(s, std::integral_constant<bool, false>{});
+    for (; s < s1; ++s) {
+      Rows r;
+      Weights w;
+      load_rows(r, s, cut);
+#pragma unroll
+      for (int b = 0; b < B; ++b) {
+        load_weights(w, b, s, cut);
+        multiply(w, r, b);
+      }
+    }
 
     // the waves' sums, halved round by round
 #pragma unroll
     for (int half = W / 2; half >= 1; half /= 2) {
       if (wave >= half && wave < 2 * half) {
 #pragma unroll
-        for (int q = 0; q < B * 8 * MR; ++q) {
-          lds[((wave - half) * B * 8 * MR + q) * 64 + lane] = __builtin_bit_cast(i4, acc[q / (8 * MR)][q / MR % 8][q % MR]);
+        for (int q = 0; q < B * C * MR; ++q) {
+          lds[((wave - half) * B * C * MR + q) * 64 + lane] = __builtin_bit_cast(i4, acc[q / (C * MR)][q / MR % C][q % MR]);
         }
       }
       __syncthreads();
       if (wave < half) {
 #pragma unroll
-        for (int q = 0; q < B * 8 * MR; ++q) {
-          acc[q / (8 * MR)][q / MR % 8][q % MR] += __builtin_bit_cast(Acc, lds[(wave * B * 8 * MR + q) * 64 + lane]);
+        for (int q = 0; q < B * C * MR; ++q) {
+          acc[q / (C * MR)][q / MR % C][q % MR] += __builtin_bit_cast(Acc, lds[(wave * B * C * MR + q) * 64 + lane]);
         }
       }
       __syncthreads();
@@ -224,26 +308,26 @@ __global__ __launch_bounds__(64 * W) void rr_expert_rows_kernel(Product prm, flo
       const int r = r0 + 16 * i + li;
       if (r >= count) continue;
       const std::size_t row = static_cast<std::size_t>(first) + r;
-      constexpr int V = kKC ? 4 : 8;
+      constexpr int E = kKC ? 4 : 8;  // columns of a store
 #pragma unroll
-      for (int p = 0; p < 32 / V; ++p) {
+      for (int p = 0; p < 4; ++p) {
         const int n = n0 + (kKC ? 16 * p + 4 * g : 32 * g + 8 * p);
         if (n >= N) continue;
-        float v[B][V];
+        float v[B][E];
 #pragma unroll
         for (int b = 0; b < B; ++b) {
 #pragma unroll
-          for (int q = 0; q < V; ++q) v[b][q] = static_cast<float>(kKC ? acc[b][p][i][q] : acc[b][q][i][p]);
+          for (int q = 0; q < E; ++q) v[b][q] = static_cast<float>(kKC ? acc[b][p][i][q] : acc[b][q][i][p]);
         }
         if (parts != nullptr) {
 #pragma unroll
           for (int b = 0; b < B; ++b) {
-            Cols<float, V>::store(parts + (static_cast<std::size_t>(b * splits + split) * prm.rows + row) * N + n, v[b], N - n);
+            Cols<float, E>::store(parts + (static_cast<std::size_t>(b * splits + split) * prm.rows + row) * N + n, v[b], N - n);
           }
         } else if constexpr (Epi::kDual) {
-          Epi::template emit<V>(prm, e, row, n, N - n, v[0], v[1]);
+          Epi::template emit<E>(prm, e, row, n, N - n, v[0], v[1]);
         } else {
-          Epi::template emit<V>(prm, e, row, n, N - n, v[0]);
+          Epi::template emit<E>(prm, e, row, n, N - n, v[0]);
         }
       }
     }
@@ -279,17 +363,17 @@ __global__ __launch_bounds__(256) void rr_expert_rows_sum_kernel(Product prm, co
   }
 }
 
-template <typename T, class Epi, int MR, int W>
+template <typename T, class Epi, int MR, int W, int POLICY>
 hipError_t launch(const Product& prm, float* parts, int splits, hipStream_t stream) {
-  constexpr std::size_t lds = static_cast<std::size_t>(W / 2) * (Epi::kDual ? 2 : 1) * 8 * MR * 64 * sizeof(i4);
+  constexpr std::size_t lds = static_cast<std::size_t>(W / 2) * (Epi::kDual ? 2 : 1) * (Step<T>::kKC ? 4 : 8) * MR * 64 * sizeof(i4);
   if constexpr (lds > 64 * 1024) {
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(rr_expert_rows_kernel<T, Epi, MR, W>),
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(rr_expert_rows_kernel<T, Epi, MR, W, POLICY>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     if (attr != hipSuccess) return attr;
   }
-  const int blocks = (prm.N + kCols - 1) / kCols;
+  const int blocks = (prm.N + Step<T>::kCols - 1) / Step<T>::kCols;
   const std::size_t grid = static_cast<std::size_t>(std::min(prm.experts, prm.rows)) * blocks * splits;
-  rr_expert_rows_kernel<T, Epi, MR, W><<<dim3(static_cast<unsigned>(grid)), 64 * W, lds, stream>>>(prm, parts, splits, blocks);
+  rr_expert_rows_kernel<T, Epi, MR, W, POLICY><<<dim3(static_cast<unsigned>(grid)), 64 * W, lds, stream>>>(prm, parts, splits, blocks);
   if (splits > 1) {
     if constexpr (sizeof(T) == 2) {
       const std::size_t threads = static_cast<std::size_t>(prm.rows) * ((prm.N + 7) / 8);
@@ -300,11 +384,22 @@ hipError_t launch(const Product& prm, float* parts, int splits, hipStream_t stre
   return hipGetLastError();
 }
 
-template <typename T, class Epi, int MR>
+// Waves that share a sum: so that each has six steps and more, but four where there are
+// four steps.
+template <typename T, class Epi, int MR, int POLICY>
 hipError_t launch_waves(const Product& prm, float* parts, int splits, hipStream_t stream) {
-  const int steps = prm.K / Step<T>::kK / splits;
-  if (steps >= 48) return launch<T, Epi, MR, 8>(prm, parts, splits, stream);
-  return steps >= 8 ? launch<T, Epi, MR, 4>(prm, parts, splits, stream) : launch<T, Epi, MR, 2>(prm, parts, splits, stream);
+  const int steps = (prm.K + Step<T>::kK - 1) / Step<T>::kK / splits;
+  return steps >= 48 ? launch<T, Epi, MR, 8, POLICY>(prm, parts, splits, stream)
+                     : launch<T, Epi, MR, 4, POLICY>(prm, parts, splits, stream);
+}
+
+template <typename T, class Epi, int MR>
+hipError_t launch_policy(const Product& prm, float* parts, int splits, hipStream_t stream) {
+  if constexpr (!Step<T>::kKC) {
+    const std::size_t bytes = static_cast<std::size_t>(std::min(prm.experts, prm.rows)) * prm.K * prm.N * sizeof(T);
+    if (bytes > kStreamedBytes) return launch_waves<T, Epi, MR, kStreamed>(prm, parts, splits, stream);
+  }
+  return launch_waves<T, Epi, MR, kCached>(prm, parts, splits, stream);
 }
 
 }  // namespace
@@ -316,7 +411,7 @@ bool expert_rows_ok(int rows, int experts) {
 
 int expert_rows_splits(int rows, int experts, int columns, int length) {
   if (!expert_rows_ok(rows, experts)) return 1;
-  const int groups = std::min(rows, experts) * ((columns + kCols - 1) / kCols);
+  const int groups = std::min(rows, experts) * ((columns + Step<bf16>::kCols - 1) / Step<bf16>::kCols);
   const int most = std::min(length / 1024, 8);
   return std::max(1, std::min(most, kCus / groups));
 }
@@ -324,8 +419,8 @@ int expert_rows_splits(int rows, int experts, int columns, int length) {
 template <typename T, class Epi>
 hipError_t expert_rows(const Product& prm, float* parts, int splits, hipStream_t stream) {
   const int active = std::min(prm.rows, prm.experts);
-  if (prm.rows <= 16 || prm.rows <= 5 * active) return launch_waves<T, Epi, 1>(prm, parts, splits, stream);
-  return launch_waves<T, Epi, 2>(prm, parts, splits, stream);
+  if (prm.rows <= 16 || prm.rows <= 5 * active) return launch_policy<T, Epi, 1>(prm, parts, splits, stream);
+  return launch_policy<T, Epi, 2>(prm, parts, splits, stream);
 }
 
 template hipError_t expert_rows<bf16, EpiGate<bf16>>(const Product&, float*, int, hipStream_t);
