@@ -290,15 +290,18 @@ __global__ __launch_bounds__(G) void rr_block_norm_backward_kernel(NormParams p,
     if (dn != nullptr) wpre[c].load(static_cast<const T*>(p.pre_weight) + col, left);
   });
   float spre[NV][V] = {}, spost[NV][V] = {}, sgate[NV][V] = {};
-  Raw<T, V> rh[NV], rdh[NV], rdn[NV], rg[NV];
-  Raw<TB, V> rb[NV];
+  // The next row is on its way while one is worked on (1024 threads have no registers for
+  // it).
+  constexpr bool kAhead = G < 1024;
+  Raw<T, V> rh[NV], rdh[NV], rdn[NV], rg[NV], next_h[NV], next_dh[NV], next_dn[NV];
+  Raw<TB, V> rb[NV], next_b[NV];
   auto fetch = [&](int t) {
     const std::size_t row = static_cast<std::size_t>(t) * D;
     for_chunks<V, G, NV>(D, [&](int c, int col, int left) {
-      rh[c].load(h + row + col, left);
-      if (dh != nullptr) rdh[c].load(dh + row + col, left);
-      if (dn != nullptr) rdn[c].load(dn + row + col, left);
-      if (block != nullptr) rb[c].load(block + row + col, left);
+      next_h[c].load(h + row + col, left);
+      if (dh != nullptr) next_dh[c].load(dh + row + col, left);
+      if (dn != nullptr) next_dn[c].load(dn + row + col, left);
+      if (block != nullptr) next_b[c].load(block + row + col, left);
     });
   };
   auto fetch_gate = [&](int t) {
@@ -309,12 +312,21 @@ __global__ __launch_bounds__(G) void rr_block_norm_backward_kernel(NormParams p,
   int first, end;
   part_range(parts, p.tokens, static_cast<int>(blockIdx.x), &first, &end);
   if (first < end) {
-    fetch(first);
+    if (kAhead) fetch(first);
     if (gate != nullptr) fetch_gate(first);
   }
   int until_gate = parts.group;  // tokens to the next gate row, in parts of whole ones
   for (int t = first; t < end; ++t) {
     const std::size_t row = static_cast<std::size_t>(t) * D;
+    if (!kAhead) fetch(t);
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+      rh[c] = next_h[c];
+      rdh[c] = next_dh[c];
+      rdn[c] = next_dn[c];
+      rb[c] = next_b[c];
+    }
+    if (kAhead && t + 1 < end) fetch(t + 1);
     float s[3] = {0.0F, 0.0F, 0.0F};  // h^2, dn pre_weight h, block^2
     for_chunks<V, G, NV>(D, [&](int c, int col, int left) {
       for (int i = 0; i < V; ++i) {
@@ -368,7 +380,6 @@ __global__ __launch_bounds__(G) void rr_block_norm_backward_kernel(NormParams p,
         out.store(static_cast<TB*>(p.dblock) + row + col, left);
       });
     }
-    if (t + 1 < end) fetch(t + 1);
     if (gate != nullptr && parts.per_group == 0 && (--until_gate == 0 || t + 1 == end)) {
       until_gate = parts.group;
       if (p.dgate != nullptr) {
