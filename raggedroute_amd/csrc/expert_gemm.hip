@@ -503,9 +503,12 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
     fetch(stage, 0, 1);
     // A slice takes PH phases of MA x 4 products, each under the fetch of the next one's
     // operands. Before its last phase the slice has been read whole by every wave and the
-    // next slice, loaded since that point of the slice before, has landed: one barrier,
-    // then the next slice's operands are fetched and the slice after it is loaded into
-    // the stage that came free.
+    // next slice, loaded since that point of the slice before, has landed: a barrier, then
+    // the next slice's operands are fetched and the slice after it is loaded into the stage
+    // that came free. Of four phases the third no longer reads B of the slice, whose stage is
+    // then loaded half a slice's worth of loads earlier (all loads at once took the address
+    // unit, 28 cycles each, longer than the products of a slice).
+    constexpr int kLoadB = P::kDirect && PH == 4 ? 2 : PH - 1;  // the phase that loads B
 #pragma unroll 1
     for (int kt = 0; kt < tl.slices; ++kt, ++step) {
       const bool last = kt + 1 == tl.slices;  // (the next tile fetches its own operands)
@@ -513,11 +516,13 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
 #pragma unroll
       for (int p = 0; p < PH; ++p) {
         const int h = p / (PH / 2), i0 = MA * (p % (PH / 2));
-        if (p == PH - 1) {
+        if (p == PH - 1 || p == kLoadB) {
           wait_lds();
-          if constexpr (P::kDirect) wait_loads<0>();
+          if constexpr (P::kDirect) {
+            if (p == PH - 1) wait_loads<kLoadB < PH - 1 ? 4 : 0>();
+          }
           wave_barrier();
-          stage ^= kStageBytes;
+          if (p == PH - 1) stage ^= kStageBytes;
         }
 #pragma unroll
         for (int i = 0; i < MA; ++i) {
@@ -528,14 +533,12 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
               fetch(stage, 0, i);
             }
           }
-          if (p == PH - 1) {
 #pragma unroll
-            for (int q = i * 4 / MA; q < (i + 1) * 4 / MA; ++q) {
-              if (q < QA) put_a(st, q);
-              put_b(st, q);
-              if (q < QA) load_a(st, q);
-              load_b(st, q);
-            }
+          for (int q = i * 4 / MA; q < (i + 1) * 4 / MA; ++q) {
+            if (p == PH - 1 && q < QA) put_a(st, q);
+            if (p == kLoadB) put_b(st, q);
+            if (p == PH - 1 && q < QA) load_a(st, q);
+            if (p == kLoadB) load_b(st, q);
           }
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
