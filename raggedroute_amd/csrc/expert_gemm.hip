@@ -254,8 +254,9 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
   // ---- the stream of slices into LDS ----
   // Wave w brings rows 32 w .. + 31 (KC) or k rows 16 (w % 4) .. + 15 of half w / 4 (KS) of
   // each operand in four loads; half w / 4 is the columns (of KS A: rows of the result)
-  // from 128 on, or in a dual product the right operand b_up. A of a 128-row tile is one
-  // half, brought by all waves in two loads.
+  // from 128 on, or in a dual product the right operand b_up. KC A goes in 16 rows of half
+  // w / 4 from 16 (w % 4) and from 64 + 16 (w % 4), in the order in which the products use
+  // them. A of a 128-row tile is one half, brought by all waves in two loads.
   constexpr int QA = P::kTileRows / 64;  // loads of A
   const int half = wave >> 2;
   const int a_half = P::kTileRows == 256 ? half : 0;
@@ -264,7 +265,9 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
   uint32_t a_lane[QA], b_lane[4], a_chunk = 0, b_chunk[2] = {};
   constexpr int b_bit = P::kDual ? 0 : 1;  // the bit of q that B's chunk depends on (KC)
   auto a_row = [&](int q) {  // KC: row, KS: k
-    return P::kAKC ? 8 * QA * wave + 8 * q + (lane >> 3) : 4 * QA * a_share + 4 * q + (lane >> 4);
+    if constexpr (!P::kAKC) return 4 * QA * a_share + 4 * q + (lane >> 4);
+    const int first = QA == 4 ? 128 * half + 64 * (q >> 1) + 16 * wn + 8 * (q & 1) : 16 * wave + 8 * q;
+    return first + (lane >> 3);
   };
   auto b_row = [&](int q) { return P::kBKC ? 32 * wn + 8 * q + (lane >> 3) : 16 * wn + 4 * q + (lane >> 4); };
 #pragma unroll
@@ -285,7 +288,8 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
   // bytes between slices
   const int64_t a_slice = P::kAKC ? kSliceBytes : static_cast<int64_t>(P::kSlice) * prm.lda * S;
   const int64_t b_slice = P::kBKC ? kSliceBytes : static_cast<int64_t>(P::kSlice) * prm.ldb * S;
-  const uint32_t to_a = lds0 + wave * (QA * 1024);
+  const uint32_t to_a = lds0 + (P::kAKC && QA == 4 ? half * kHalfBytes + wn * 2048 : wave * (QA * 1024));
+  auto a_to = [&](int q) -> uint32_t { return P::kAKC ? (q >> 1) * 8192 + (q & 1) * 1024 : q * 1024; };
   const uint32_t to_b = lds0 + kOperandBytes + wave * 4096;
 
   Tile next;               // the tile whose slices are being loaded
@@ -360,7 +364,7 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
   };
   auto load_a = [&](int stage, int q) {
     if constexpr (P::kDirect) {
-      load_to_lds(make_buffer(a_at, a_left), P::kAKC ? cut(a_lane[q], a_chunk) : a_lane[q], to_a + stage * kStageBytes + q * 1024);
+      load_to_lds(make_buffer(a_at, a_left), P::kAKC ? cut(a_lane[q], a_chunk) : a_lane[q], to_a + stage * kStageBytes + a_to(q));
     } else {
       const int r = a_row(q);
       const int at = static_cast<int>(a_lane[q] - static_cast<uint32_t>(r) * static_cast<uint32_t>(prm.lda) * S);  // chunk
@@ -378,7 +382,7 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
     }
   };
   auto put_a = [&](int stage, int q) {
-    if constexpr (!P::kDirect) *reinterpret_cast<RR_LDS i4*>(to_a + stage * kStageBytes + q * 1024 + lane * 16) = a_held[q];
+    if constexpr (!P::kDirect) *reinterpret_cast<RR_LDS i4*>(to_a + stage * kStageBytes + a_to(q) + lane * 16) = a_held[q];
   };
   auto put_b = [&](int stage, int q) {
     if constexpr (!P::kDirect) *reinterpret_cast<RR_LDS i4*>(to_b + stage * kStageBytes + q * 1024 + lane * 16) = b_held[q];
@@ -463,7 +467,7 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
   auto run_tile = [&](auto mi) {
     constexpr int MI = decltype(mi)::value;  // 16-row fragments of a wave
     constexpr int MA = MI < 4 ? MI : 4;      // of them in a phase
-    constexpr int PH = 2 * MI / MA;          // phases of a slice: k half p / (PH / 2), fragments from MA (p % (PH / 2))
+    constexpr int PH = 2 * MI / MA;          // phases of a slice: k half p % 2, fragments from MA (p / 2)
     Acc acc[MI][4] = {};
     const int wrow = wm * 16 * MI;
     uint32_t a_read[P::kAKC ? 2 : MI];
@@ -490,8 +494,8 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
     i4 a[2][MA], b[2][4];  // of this phase and the next, of both k halves
     // the operands of phase p, in two parts
     auto fetch = [&](uint32_t stage, int p, int part) {
-      const int h = p / (PH / 2), i0 = MA * (p % (PH / 2));
-      if (p % (PH / 2) == 0) {
+      const int h = p % 2, i0 = MA * (p / 2);
+      if (p < 2) {
 #pragma unroll
         for (int j = 2 * part; j < 2 * part + 2; ++j) b[h][j] = read_b(stage, j, h);
       }
@@ -505,21 +509,24 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
     // operands. Before its last phase the slice has been read whole by every wave and the
     // next slice, loaded since that point of the slice before, has landed: a barrier, then
     // the next slice's operands are fetched and the slice after it is loaded into the stage
-    // that came free. Of four phases the third no longer reads B of the slice, whose stage is
-    // then loaded half a slice's worth of loads earlier (all loads at once took the address
-    // unit, 28 cycles each, longer than the products of a slice).
-    constexpr int kLoadB = P::kDirect && PH == 4 ? 2 : PH - 1;  // the phase that loads B
+    // that came free. Of four phases the second no longer reads B of the slice nor, KC, the
+    // first half of A's rows: a barrier there frees them half a slice earlier, and the loads
+    // spread over three phases (all loads at once take the address unit, 28 cycles each,
+    // longer than a phase's products).
+    constexpr bool kSpread = P::kDirect && PH == 4;
+    auto a_phase = [](int q) { return kSpread && P::kAKC && q < 2 ? 2 : PH - 1; };
+    auto b_phase = [](int q) { return !kSpread ? PH - 1 : q < (P::kAKC ? 3 : 2) ? 1 : 2; };
 #pragma unroll 1
     for (int kt = 0; kt < tl.slices; ++kt, ++step) {
       const bool last = kt + 1 == tl.slices;  // (the next tile fetches its own operands)
       const int st = step & 1;
 #pragma unroll
       for (int p = 0; p < PH; ++p) {
-        const int h = p / (PH / 2), i0 = MA * (p % (PH / 2));
-        if (p == PH - 1 || p == kLoadB) {
+        const int h = p % 2, i0 = MA * (p / 2);
+        if (p == PH - 1 || (kSpread && p == 1)) {
           wait_lds();
           if constexpr (P::kDirect) {
-            if (p == PH - 1) wait_loads<kLoadB < PH - 1 ? 4 : 0>();
+            if (p == PH - 1) wait_loads<!kSpread ? 0 : P::kAKC ? 6 : 4>();  // all but this slice's
           }
           wave_barrier();
           if (p == PH - 1) stage ^= kStageBytes;
@@ -535,10 +542,10 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
           }
 #pragma unroll
           for (int q = i * 4 / MA; q < (i + 1) * 4 / MA; ++q) {
-            if (p == PH - 1 && q < QA) put_a(st, q);
-            if (p == kLoadB) put_b(st, q);
-            if (p == PH - 1 && q < QA) load_a(st, q);
-            if (p == kLoadB) load_b(st, q);
+            if (q < QA && p == a_phase(q)) put_a(st, q);
+            if (p == b_phase(q)) put_b(st, q);
+            if (q < QA && p == a_phase(q)) load_a(st, q);
+            if (p == b_phase(q)) load_b(st, q);
           }
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
