@@ -48,9 +48,7 @@ constexpr int kBufferFlags = 0x00027000;  // raw 32-bit buffer
 constexpr uint32_t kPast = 0x80000000U;   // an offset past every record count
 constexpr int kTileCols = 256;
 constexpr int kSliceBytes = 128;              // of every row
-constexpr int kOperandBytes = 256 * kSliceBytes;  // one operand's slice (A of 128-row tiles fills half)
-constexpr int kHalfBytes = kOperandBytes / 2;
-constexpr int kStageBytes = 2 * kOperandBytes;
+constexpr int kHalfBytes = 128 * kSliceBytes;  // half an operand's slice
 constexpr int kThreads = 512;
 
 template <typename T>
@@ -80,13 +78,18 @@ struct Matrix<int8_t> {
 };
 
 // A kernel: element type, whether A and B have k along rows (KC), weight gradients or row
-// products, epilogue, and how slices come: DIRECT into LDS, or through registers.
-template <typename T_, bool A_KC, bool B_KC, bool WEIGHTS, class Epi_, bool DIRECT>
+// products, epilogue, how slices come (DIRECT into LDS, or through registers), and the
+// rows of a tile. Tiles of 128 rows leave room for a third stage of LDS.
+template <typename T_, bool A_KC, bool B_KC, bool WEIGHTS, class Epi_, bool DIRECT, int ROWS>
 struct Kind {
   using T = T_;
   using Epi = Epi_;
   static constexpr bool kAKC = A_KC, kBKC = B_KC, kWeights = WEIGHTS, kDual = Epi_::kDual, kDirect = DIRECT;
-  static constexpr int kTileRows = DIRECT ? 256 : 128;
+  static constexpr int kTileRows = ROWS;
+  static constexpr int kStages = DIRECT && ROWS == 128 ? 3 : 2;
+  static constexpr int kABytes = ROWS * kSliceBytes;  // A's slice
+  static constexpr int kStageBytes = kABytes + kTileCols * kSliceBytes;
+  static_assert(ROWS == 128 || (DIRECT && ROWS == 256), "through registers a tile has 128 rows");
   static constexpr int kSlice = kSliceBytes / sizeof(T_);  // k of a slice
   static constexpr int kCols = kDual ? kTileCols / 2 : kTileCols;
   static_assert(A_KC || sizeof(T_) == 2, "transposing reads are 16-bit");
@@ -174,7 +177,7 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
   constexpr int S = sizeof(T);
   extern __shared__ __align__(16) char smem[];
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((RR_LDS char*)smem));
-  int32_t* s_off = reinterpret_cast<int32_t*>(smem + 2 * kStageBytes);  // [E + 1]
+  int32_t* s_off = reinterpret_cast<int32_t*>(smem + P::kStages * P::kStageBytes);  // [E + 1]
   int32_t* s_pre = s_off + prm.experts + 1;                             // [E + 1] full row tiles before expert e
   int32_t* s_pre2 = s_pre + prm.experts + 1;                            // [E + 1] short row tiles before expert e
   const int tid = static_cast<int>(threadIdx.x);
@@ -214,7 +217,7 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
     if (left <= 0) return false;
     int t = dealt + worker, sub = 0, span = P::kTileRows;
     if (left < grid) {
-      const int cuts = P::kDirect && 4 * left <= grid ? 4 : 2 * left <= grid ? 2 : 1;
+      const int cuts = P::kTileRows == 256 && 4 * left <= grid ? 4 : 2 * left <= grid ? 2 : 1;
       const int mine = mixed ? grid - 1 - worker : static_cast<int>(blockIdx.x);
       sub = mine / left;
       if (sub >= cuts) return false;
@@ -290,7 +293,7 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
   const int64_t b_slice = P::kBKC ? kSliceBytes : static_cast<int64_t>(P::kSlice) * prm.ldb * S;
   const uint32_t to_a = lds0 + (P::kAKC && QA == 4 ? half * kHalfBytes + wn * 2048 : wave * (QA * 1024));
   auto a_to = [&](int q) -> uint32_t { return P::kAKC ? (q >> 1) * 8192 + (q & 1) * 1024 : q * 1024; };
-  const uint32_t to_b = lds0 + kOperandBytes + wave * 4096;
+  const uint32_t to_b = lds0 + P::kABytes + wave * 4096;
 
   Tile next;               // the tile whose slices are being loaded
   int dealt = 0;           // its round
@@ -362,30 +365,30 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
     }
     return __builtin_bit_cast(i4, v);
   };
-  auto load_a = [&](int stage, int q) {
+  auto load_a = [&](uint32_t stage, int q) {
     if constexpr (P::kDirect) {
-      load_to_lds(make_buffer(a_at, a_left), P::kAKC ? cut(a_lane[q], a_chunk) : a_lane[q], to_a + stage * kStageBytes + a_to(q));
+      load_to_lds(make_buffer(a_at, a_left), P::kAKC ? cut(a_lane[q], a_chunk) : a_lane[q], to_a + stage + a_to(q));
     } else {
       const int r = a_row(q);
       const int at = static_cast<int>(a_lane[q] - static_cast<uint32_t>(r) * static_cast<uint32_t>(prm.lda) * S);  // chunk
       a_held[q] = read_cut(a_at, a_lane[q], r < a_rows ? a_width - at : 0);
     }
   };
-  auto load_b = [&](int stage, int q) {
+  auto load_b = [&](uint32_t stage, int q) {
     if constexpr (P::kDirect) {
       load_to_lds(make_buffer(b_at, b_left), P::kBKC ? cut(b_lane[q], b_chunk[(q >> b_bit) & 1]) : b_lane[q],
-                  to_b + stage * kStageBytes + q * 1024);
+                  to_b + stage + q * 1024);
     } else {
       const int r = b_row(q);
       const int at = static_cast<int>(b_lane[q] - static_cast<uint32_t>(r) * static_cast<uint32_t>(prm.ldb) * S);
       b_held[q] = read_cut(b_at, b_lane[q], r < b_rows ? b_width - at : 0);
     }
   };
-  auto put_a = [&](int stage, int q) {
-    if constexpr (!P::kDirect) *reinterpret_cast<RR_LDS i4*>(to_a + stage * kStageBytes + a_to(q) + lane * 16) = a_held[q];
+  auto put_a = [&](uint32_t stage, int q) {
+    if constexpr (!P::kDirect) *reinterpret_cast<RR_LDS i4*>(to_a + stage + a_to(q) + lane * 16) = a_held[q];
   };
-  auto put_b = [&](int stage, int q) {
-    if constexpr (!P::kDirect) *reinterpret_cast<RR_LDS i4*>(to_b + stage * kStageBytes + q * 1024 + lane * 16) = b_held[q];
+  auto put_b = [&](uint32_t stage, int q) {
+    if constexpr (!P::kDirect) *reinterpret_cast<RR_LDS i4*>(to_b + stage + q * 1024 + lane * 16) = b_held[q];
   };
   auto advance = [&]() {  // to the next slice
     if (!open) return;
@@ -409,12 +412,12 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
   uint32_t b_read[2];  // per k half (KC), per fragment pair (KS)
   if constexpr (P::kBKC) {
     const int r = (P::kDual ? 32 * wn + 8 * (li >> 2) : 64 * (wn & 1) + 16 * (li >> 2)) + (li & 3);
-    const uint32_t base = lds0 + kOperandBytes + (P::kDual ? 0 : (wn >> 1) * kHalfBytes) + r * kSliceBytes;
+    const uint32_t base = lds0 + P::kABytes + (P::kDual ? 0 : (wn >> 1) * kHalfBytes) + r * kSliceBytes;
 #pragma unroll
     for (int h = 0; h < 2; ++h) b_read[h] = base + (static_cast<uint32_t>((4 * h + g) ^ swizzle_b_row<P::kDual>(r)) << 4);
   } else {
     const int k = 8 * g + (li >> 2);
-    const uint32_t base = lds0 + kOperandBytes + (P::kDual ? 0 : (wn >> 1) * kHalfBytes) + k * 256;
+    const uint32_t base = lds0 + P::kABytes + (P::kDual ? 0 : (wn >> 1) * kHalfBytes) + k * 256;
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
       const int chunk = P::kDual ? 4 * wn + (li & 3) : 8 * (wn & 1) + 2 * (li & 3) + v;
@@ -436,21 +439,21 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
   if (!open) return;
   Tile tl = next;
 #pragma unroll
-  for (int st = 0; st < 2; ++st) {
+  for (int st = 0; st < P::kStages; ++st) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      if (q < QA) load_a(st, q);
-      load_b(st, q);
+      if (q < QA) load_a(st * P::kStageBytes, q);
+      load_b(st * P::kStageBytes, q);
     }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      if (q < QA) put_a(st, q);
-      put_b(st, q);
+      if (q < QA) put_a(st * P::kStageBytes, q);
+      put_b(st * P::kStageBytes, q);
     }
     advance();
   }
   if constexpr (P::kDirect) {
-    wait_loads<8>();
+    wait_loads<(P::kStages - 1) * (QA + 4)>();
   } else {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {  // (the third slice, on its way)
@@ -461,7 +464,7 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
     wait_lds();
   }
   wave_barrier();
-  int step = 0;  // slices multiplied: the stage is step & 1
+  uint32_t stage = 0;  // of the slice to be multiplied
   int round = 0;
 
   auto run_tile = [&](auto mi) {
@@ -502,7 +505,6 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
 #pragma unroll
       for (int i = part * (MA / 2); i < (part + 1) * (MA / 2); ++i) a[p & 1][i] = read_a(stage, i0 + i, h);
     };
-    uint32_t stage = (step & 1) * kStageBytes;
     fetch(stage, 0, 0);
     fetch(stage, 0, 1);
     // A slice takes PH phases of MA x 4 products, each under the fetch of the next one's
@@ -517,19 +519,19 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
     auto a_phase = [](int q) { return kSpread && P::kAKC && q < 2 ? 2 : PH - 1; };
     auto b_phase = [](int q) { return !kSpread ? PH - 1 : q < (P::kAKC ? 3 : 2) ? 1 : 2; };
 #pragma unroll 1
-    for (int kt = 0; kt < tl.slices; ++kt, ++step) {
+    for (int kt = 0; kt < tl.slices; ++kt) {
       const bool last = kt + 1 == tl.slices;  // (the next tile fetches its own operands)
-      const int st = step & 1;
+      const uint32_t st = stage;
 #pragma unroll
       for (int p = 0; p < PH; ++p) {
         const int h = p % 2, i0 = MA * (p / 2);
         if (p == PH - 1 || (kSpread && p == 1)) {
           wait_lds();
           if constexpr (P::kDirect) {
-            if (p == PH - 1) wait_loads<!kSpread ? 0 : P::kAKC ? 6 : 4>();  // all but this slice's
+            if (p == PH - 1) wait_loads<kSpread ? (P::kAKC ? 6 : 4) : (P::kStages - 2) * (QA + 4)>();  // the next slice's
           }
           wave_barrier();
-          if (p == PH - 1) stage ^= kStageBytes;
+          if (p == PH - 1) stage = stage == (P::kStages - 1) * P::kStageBytes ? 0 : stage + P::kStageBytes;
         }
 #pragma unroll
         for (int i = 0; i < MA; ++i) {
@@ -587,8 +589,8 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
 
 #pragma unroll 1
   for (;;) {
-    if (P::kDirect && tl.rows > 128) {
-      if constexpr (P::kDirect) run_tile(std::integral_constant<int, 8>{});
+    if (P::kTileRows == 256 && tl.rows > 128) {
+      if constexpr (P::kTileRows == 256) run_tile(std::integral_constant<int, 8>{});
     } else if (tl.rows > 64) {
       run_tile(std::integral_constant<int, 4>{});
     } else {
@@ -622,27 +624,27 @@ hipError_t launch(const Product& prm, hipStream_t stream) {
                                 : prm.rows / 64 + std::min<long>(prm.experts, prm.rows);
   long grid = std::min<long>(cols * rows, cu_count());
   if (grid >= kXcds) grid = grid / kXcds * kXcds;
-  const std::size_t lds = 2 * kStageBytes + 3 * static_cast<std::size_t>(prm.experts + 1) * sizeof(int32_t);
+  const std::size_t lds = P::kStages * P::kStageBytes + 3 * static_cast<std::size_t>(prm.experts + 1) * sizeof(int32_t);
   rr_expert_gemm_kernel<P><<<dim3(static_cast<unsigned>(grid)), kThreads, lds, stream>>>(prm);
   return hipGetLastError();
 }
 
-template <typename T, bool DIRECT>
-using GateUp = Kind<T, true, false, false, EpiGate<T>, DIRECT>;  // x [Wg | Wu]
-template <typename T, bool DIRECT>
-using Down = Kind<T, true, false, false, EpiStore<T>, DIRECT>;  // a Wd
-template <typename T, bool DIRECT>
-using DGateUp = Kind<T, true, true, false, EpiDGate<T>, DIRECT>;  // dy Wd^T
-template <typename T, bool DIRECT>
-using Dx = Kind<T, true, true, false, EpiStore<T>, DIRECT>;  // dg Wg^T + du Wu^T
-template <typename T, bool DIRECT>
-using DwPair = Kind<T, false, false, true, EpiPair<T>, DIRECT>;  // x^T [dg | du]
-template <typename T, bool DIRECT>
-using Dw = Kind<T, false, false, true, EpiStore<T>, DIRECT>;  // a^T dy
-template <typename T, bool DIRECT>
-using Int8 = Kind<int8_t, true, true, false, EpiInt8<T>, DIRECT>;
-template <typename T, bool DIRECT>
-using Int8Gate = Kind<int8_t, true, true, false, EpiInt8Gate<T>, DIRECT>;
+template <typename T, bool DIRECT, int ROWS>
+using GateUp = Kind<T, true, false, false, EpiGate<T>, DIRECT, ROWS>;  // x [Wg | Wu]
+template <typename T, bool DIRECT, int ROWS>
+using Down = Kind<T, true, false, false, EpiStore<T>, DIRECT, ROWS>;  // a Wd
+template <typename T, bool DIRECT, int ROWS>
+using DGateUp = Kind<T, true, true, false, EpiDGate<T>, DIRECT, ROWS>;  // dy Wd^T
+template <typename T, bool DIRECT, int ROWS>
+using Dx = Kind<T, true, true, false, EpiStore<T>, DIRECT, ROWS>;  // dg Wg^T + du Wu^T
+template <typename T, bool DIRECT, int ROWS>
+using DwPair = Kind<T, false, false, true, EpiPair<T>, DIRECT, ROWS>;  // x^T [dg | du]
+template <typename T, bool DIRECT, int ROWS>
+using Dw = Kind<T, false, false, true, EpiStore<T>, DIRECT, ROWS>;  // a^T dy
+template <typename T, bool DIRECT, int ROWS>
+using Int8 = Kind<int8_t, true, true, false, EpiInt8<T>, DIRECT, ROWS>;
+template <typename T, bool DIRECT, int ROWS>
+using Int8Gate = Kind<int8_t, true, true, false, EpiInt8Gate<T>, DIRECT, ROWS>;
 
 // Loads straight into LDS need every row of every operand on a 16-byte boundary.
 bool aligned16(std::initializer_list<const void*> pointers) {
@@ -650,6 +652,24 @@ bool aligned16(std::initializer_list<const void*> pointers) {
     if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return false;
   }
   return true;
+}
+
+// Tiles of 128 rows and a third stage where an expert has 192 rows or fewer on average: fewer
+// rows of zeros are multiplied, and slices that come from HBM have twice the time to land
+// (8192 rows of 64 experts, K = 1024, N = 512: the four row products of a training step 166
+// us against 207, the gradient of Wd 39 against 43). With more rows weights would be read
+// again for every 128 of them (32768 rows of 128 experts, K = 2048, N = 768: gate and up 314
+// us against 288). The paired weight gradients, whose tiles are mostly stores, keep 256 rows
+// (64 us against 70).
+template <typename T, bool DIRECT, template <typename, bool, int> class K>
+hipError_t launch_kind(const Product& p, hipStream_t stream) {
+  if constexpr (!DIRECT) {
+    return launch<K<T, false, 128>>(p, stream);
+  } else if constexpr (K<T, true, 256>::kWeights && K<T, true, 256>::kDual) {
+    return launch<K<T, true, 256>>(p, stream);
+  } else {
+    return p.rows <= 192L * p.experts ? launch<K<T, true, 128>>(p, stream) : launch<K<T, true, 256>>(p, stream);
+  }
 }
 
 Product base_of(const FfnParams& f) {
@@ -677,7 +697,7 @@ hipError_t forward(const FfnParams& f, hipStream_t stream) {
   const bool few = expert_rows_ok(f.rows, f.experts);
   int splits = expert_rows_splits(f.rows, f.experts, f.inner, f.hidden);
   const hipError_t error = few ? expert_rows<T, EpiGate<T>>(p, splits > 1 ? f.parts : nullptr, splits, stream)
-                               : launch<GateUp<T, DIRECT>>(p, stream);
+                               : launch_kind<T, DIRECT, GateUp>(p, stream);
   if (error != hipSuccess) return error;
   p = base_of(f);
   p.a = f.act;
@@ -688,7 +708,7 @@ hipError_t forward(const FfnParams& f, hipStream_t stream) {
   p.K = f.inner;
   p.lda = f.inner;
   p.ldb = f.output;
-  if (!few) return launch<Down<T, DIRECT>>(p, stream);
+  if (!few) return launch_kind<T, DIRECT, Down>(p, stream);
   splits = expert_rows_splits(f.rows, f.experts, f.output, f.inner);
   return expert_rows<T, EpiStore<T>>(p, splits > 1 ? f.parts : nullptr, splits, stream);
 }
@@ -707,7 +727,7 @@ hipError_t backward(const FfnParams& f, hipStream_t stream) {
     p.N = f.inner;
     p.K = f.output;
     p.lda = p.ldb = f.output;
-    error = launch<DGateUp<T, DIRECT>>(p, stream);
+    error = launch_kind<T, DIRECT, DGateUp>(p, stream);
   }
   if (error == hipSuccess && f.rows != 0 && f.dx != nullptr) {
     Product p = base_of(f);
@@ -719,7 +739,7 @@ hipError_t backward(const FfnParams& f, hipStream_t stream) {
     p.N = f.hidden;
     p.K = f.inner;
     p.lda = p.ldb = f.inner;
-    error = launch<Dx<T, DIRECT>>(p, stream);
+    error = launch_kind<T, DIRECT, Dx>(p, stream);
   }
   if (error == hipSuccess && f.dw_gate != nullptr) {
     Product p = base_of(f);
@@ -732,7 +752,7 @@ hipError_t backward(const FfnParams& f, hipStream_t stream) {
     p.N = f.inner;
     p.lda = f.hidden;
     p.ldb = f.inner;
-    error = launch<DwPair<T, DIRECT>>(p, stream);
+    error = launch_kind<T, DIRECT, DwPair>(p, stream);
   }
   if (error == hipSuccess && f.dw_down != nullptr) {
     Product p = base_of(f);
@@ -743,7 +763,7 @@ hipError_t backward(const FfnParams& f, hipStream_t stream) {
     p.N = f.output;
     p.lda = f.inner;
     p.ldb = f.output;
-    error = launch<Dw<T, DIRECT>>(p, stream);
+    error = launch_kind<T, DIRECT, Dw>(p, stream);
   }
   return error;
 }
@@ -769,8 +789,8 @@ hipError_t int8_product(const Int8Params& f, hipStream_t stream) {
     return f.w_up != nullptr ? expert_rows<int8_t, EpiInt8Gate<T>>(p, nullptr, 1, stream)
                              : expert_rows<int8_t, EpiInt8<T>>(p, nullptr, 1, stream);
   }
-  return f.w_up != nullptr ? launch<Int8Gate<T, DIRECT>>(p, stream)
-                           : launch<Int8<T, DIRECT>>(p, stream);
+  return f.w_up != nullptr ? launch_kind<T, DIRECT, Int8Gate>(p, stream)
+                           : launch_kind<T, DIRECT, Int8>(p, stream);
 }
 
 }  // namespace
