@@ -194,6 +194,16 @@ def test_backward_longer_sums(device, counts, k, f, n):
     check_backward(v, backward(b, counts, rows, k, f, n, "bf16", "silu"), counts, "bf16", "silu")
 
 
+@pytest.mark.parametrize("counts,k,f,n", [([256, 0, 600], 264, 136, 392), ([257, 511, 300], 64, 520, 72),
+                                          ([1000], 200, 264, 128)])
+@pytest.mark.parametrize("dtype,act", [("bf16", "silu"), ("f16", "gelu")])
+def test_many_rows_an_expert(device, counts, k, f, n, dtype, act):
+    """Segments on both sides of 256 rows and of its cuts, slices and columns that end inside."""
+    v, b, rows = make(counts, k, f, n, dtype, seed=11)
+    check_forward(v, forward(b, counts, rows, k, f, n, dtype, act), counts, dtype, act)
+    check_backward(v, backward(b, counts, rows, k, f, n, dtype, act), counts, dtype, act)
+
+
 @pytest.mark.parametrize("skip", [("dx",), ("dw_gate", "dw_up"), ("dw_down",), ("dx", "dw_down")])
 def test_backward_unwanted_gradients(device, skip):
     counts, k, f, n = [20, 0, 9], 72, 40, 64
