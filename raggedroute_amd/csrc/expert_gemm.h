@@ -173,7 +173,7 @@ struct EpiInt8Gate {
 
 // ---- few rows an expert (expert_rows.hip) ----
 // Whether the kernel for few rows takes a row product of this many rows.
-bool expert_rows_ok(int rows, int experts);
+bool expert_rows_ok(int rows, int experts, bool int8);
 // Workgroups that share an expert's sum of `length` (1: no parts are needed).
 int expert_rows_splits(int rows, int experts, int columns, int length);
 // parts: FP32 [1, dual products 2][splits][rows][N] where splits > 1 (16-bit products only).

@@ -654,13 +654,15 @@ bool aligned16(std::initializer_list<const void*> pointers) {
   return true;
 }
 
-// Tiles of 128 rows and a third stage where an expert has 192 rows or fewer on average: fewer
-// rows of zeros are multiplied, and slices that come from HBM have twice the time to land
-// (8192 rows of 64 experts, K = 1024, N = 512: the four row products of a training step 166
-// us against 207, the gradient of Wd 39 against 43). With more rows weights would be read
-// again for every 128 of them (32768 rows of 128 experts, K = 2048, N = 768: gate and up 314
-// us against 288). The paired weight gradients, whose tiles are mostly stores, keep 256 rows
-// (64 us against 70).
+// Tiles of 128 rows and a third stage where an expert has 160 rows or fewer on average (int8:
+// 96): fewer rows of zeros are multiplied, tiles divide better among the CUs, and slices
+// that come from HBM have twice the time to land (8192 rows of 64 experts, K = 1024, N =
+// 512: the four row products of a training step 166 us against 207, the gradient of Wd 39
+// against 43; a forward pass of 8192 rows of 128 experts, K = 2048, F = 768, 311 us against
+// 345). With more rows weights would be read again for every 128 of them (32768 rows of
+// those experts: gate and up 314 us against 288; int8, K = 2048, N = 768: 8192 rows 146 us
+// against 163, but 1024 rows of eight experts, K = 4096, N = 14336, 206 against 184). The
+// paired weight gradients, whose tiles are mostly stores, keep 256 rows (64 us against 70).
 template <typename T, bool DIRECT, template <typename, bool, int> class K>
 hipError_t launch_kind(const Product& p, hipStream_t stream) {
   if constexpr (!DIRECT) {
@@ -668,7 +670,8 @@ hipError_t launch_kind(const Product& p, hipStream_t stream) {
   } else if constexpr (K<T, true, 256>::kWeights && K<T, true, 256>::kDual) {
     return launch<K<T, true, 256>>(p, stream);
   } else {
-    return p.rows <= 192L * p.experts ? launch<K<T, true, 128>>(p, stream) : launch<K<T, true, 256>>(p, stream);
+    constexpr long kFew = sizeof(typename K<T, true, 256>::T) == 1 ? 96 : 160;
+    return p.rows <= kFew * p.experts ? launch<K<T, true, 128>>(p, stream) : launch<K<T, true, 256>>(p, stream);
   }
 }
 
@@ -694,7 +697,7 @@ hipError_t forward(const FfnParams& f, hipStream_t stream) {
   p.K = f.hidden;
   p.lda = f.hidden;
   p.ldb = f.inner;
-  const bool few = expert_rows_ok(f.rows, f.experts);
+  const bool few = expert_rows_ok(f.rows, f.experts, false);
   int splits = expert_rows_splits(f.rows, f.experts, f.inner, f.hidden);
   const hipError_t error = few ? expert_rows<T, EpiGate<T>>(p, splits > 1 ? f.parts : nullptr, splits, stream)
                                : launch_kind<T, DIRECT, GateUp>(p, stream);
@@ -785,7 +788,7 @@ hipError_t int8_product(const Int8Params& f, hipStream_t stream) {
   p.N = f.output;
   p.K = f.hidden;
   p.lda = p.ldb = f.hidden;
-  if (expert_rows_ok(f.rows, f.experts)) {
+  if (expert_rows_ok(f.rows, f.experts, true)) {
     return f.w_up != nullptr ? expert_rows<int8_t, EpiInt8Gate<T>>(p, nullptr, 1, stream)
                              : expert_rows<int8_t, EpiInt8<T>>(p, nullptr, 1, stream);
   }

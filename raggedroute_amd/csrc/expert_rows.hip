@@ -2,7 +2,7 @@
 // read once from memory, straight into registers in matrix-operand order.
 //
 // A workgroup of W waves takes 128 columns (int8: 64) of one expert (of each right operand) and its
-// rows in blocks of 16 MR; the waves share the sum's length and add up through LDS in a
+// rows 16 at a time; the waves share the sum's length and add up through LDS in a
 // fixed order. What bounds it is memory: a wave has 8 to 16 loads of 1 KB in flight and
 // never passes weights through LDS.
 //  - 16-bit weights lie [K, N]: a lane (i, g) loads 8 columns 8 i .. + 7 of the k rows 8 g .. + 7
@@ -126,7 +126,7 @@ __device__ __forceinline__ int find_expert(const Product& p, int index, int* fir
 }
 
 // (waves a SIMD: what the accumulators and the two sets of weights leave room for)
-template <typename T, class Epi, int MR, int W, int POLICY>
+template <typename T, class Epi, int W, int POLICY>
 __global__ __launch_bounds__(64 * W, Epi::kDual ? 2 : 3) void rr_expert_rows_kernel(Product prm, float* parts, int splits, int blocks) {
   using M = Step<T>;
   using Acc = typename M::acc;
@@ -136,7 +136,7 @@ __global__ __launch_bounds__(64 * W, Epi::kDual ? 2 : 3) void rr_expert_rows_ker
   constexpr int X = kKC ? 2 : 1;       // matrix instructions of a step for each
   constexpr int V = 16 / sizeof(T);    // elements of a load
   extern __shared__ __align__(16) char smem[];
-  i4* lds = reinterpret_cast<i4*>(smem);  // [W / 2][B * C * MR][64]
+  i4* lds = reinterpret_cast<i4*>(smem);  // [W / 2][B * C][64]
   const int lane = static_cast<int>(threadIdx.x) & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int li = lane & 15, g = lane >> 4;
@@ -159,15 +159,13 @@ __global__ __launch_bounds__(64 * W, Epi::kDual ? 2 : 3) void rr_expert_rows_ker
                          reinterpret_cast<uintptr_t>(weights[1]) | sizeof(T) * K | (kKC ? 0 : sizeof(T) * N)) & 3) == 0;
 
 #pragma unroll 1
-  for (int r0 = 0; r0 < count; r0 += 16 * MR) {
-    Acc acc[B][C][MR] = {};
+  for (int r0 = 0; r0 < count; r0 += 16) {
+    Acc acc[B][C] = {};
     // byte offsets of the lane: of its rows (rows past the last repeat it: their results
     // are not stored) and in the weights
     constexpr uint32_t S = sizeof(T);
     const T* x = static_cast<const T*>(prm.a) + static_cast<std::size_t>(first + r0) * K;
-    uint32_t x_at[MR];
-#pragma unroll
-    for (int i = 0; i < MR; ++i) x_at[i] = S * (static_cast<uint32_t>(min(16 * i + li, count - 1 - r0)) * static_cast<uint32_t>(K) + g * V);
+    const uint32_t x_at = S * (static_cast<uint32_t>(min(li, count - 1 - r0)) * static_cast<uint32_t>(K) + g * V);
     uint32_t w_at[kKC ? 4 : 1];
 #pragma unroll
     for (int j = 0; j < (kKC ? 4 : 1); ++j) {
@@ -175,7 +173,7 @@ __global__ __launch_bounds__(64 * W, Epi::kDual ? 2 : 3) void rr_expert_rows_ker
                     : S * (static_cast<uint32_t>(8 * g) * static_cast<uint32_t>(N) + 8 * li);
     }
     struct Rows {
-      i4 v[MR][X];
+      i4 v[X];
     };
     struct Weights {
       i4 v[8];
@@ -184,10 +182,7 @@ __global__ __launch_bounds__(64 * W, Epi::kDual ? 2 : 3) void rr_expert_rows_ker
     auto load_rows = [&](Rows& o, int s, auto whole) {
 #pragma unroll
       for (int h = 0; h < X; ++h) {
-#pragma unroll
-        for (int i = 0; i < MR; ++i) {
-          o.v[i][h] = load16<decltype(whole)::value, kCached>(x + s * M::kK, S * 4 * h * V, x_at[i], K - s * M::kK - (4 * h + g) * V);
-        }
+        o.v[h] = load16<decltype(whole)::value, kCached>(x + s * M::kK, S * 4 * h * V, x_at, K - s * M::kK - (4 * h + g) * V);
       }
     };
     auto load_weights = [&](Weights& o, int b, int s, auto whole) {
@@ -214,10 +209,7 @@ __global__ __launch_bounds__(64 * W, Epi::kDual ? 2 : 3) void rr_expert_rows_ker
       for (int c = 0; c < C; ++c) {
         if constexpr (kKC) {
 #pragma unroll
-          for (int h = 0; h < X; ++h) {
-#pragma unroll
-            for (int i = 0; i < MR; ++i) acc[b][c][i] = M::mul(w.v[2 * c + h], r.v[i][h], acc[b][c][i]);
-          }
+          for (int h = 0; h < X; ++h) acc[b][c] = M::mul(w.v[2 * c + h], r.v[h], acc[b][c]);
         } else {
           i4 column;
 #pragma unroll
@@ -226,8 +218,7 @@ __global__ __launch_bounds__(64 * W, Epi::kDual ? 2 : 3) void rr_expert_rows_ker
                                                                static_cast<uint32_t>(w.v[2 * m][c >> 1]),
                                                                (c & 1) != 0 ? 0x07060302U : 0x05040100U));
           }
-#pragma unroll
-          for (int i = 0; i < MR; ++i) acc[b][c][i] = M::mul(column, r.v[i][0], acc[b][c][i]);
+          acc[b][c] = M::mul(column, r.v[0], acc[b][c]);
         }
       }
     };
@@ -288,47 +279,44 @@ __global__ __launch_bounds__(64 * W, Epi::kDual ? 2 : 3) void rr_expert_rows_ker
     for (int half = W / 2; half >= 1; half /= 2) {
       if (wave >= half && wave < 2 * half) {
 #pragma unroll
-        for (int q = 0; q < B * C * MR; ++q) {
-          lds[((wave - half) * B * C * MR + q) * 64 + lane] = __builtin_bit_cast(i4, acc[q / (C * MR)][q / MR % C][q % MR]);
+        for (int q = 0; q < B * C; ++q) {
+          lds[((wave - half) * B * C + q) * 64 + lane] = __builtin_bit_cast(i4, acc[q / C][q % C]);
         }
       }
       __syncthreads();
       if (wave < half) {
 #pragma unroll
-        for (int q = 0; q < B * C * MR; ++q) {
-          acc[q / (C * MR)][q / MR % C][q % MR] += __builtin_bit_cast(Acc, lds[(wave * B * C * MR + q) * 64 + lane]);
+        for (int q = 0; q < B * C; ++q) {
+          acc[q / C][q % C] += __builtin_bit_cast(Acc, lds[(wave * B * C + q) * 64 + lane]);
         }
       }
       __syncthreads();
     }
     if (wave != 0) continue;
-    // lane: row 16 i + li; columns 32 g + 8 r + 0..7 (KC: 16 j + 4 g + 0..3)
+    // lane: row li; columns 32 g + 8 r + 0..7 (KC: 16 j + 4 g + 0..3)
+    const int r = r0 + li;
+    if (r >= count) continue;
+    const std::size_t row = static_cast<std::size_t>(first) + r;
+    constexpr int E = kKC ? 4 : 8;  // columns of a store
 #pragma unroll
-    for (int i = 0; i < MR; ++i) {
-      const int r = r0 + 16 * i + li;
-      if (r >= count) continue;
-      const std::size_t row = static_cast<std::size_t>(first) + r;
-      constexpr int E = kKC ? 4 : 8;  // columns of a store
+    for (int p = 0; p < 4; ++p) {
+      const int n = n0 + (kKC ? 16 * p + 4 * g : 32 * g + 8 * p);
+      if (n >= N) continue;
+      float v[B][E];
 #pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        const int n = n0 + (kKC ? 16 * p + 4 * g : 32 * g + 8 * p);
-        if (n >= N) continue;
-        float v[B][E];
+      for (int b = 0; b < B; ++b) {
+#pragma unroll
+        for (int q = 0; q < E; ++q) v[b][q] = static_cast<float>(kKC ? acc[b][p][q] : acc[b][q][p]);
+      }
+      if (parts != nullptr) {
 #pragma unroll
         for (int b = 0; b < B; ++b) {
-#pragma unroll
-          for (int q = 0; q < E; ++q) v[b][q] = static_cast<float>(kKC ? acc[b][p][i][q] : acc[b][q][i][p]);
+          Cols<float, E>::store(parts + (static_cast<std::size_t>(b * splits + split) * prm.rows + row) * N + n, v[b], N - n);
         }
-        if (parts != nullptr) {
-#pragma unroll
-          for (int b = 0; b < B; ++b) {
-            Cols<float, E>::store(parts + (static_cast<std::size_t>(b * splits + split) * prm.rows + row) * N + n, v[b], N - n);
-          }
-        } else if constexpr (Epi::kDual) {
-          Epi::template emit<E>(prm, e, row, n, N - n, v[0], v[1]);
-        } else {
-          Epi::template emit<E>(prm, e, row, n, N - n, v[0]);
-        }
+      } else if constexpr (Epi::kDual) {
+        Epi::template emit<E>(prm, e, row, n, N - n, v[0], v[1]);
+      } else {
+        Epi::template emit<E>(prm, e, row, n, N - n, v[0]);
       }
     }
   }
@@ -363,17 +351,13 @@ __global__ __launch_bounds__(256) void rr_expert_rows_sum_kernel(Product prm, co
   }
 }
 
-template <typename T, class Epi, int MR, int W, int POLICY>
+template <typename T, class Epi, int W, int POLICY>
 hipError_t launch(const Product& prm, float* parts, int splits, hipStream_t stream) {
-  constexpr std::size_t lds = static_cast<std::size_t>(W / 2) * (Epi::kDual ? 2 : 1) * (Step<T>::kKC ? 4 : 8) * MR * 64 * sizeof(i4);
-  if constexpr (lds > 64 * 1024) {
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(rr_expert_rows_kernel<T, Epi, MR, W, POLICY>),
-                                                       hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-    if (attr != hipSuccess) return attr;
-  }
+  constexpr std::size_t lds = static_cast<std::size_t>(W / 2) * (Epi::kDual ? 2 : 1) * (Step<T>::kKC ? 4 : 8) * 64 * sizeof(i4);
+  static_assert(lds <= 64 * 1024, "no attribute raises the limit");
   const int blocks = (prm.N + Step<T>::kCols - 1) / Step<T>::kCols;
   const std::size_t grid = static_cast<std::size_t>(std::min(prm.experts, prm.rows)) * blocks * splits;
-  rr_expert_rows_kernel<T, Epi, MR, W, POLICY><<<dim3(static_cast<unsigned>(grid)), 64 * W, lds, stream>>>(prm, parts, splits, blocks);
+  rr_expert_rows_kernel<T, Epi, W, POLICY><<<dim3(static_cast<unsigned>(grid)), 64 * W, lds, stream>>>(prm, parts, splits, blocks);
   if (splits > 1) {
     if constexpr (sizeof(T) == 2) {
       const std::size_t threads = static_cast<std::size_t>(prm.rows) * ((prm.N + 7) / 8);
@@ -386,31 +370,26 @@ hipError_t launch(const Product& prm, float* parts, int splits, hipStream_t stre
 
 // Waves that share a sum: so that each has six steps and more, but four where there are
 // four steps.
-template <typename T, class Epi, int MR, int POLICY>
+template <typename T, class Epi, int POLICY>
 hipError_t launch_waves(const Product& prm, float* parts, int splits, hipStream_t stream) {
   const int steps = (prm.K + Step<T>::kK - 1) / Step<T>::kK / splits;
-  return steps >= 48 ? launch<T, Epi, MR, 8, POLICY>(prm, parts, splits, stream)
-                     : launch<T, Epi, MR, 4, POLICY>(prm, parts, splits, stream);
-}
-
-template <typename T, class Epi, int MR>
-hipError_t launch_policy(const Product& prm, float* parts, int splits, hipStream_t stream) {
-  if constexpr (!Step<T>::kKC) {
-    const std::size_t bytes = static_cast<std::size_t>(std::min(prm.experts, prm.rows)) * prm.K * prm.N * sizeof(T);
-    if (bytes > kStreamedBytes) return launch_waves<T, Epi, MR, kStreamed>(prm, parts, splits, stream);
-  }
-  return launch_waves<T, Epi, MR, kCached>(prm, parts, splits, stream);
+  return steps >= 48 ? launch<T, Epi, 8, POLICY>(prm, parts, splits, stream)
+                     : launch<T, Epi, 4, POLICY>(prm, parts, splits, stream);
 }
 
 }  // namespace
 
-bool expert_rows_ok(int rows, int experts) {
-  const int active = std::min(rows, experts);
-  return rows <= 16 || rows <= 24 * active;
+// Five rows an expert on average, of int8 three: tiles then multiply 64 rows for every few,
+// but an expert's weights are read once however many rows it has, and here again for every
+// 16 (E = 128, K = 2048, F = 768, skewed: 512 rows 233 us, tiles 248; 768 rows 270, tiles
+// 250; 1024 rows 293, tiles 249; E = 8, K = 4096, F = 14336: 16 rows 463, tiles 558; int8,
+// E = 128, K = 2048, N = 768: 384 rows 115, tiles 114; 640 rows 127, tiles 113).
+bool expert_rows_ok(int rows, int experts, bool int8) {
+  return rows <= 16 || rows <= (int8 ? 3 : 5) * std::min(rows, experts);
 }
 
 int expert_rows_splits(int rows, int experts, int columns, int length) {
-  if (!expert_rows_ok(rows, experts)) return 1;
+  if (!expert_rows_ok(rows, experts, false)) return 1;
   const int groups = std::min(rows, experts) * ((columns + Step<bf16>::kCols - 1) / Step<bf16>::kCols);
   const int most = std::min(length / 1024, 8);
   return std::max(1, std::min(most, kCus / groups));
@@ -418,9 +397,11 @@ int expert_rows_splits(int rows, int experts, int columns, int length) {
 
 template <typename T, class Epi>
 hipError_t expert_rows(const Product& prm, float* parts, int splits, hipStream_t stream) {
-  const int active = std::min(prm.rows, prm.experts);
-  if (prm.rows <= 16 || prm.rows <= 5 * active) return launch_policy<T, Epi, 1>(prm, parts, splits, stream);
-  return launch_policy<T, Epi, 2>(prm, parts, splits, stream);
+  if constexpr (!Step<T>::kKC) {
+    const std::size_t bytes = static_cast<std::size_t>(std::min(prm.experts, prm.rows)) * prm.K * prm.N * sizeof(T);
+    if (bytes > kStreamedBytes) return launch_waves<T, Epi, kStreamed>(prm, parts, splits, stream);
+  }
+  return launch_waves<T, Epi, kCached>(prm, parts, splits, stream);
 }
 
 template hipError_t expert_rows<bf16, EpiGate<bf16>>(const Product&, float*, int, hipStream_t);

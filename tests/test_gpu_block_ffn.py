@@ -194,6 +194,15 @@ def test_backward_longer_sums(device, counts, k, f, n):
     check_backward(v, backward(b, counts, rows, k, f, n, "bf16", "silu"), counts, "bf16", "silu")
 
 
+@pytest.mark.parametrize("k,f,n", [(2048, 40, 72), (40, 264, 17), (256, 128, 256)])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_few_rows_and_a_long_expert(device, k, f, n, dtype):
+    """Few rows an expert on average, but one expert with more than a block of them."""
+    counts = [0, 37, 0, 1, 2] + [0] * 7
+    v, b, rows = make(counts, k, f, n, dtype, seed=12)
+    check_forward(v, forward(b, counts, rows, k, f, n, dtype), counts, dtype, "silu")
+
+
 @pytest.mark.parametrize("counts,k,f,n", [([256, 0, 600], 264, 136, 392), ([257, 511, 300], 64, 520, 72),
                                           ([1000], 200, 264, 128)])
 @pytest.mark.parametrize("dtype,act", [("bf16", "silu"), ("f16", "gelu")])

@@ -91,6 +91,7 @@ SHAPES = [
     ([129, 64, 1], 257, 130),
     ([256, 300], 128, 264),
     ([600, 9], 1040, 512),
+    ([0, 37, 0, 1, 2] + [0] * 9, 272, 96),
 ]
 
 
