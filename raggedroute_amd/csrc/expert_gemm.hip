@@ -301,9 +301,8 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
   int slice = 0;           // its slice to be loaded
   const char *a_at, *b_at;  // the slice of each operand, and the bytes to the operand's end from there
   int64_t a_left, b_left;
-  int k_left;  // bytes of a row's sum from the slice on
-  // through registers: rows (k rows) of each operand from the slice on, and bytes of them from its first column
-  int a_rows = 0, b_rows = 0, a_width = 0, b_width = 0;
+  int k_left;      // bytes of a row's sum from the slice on
+  int k_rows = 0;  // through registers: k rows of KS operands from the slice on
   auto start_part = [&](int part) {
     const char* a = static_cast<const char*>(part == 0 ? prm.a : prm.a2);
     const char* b = static_cast<const char*>(P::kDual ? (half == 0 ? prm.b : prm.b_up) : part == 0 ? prm.b : prm.b_up);
@@ -316,9 +315,7 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
       a_left = m < prm.M ? (rows * prm.lda - m) * S : 0;
       b_at = b + (static_cast<int64_t>(next.first) * prm.ldb + n) * S;
       b_left = n < prm.N ? (rows * prm.ldb - n) * S : 0;
-      a_rows = b_rows = static_cast<int>(rows);
-      a_width = (prm.M - m) * S;
-      b_width = (prm.N - n) * S;
+      k_rows = static_cast<int>(rows);
     } else {
       a_at = a + static_cast<int64_t>(next.row0) * prm.lda * S;
       a_left = static_cast<int64_t>(next.rows) * prm.lda * S;
@@ -330,10 +327,7 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
         b_left = n < prm.N ? (static_cast<int64_t>(prm.K) * prm.ldb - n) * S : 0;
       }
       k_left = prm.K * S;
-      a_rows = next.rows;
-      a_width = k_left;
-      b_rows = P::kBKC ? prm.N - n : prm.K;
-      b_width = P::kBKC ? k_left : (prm.N - n) * S;
+      k_rows = prm.K;
     }
   };
   auto start_tile = [&]() {
@@ -343,62 +337,94 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
       start_part(0);
     } else {
       a_left = b_left = 0;
-      a_rows = b_rows = 0;
     }
   };
   auto cut = [&](uint32_t offset, uint32_t chunk) { return static_cast<int>(chunk) < k_left ? offset : kPast; };
+  // (record counts in whole words do not end a KS operand exactly)
+  auto cut_row = [&](uint32_t offset, int k) { return P::kDirect || k < k_rows ? offset : kPast; };
   // The wave's load q of each operand's slice. Direct: into the stage. Through registers:
-  // `put` writes what the last `load` of the same q brought, 16 bytes of any alignment;
-  // chunks that a row's or the operand's end cuts are read element by element.
-  i4 a_held[P::kDirect ? 1 : QA], b_held[P::kDirect ? 1 : 4];
-  // 16 bytes at `at` + offset, of which the first `bytes` exist
-  auto read_cut = [&](const char* at, uint32_t offset, int bytes) -> i4 {
-    typedef T chunk __attribute__((ext_vector_type(16 / S), aligned(S)));
-    chunk v = {};
-    if (bytes >= 16) {
-      v = *reinterpret_cast<const chunk*>(at + offset);
-    } else {
+  // `put` writes what the last `load` of the same q brought. Chunks of any alignment come as
+  // the five aligned words that they touch, shifted together when they are put (one load of
+  // 16 bytes off a word boundary takes the address unit several times as long: 6002 rows of
+  // eight experts, K = 1023, F = 1535: 393 us); the last chunk of a row's sum, which a row's
+  // end may cut (KC), is cleared behind it there.
+  struct Held {
+    i4 v;
+    int more;
+  };
+  Held a_held[P::kDirect ? 1 : QA], b_held[P::kDirect ? 1 : 4];
+  uint32_t a_skew = 0, b_skew = 0;  // of the held slice: its start past a word's,
+  int k_held = 0;                   // and the bytes of a row's sum from it on
+  auto load_words = [&](const char* at, int64_t left, uint32_t offset) {
+    const uint32_t skew = reinterpret_cast<uintptr_t>(at) & 3;
+    // (records to the end of the word that holds the operand's last element)
+    const int64_t records = left <= 0 ? 0 : (left + skew + 3) & ~static_cast<int64_t>(3);
+    const auto buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(at - skew), 0,
+                                                          static_cast<int>(records < 0x7FFFFFFC ? records : 0x7FFFFFFC), kBufferFlags);
+    const int from = static_cast<int>((offset + skew) & ~3U);
+    Held h;
+    h.v = __builtin_bit_cast(i4, __builtin_amdgcn_raw_buffer_load_b128(buffer, from, 0, 0));
+    h.more = static_cast<int>(__builtin_amdgcn_raw_buffer_load_b32(buffer, from + 16, 0, 0));
+    return h;
+  };
+  auto joined = [&](const Held& h, uint32_t offset, uint32_t chunk, bool along_k) {
+    const uint32_t shift = (offset & 3) * 8;
+    i4 o;
 #pragma unroll
-      for (int i = 0; i < 16 / S; ++i) {
-        if (i * S < bytes) v[i] = *reinterpret_cast<const T*>(at + offset + i * S);
+    for (int i = 0; i < 4; ++i) {
+      o[i] = static_cast<int>(__builtin_amdgcn_alignbit(static_cast<uint32_t>(i < 3 ? h.v[i < 3 ? i + 1 : 3] : h.more), static_cast<uint32_t>(h.v[i]), shift));
+    }
+    if (along_k && k_held < kSliceBytes) {
+      const int bytes = k_held - static_cast<int>(chunk);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int n = bytes - 4 * i;
+        o[i] = n >= 4 ? o[i] : n <= 0 ? 0 : o[i] & ((1 << (8 * n)) - 1);
       }
     }
-    return __builtin_bit_cast(i4, v);
+    return o;
   };
   auto load_a = [&](uint32_t stage, int q) {
+    const uint32_t offset = P::kAKC ? cut(a_lane[q], a_chunk) : cut_row(a_lane[q], a_row(q));
     if constexpr (P::kDirect) {
-      load_to_lds(make_buffer(a_at, a_left), P::kAKC ? cut(a_lane[q], a_chunk) : a_lane[q], to_a + stage + a_to(q));
+      load_to_lds(make_buffer(a_at, a_left), offset, to_a + stage + a_to(q));
     } else {
-      const int r = a_row(q);
-      const int at = static_cast<int>(a_lane[q] - static_cast<uint32_t>(r) * static_cast<uint32_t>(prm.lda) * S);  // chunk
-      a_held[q] = read_cut(a_at, a_lane[q], r < a_rows ? a_width - at : 0);
+      a_held[q] = load_words(a_at, a_left, offset);
     }
   };
   auto load_b = [&](uint32_t stage, int q) {
+    const uint32_t offset = P::kBKC ? cut(b_lane[q], b_chunk[(q >> b_bit) & 1]) : cut_row(b_lane[q], b_row(q));
     if constexpr (P::kDirect) {
-      load_to_lds(make_buffer(b_at, b_left), P::kBKC ? cut(b_lane[q], b_chunk[(q >> b_bit) & 1]) : b_lane[q],
-                  to_b + stage + q * 1024);
+      load_to_lds(make_buffer(b_at, b_left), offset, to_b + stage + q * 1024);
     } else {
-      const int r = b_row(q);
-      const int at = static_cast<int>(b_lane[q] - static_cast<uint32_t>(r) * static_cast<uint32_t>(prm.ldb) * S);
-      b_held[q] = read_cut(b_at, b_lane[q], r < b_rows ? b_width - at : 0);
+      b_held[q] = load_words(b_at, b_left, offset);
     }
   };
   auto put_a = [&](uint32_t stage, int q) {
-    if constexpr (!P::kDirect) *reinterpret_cast<RR_LDS i4*>(to_a + stage + a_to(q) + lane * 16) = a_held[q];
+    if constexpr (!P::kDirect) {
+      *reinterpret_cast<RR_LDS i4*>(to_a + stage + a_to(q) + lane * 16) = joined(a_held[q], a_lane[q] + a_skew, a_chunk, P::kAKC);
+    }
   };
   auto put_b = [&](uint32_t stage, int q) {
-    if constexpr (!P::kDirect) *reinterpret_cast<RR_LDS i4*>(to_b + stage + q * 1024 + lane * 16) = b_held[q];
+    if constexpr (!P::kDirect) {
+      *reinterpret_cast<RR_LDS i4*>(to_b + stage + q * 1024 + lane * 16) =
+          joined(b_held[q], b_lane[q] + b_skew, b_chunk[(q >> b_bit) & 1], P::kBKC);
+    }
+  };
+  auto hold = [&]() {  // notes what `put` has to know of the slice just loaded
+    a_skew = reinterpret_cast<uintptr_t>(a_at) & 3;
+    b_skew = reinterpret_cast<uintptr_t>(b_at) & 3;
+    k_held = k_left;
   };
   auto advance = [&]() {  // to the next slice
+    if constexpr (!P::kDirect) hold();
     if (!open) return;
     a_at += a_slice;
     a_left -= a_slice;
     b_at += b_slice;
     b_left -= b_slice;
     k_left -= kSliceBytes;
-    if (P::kAKC) a_width -= kSliceBytes; else a_rows -= P::kSlice;
-    if (P::kBKC) b_width -= kSliceBytes; else b_rows -= P::kSlice;
+    k_rows -= P::kSlice;
     ++slice;
     if (slice == next.slices) {
       dealt += grid;
@@ -445,6 +471,7 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
       if (q < QA) load_a(st * P::kStageBytes, q);
       load_b(st * P::kStageBytes, q);
     }
+    if constexpr (!P::kDirect) hold();
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       if (q < QA) put_a(st * P::kStageBytes, q);
