@@ -7,6 +7,10 @@
 // V-element (16-byte) chunks t, t + G, ...; the last chunk of a row is cut element by
 // element, so rows of any width and alignment take one path (a row that starts off a
 // 16-byte boundary only splits its accesses over cache lines).
+//
+// BF16 rows of 4096, each tensor once: 16384 rows forward (x, block, h, n) 100 us = 5.4 TB/s;
+// 8192 rows backward (h, block, dh, dn, dx, dblock) 88 us = 4.6 TB/s and 8 us for the
+// columns' sums; a copy of that size reaches 4.75 TB/s.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -116,7 +116,10 @@ struct EpiGate {
   }
 };
 
-// sums = da: out = d gate, out_up = d up, from gate (in) and up (in_up)
+// sums = da: out = d gate, out_up = d up, from gate (in) and up (in_up). Both are rounded to T
+// once, as operands of the matrix instructions; with g and u kept in T the gradients are
+// off by 1.8 times the rounding of their own result (FP32 copies of g and u, 1.4 times,
+// would double what a step keeps of every row).
 template <typename T>
 struct EpiDGate {
   static constexpr bool kDual = false;

@@ -4,7 +4,9 @@
 // A workgroup of W waves takes 128 columns (int8: 64) of one expert (of each right operand) and its
 // rows 16 at a time; the waves share the sum's length and add up through LDS in a
 // fixed order. What bounds it is memory: a wave has 8 to 16 loads of 1 KB in flight and
-// never passes weights through LDS.
+// never passes weights through LDS (one token, two experts, K = 4096, F = 14336: 470 MB of
+// gate and up in 84 us = 5.6 TB/s, of a pure read's 7.1; the same rows on tiles of 128 rows
+// 558 us for all eight experts' forward pass, here 463).
 //  - 16-bit weights lie [K, N]: a lane (i, g) loads 8 columns 8 i .. + 7 of the k rows 8 g .. + 7
 //    of a 32-k step and turns that 8 x 8 block (32 byte permutes); register c then holds
 //    eight k of column 8 i + c, the operand of one v_mfma_f32_16x16x32: the order of the
