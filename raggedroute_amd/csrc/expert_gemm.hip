@@ -142,9 +142,12 @@ __device__ __forceinline__ i4 make_buffer(const char* at, int64_t left) {
   return i4{__builtin_amdgcn_readfirstlane(static_cast<int>(p)), __builtin_amdgcn_readfirstlane(static_cast<int>(p >> 32) & 0xFFFF),
             __builtin_amdgcn_readfirstlane(records), kBufferFlags};
 }
-// 64 lanes x 16 bytes from `buffer` (a byte offset per lane) to LDS at `to` (uniform).
+// 64 lanes x 16 bytes from `buffer` (a byte offset per lane) to LDS at `to` (uniform). The
+// compiler may have written a word of the descriptor with a vector instruction (a lane read)
+// just before, which has to be five wait states ahead of a load that reads it, and it does
+// not look into assembly: the move and s_nop 3 are five.
 __device__ __forceinline__ void load_to_lds(i4 buffer, uint32_t offset, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(
                    __builtin_amdgcn_readfirstlane(static_cast<int>(to))),
                "v"(offset), "s"(buffer)
                : "memory");
