@@ -150,7 +150,7 @@ __device__ __forceinline__ void load_to_lds(i4 buffer, uint32_t offset, uint32_t
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(
                    __builtin_amdgcn_readfirstlane(static_cast<int>(to))),
                "v"(offset), "s"(buffer)
-               : "memory");
+               : "memory", "m0");
 }
 
 __device__ __forceinline__ i4 read16(uint32_t at) { return *reinterpret_cast<RR_LDS const i4*>(at); }

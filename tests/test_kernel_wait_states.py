@@ -131,6 +131,18 @@ def test_the_reader_sees_a_short_distance():
     assert too_early(near, [[], [], [1], [2, 0], [3]], ["f"] * 5)
 
 
+def test_assembly_names_m0_where_it_writes_it():
+    """m0 is the compiler's, too (LDS loads of its own, lane and register indexes): an
+    assembly statement that writes it lists it among its clobbers."""
+    writers = 0
+    for source in sorted((REPO / "raggedroute_amd" / "csrc").glob("*")):
+        for statement in re.findall(r"\basm\b.*?;", source.read_text(), re.S):
+            if re.search(r"s_mov\w*\s+m0", statement):
+                writers += 1
+                assert re.search(r":[^:]*\"m0\"[^:]*\)\s*;$", statement), f"{source.name}: {statement}"
+    assert writers > 0
+
+
 @pytest.mark.skipif(not LIBRARY.exists() or not OBJDUMP.exists(), reason="needs the built library and llvm-objdump")
 def test_scalar_registers_of_loads_and_stores(tmp_path):
     objects = list(code_objects(LIBRARY.read_bytes()))
