@@ -239,35 +239,38 @@ struct Parts {
 
 constexpr int kSumThreads = 131072;  // threads of all parts together, about eight waves a CU
 
+// (counts of tokens go up to 2^31 - 1: sums of two of them, and a part's place in a gate row
+// that ends early, pass 31 bits)
 Parts make_parts(const NormParams& p, int threads) {
   Parts s{};
   if (p.tokens == 0) return s;
-  const int want = std::max(1L, (static_cast<long>(p.tokens) * threads + kSumThreads - 1) / kSumThreads);
+  auto divide = [](int64_t a, int64_t by) { return static_cast<int>((a + by - 1) / by); };
+  const int want = std::max(1, divide(static_cast<int64_t>(p.tokens) * threads, kSumThreads));
   s.group = p.gate != nullptr ? std::min(p.gate_tokens, p.tokens) : p.tokens;
   if (s.group >= want) {
-    const int split = (s.group + want - 1) / want;
-    s.tokens = (s.group + split - 1) / split;
-    s.per_group = (s.group + s.tokens - 1) / s.tokens;
-    s.count = (p.tokens + s.group - 1) / s.group * s.per_group;
+    s.tokens = divide(s.group, divide(s.group, want));
+    s.per_group = divide(s.group, s.tokens);
+    s.count = divide(p.tokens, s.group) * s.per_group;
   } else {
     s.tokens = want / s.group * s.group;
-    s.count = (p.tokens + s.tokens - 1) / s.tokens;
+    s.count = divide(p.tokens, s.tokens);
   }
   return s;
 }
 
 // First and one past the last token of a part (a part of a short last gate row may be empty).
 __device__ __forceinline__ void part_range(const Parts& s, int tokens, int part, int* first, int* end) {
+  int64_t from, stop;
   if (s.per_group != 0) {
     const int g = part / s.per_group;
-    const int from = g * s.group + (part - g * s.per_group) * s.tokens;
-    const int stop = min(min((g + 1) * s.group, from + s.tokens), tokens);
-    *first = min(from, stop);
-    *end = stop;
+    from = static_cast<int64_t>(g) * s.group + static_cast<int64_t>(part - g * s.per_group) * s.tokens;
+    stop = min(static_cast<int64_t>(g + 1) * s.group, from + s.tokens);
   } else {
-    *first = part * s.tokens;
-    *end = min(*first + s.tokens, tokens);
+    from = static_cast<int64_t>(part) * s.tokens;
+    stop = from + s.tokens;
   }
+  *end = static_cast<int>(min(stop, static_cast<int64_t>(tokens)));
+  *first = static_cast<int>(min(from, static_cast<int64_t>(*end)));
 }
 
 // Column sums of part `part`: [0] pre_weight, [1] post_weight, [2] gate.

@@ -1,0 +1,57 @@
+"""The expert block's operators at the ends of their ranges: row counts next to 2^31."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import raggedroute_amd as rr
+from block_helpers import CODES, context
+
+pytestmark = pytest.mark.gpu
+MOST = 2 ** 31 - 1
+BF16 = torch.bfloat16
+
+
+def signs(seed):
+    """2^31 - 1 values of 1 and -1, and the same as BF16."""
+    gen = torch.Generator(device="cuda:0")
+    gen.manual_seed(seed)
+    return torch.randint(0, 2, (MOST,), device="cuda:0", generator=gen, dtype=torch.int8).mul_(2).sub_(1)
+
+
+def pieces():
+    step = 1 << 28
+    return [slice(at, min(at + step, MOST)) for at in range(0, MOST, step)]
+
+
+@pytest.mark.parametrize("gate_tokens", [0, 1500000000])
+def test_norm_gradients_of_most_tokens(device, gate_tokens):
+    """dblock = scale gate dh, dgate = sum of scale block dh over a gate row. Signs, powers of
+    two and a block of ones: the sums of up to 2^31 halves are exact in FP32 as long as
+    parts of 2^20 and totals stay below 2^23 (a sum of n random signs is about n^0.5)."""
+    sign = signs(1)
+    dh, block = sign.to(BF16), torch.ones(MOST, dtype=BF16, device="cuda:0")
+    dx, dblock = torch.full_like(dh, float("nan")), torch.full_like(dh, float("nan"))
+    gate = torch.tensor([[2.0], [0.25]], dtype=BF16, device="cuda:0")
+    dgate = torch.full_like(gate, float("nan"))
+    args = rr.BlockNormBackwardArgs(
+        h=dh.data_ptr(), block=block.data_ptr(), gate=gate.data_ptr() if gate_tokens else None, gate_tokens=gate_tokens,
+        dh=dh.data_ptr(), dx=dx.data_ptr(), dblock=dblock.data_ptr(), dgate=dgate.data_ptr() if gate_tokens else None,
+        residual_scale=0.5, tokens=MOST, hidden=1, dtype=CODES["bf16"])
+    ctx, ws = context(rr.get_block_norm_backward_workspace_size(args))
+    status = rr.block_norm_backward(args, ctx)
+    assert status.ok(), status.message
+    assert ws.intact()
+    sums = [0, 0]
+    for piece in pieces():
+        assert torch.equal(dx[piece], dh[piece])
+        want = 0.5 * sign[piece].float()
+        if gate_tokens:
+            second = torch.arange(piece.start, piece.stop, device="cuda:0") >= gate_tokens
+            want = torch.where(second, want * 0.25, want * 2.0)
+            sums[0] += sign[piece][~second].sum(dtype=torch.int64).item()
+            sums[1] += sign[piece][second].sum(dtype=torch.int64).item()
+        assert torch.equal(dblock[piece], want.to(BF16))
+    if gate_tokens:
+        assert max(map(abs, sums)) < 2 ** 23
+        assert torch.equal(dgate.cpu(), torch.tensor(sums).mul(0.5).to(BF16)[:, None])
