@@ -99,6 +99,12 @@ __device__ __forceinline__ void for_chunks(int D, F f) {
   }
 }
 
+// The workgroup's row after `row`, `rows` where there is none (a sum of the two may pass 31 bits).
+__device__ __forceinline__ int next_row(int row, int rows) {
+  const int step = static_cast<int>(gridDim.x);
+  return rows - row > step ? row + step : rows;
+}
+
 template <typename T, typename TB, int G, int NV>
 __global__ __launch_bounds__(G) void rr_block_norm_kernel(NormParams p) {
   constexpr int V = kChunk<T>;
@@ -128,7 +134,7 @@ __global__ __launch_bounds__(G) void rr_block_norm_kernel(NormParams p) {
   };
   int t = static_cast<int>(blockIdx.x);
   if (t < p.tokens) fetch(t);
-  for (; t < p.tokens; t += static_cast<int>(gridDim.x)) {
+  for (; t < p.tokens; t = next_row(t, p.tokens)) {
     const std::size_t row = static_cast<std::size_t>(t) * D;
     float h[NV][V];
     float scale = p.scale;
@@ -153,7 +159,7 @@ __global__ __launch_bounds__(G) void rr_block_norm_kernel(NormParams p) {
         ss[0] = __builtin_fmaf(v, v, ss[0]);
       }
     });
-    const int next = t + static_cast<int>(gridDim.x);
+    const int next = next_row(t, p.tokens);
     if (next < p.tokens) fetch(next);
     if (p.h != nullptr) {
       for_chunks<V, G, NV>(D, [&](int c, int col, int left) {
@@ -184,7 +190,7 @@ __global__ __launch_bounds__(1024) void rr_block_norm_wide_kernel(NormParams p) 
   const float inv = 1.0F / static_cast<float>(D);
   const auto* block = static_cast<const TB*>(p.block);
   const auto* wpost = static_cast<const T*>(p.post_weight);
-  for (int t = static_cast<int>(blockIdx.x); t < p.tokens; t += static_cast<int>(gridDim.x)) {
+  for (int t = static_cast<int>(blockIdx.x); t < p.tokens; t = next_row(t, p.tokens)) {
     const std::size_t row = static_cast<std::size_t>(t) * D;
     const T* gate = p.gate != nullptr ? static_cast<const T*>(p.gate) + static_cast<std::size_t>(t / p.gate_tokens) * D : nullptr;
     float scale = p.scale;
@@ -555,7 +561,7 @@ template <typename T, int G, int NV>
 __global__ __launch_bounds__(G) void rr_quantize_rows_kernel(const T* x, int8_t* q, float* scales, int rows, int D) {
   constexpr int V = kChunk<T>;
   __shared__ uint32_t lds[G / 64];
-  for (int t = static_cast<int>(blockIdx.x); t < rows; t += static_cast<int>(gridDim.x)) {
+  for (int t = static_cast<int>(blockIdx.x); t < rows; t = next_row(t, rows)) {
     const std::size_t row = static_cast<std::size_t>(t) * D;
     Raw<T, V> v[NV];
     uint32_t top = 0;
@@ -583,7 +589,7 @@ template <typename T>
 __global__ __launch_bounds__(1024) void rr_quantize_rows_wide_kernel(const T* x, int8_t* q, float* scales, int rows, int D) {
   constexpr int G = 1024;
   __shared__ uint32_t lds[G / 64];
-  for (int t = static_cast<int>(blockIdx.x); t < rows; t += static_cast<int>(gridDim.x)) {
+  for (int t = static_cast<int>(blockIdx.x); t < rows; t = next_row(t, rows)) {
     const std::size_t row = static_cast<std::size_t>(t) * D;
     uint32_t top = 0;
     for (int col = threadIdx.x; col < D; col += G) top = max(top, magnitude(static_cast<float>(x[row + col])));

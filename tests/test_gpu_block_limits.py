@@ -55,3 +55,33 @@ def test_norm_gradients_of_most_tokens(device, gate_tokens):
     if gate_tokens:
         assert max(map(abs, sums)) < 2 ** 23
         assert torch.equal(dgate.cpu(), torch.tensor(sums).mul(0.5).to(BF16)[:, None])
+
+
+def test_norm_of_most_tokens(device):
+    """n = x w / sqrt(x^2 + eps) = the sign of x times w, within two half units of BF16 (eps is
+    2^-20 of x^2, FP32 steps are smaller still)."""
+    sign = signs(2)
+    x, n = sign.to(BF16), torch.full((MOST,), float("nan"), dtype=BF16, device="cuda:0")
+    w = torch.full((1,), 3.0, dtype=BF16, device="cuda:0")
+    args = rr.BlockNormArgs(x=x.data_ptr(), pre_weight=w.data_ptr(), n=n.data_ptr(), tokens=MOST, hidden=1,
+                            dtype=CODES["bf16"])
+    ctx, _ = context()
+    status = rr.block_norm(args, ctx)
+    assert status.ok(), status.message
+    for piece in pieces():
+        assert ((n[piece].float() - 3.0 * sign[piece]).abs() <= 2 * 2.0 ** -8 * 3.0).all()
+
+
+def test_quantize_most_rows(device):
+    """A row of one value: q = 127 times its sign, scale = its magnitude over 127."""
+    sign = signs(3)
+    x = sign.to(BF16)
+    q = torch.zeros(MOST, dtype=torch.int8, device="cuda:0")
+    scale = torch.zeros(MOST, dtype=torch.float32, device="cuda:0")
+    ctx, _ = context()
+    status = rr.quantize_rows(rr.QuantizeRowsArgs(x=x.data_ptr(), q=q.data_ptr(), scale=scale.data_ptr(), rows=MOST,
+                                                  hidden=1, dtype=CODES["bf16"]), ctx)
+    assert status.ok(), status.message
+    one = torch.tensor(1.0, device="cuda:0") / torch.tensor(127.0, device="cuda:0")
+    for piece in pieces():
+        assert torch.equal(q[piece], 127 * sign[piece]) and (scale[piece] == one).all()
