@@ -175,6 +175,11 @@ __device__ __forceinline__ void place_tile(int t, int row_tiles, int col_tiles, 
   *ct = within / rows;
 }
 
+// Slices of `rows` rows, one at least.
+__host__ __device__ constexpr int slices_of(int rows, int slice) { return rows > 0 ? (rows - 1) / slice + 1 : 1; }
+static_assert(slices_of(0, 64) == 1 && slices_of(64, 64) == 1 && slices_of(65, 64) == 2);
+static_assert(slices_of(0x7FFFFFFF, 64) == 1 << 25, "a sum with the slice would pass 31 bits");
+
 // An output tile (uniform).
 struct Tile {
   int e;           // expert
@@ -248,7 +253,7 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
       tl.row0 = rt * P::kTileRows;
       tl.rows = min(prm.M - tl.row0, P::kTileRows);
       // (an expert without rows takes one slice of zeros)
-      tl.slices = count > P::kSlice ? (count + P::kSlice - 1) / P::kSlice : 1;
+      tl.slices = slices_of(count, P::kSlice);
     } else {
       // (an expert's tiles lie together, so that those which run side by side share weights)
       const bool is_short = t >= total_full;
