@@ -435,8 +435,9 @@ void rr_chain_graph_cache_destroy(rr_chain_graph_cache* cache);
  * RR_DTYPE_BF16 (the norms and quantize_rows also RR_DTYPE_FP32). Sums are FP32
  * (int32 for int8 products). Inputs and outputs must not overlap unless a field
  * says so. Offsets are read on the device only: rising from 0, offsets[experts]
- * <= rows; larger or negative ones are cut to [0, rows] and falling ones give
- * empty experts. Rows past offsets[experts] are neither read nor written. The
+ * <= rows; larger or negative ones are cut to [0, rows], and one that falls counts as
+ * the largest before it, so that its expert is empty and no row belongs to two. Rows
+ * before the first expert's and past the last one's are neither read nor written. The
  * kernel families of the other operators apply: auto and optimized (id 950) run the gfx950 kernels, naive one thread per output. Entries allocate and
  * synchronise nothing and may be captured into graphs.
  */

@@ -40,7 +40,8 @@ __device__ __forceinline__ void activation_grad(int kind, float g, float* act, f
   *grad = s + b * slope * (s * (1.0F - s));
 }
 
-// offsets[e] cut to [0, rows]
+// offsets[e] cut to [0, rows]. Segments are bounded by the largest of these up to theirs: an
+// offset that falls leaves its expert empty, and no row belongs to two experts.
 __device__ __forceinline__ int offset_at(const int32_t* offsets, int e, int rows) {
   const int o = offsets[e];
   return o < 0 ? 0 : o > rows ? rows : o;

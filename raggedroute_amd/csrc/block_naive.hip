@@ -30,10 +30,18 @@ __device__ __forceinline__ void for_outputs(std::size_t count, F f) {
   for (std::size_t i = static_cast<std::size_t>(blockIdx.x) * kThreads + threadIdx.x; i < count; i += stride) f(i);
 }
 
-// The expert whose segment holds `row` (the first, where falling offsets make several), or -1.
+// First row of expert e: the largest offset up to its own.
+__device__ int first_row(const int32_t* offsets, int e, int rows) {
+  int most = 0;
+  for (int i = 0; i <= e; ++i) most = max(most, offset_at(offsets, i, rows));
+  return most;
+}
+
+// The expert whose segment holds `row`, or -1.
 __device__ int expert_of(const int32_t* offsets, int experts, int rows, int row) {
+  if (row < offset_at(offsets, 0, rows)) return -1;
   for (int e = 0; e < experts; ++e) {
-    if (row >= offset_at(offsets, e, rows) && row < offset_at(offsets, e + 1, rows)) return e;
+    if (row < offset_at(offsets, e + 1, rows)) return e;
   }
   return -1;
 }
@@ -132,7 +140,7 @@ __global__ void rr_ffn_dw_naive_kernel(const T* a, const T* b, T* dw, const int3
   for_outputs(experts * I * J, [&](std::size_t o) {
     const int e = static_cast<int>(o / (I * J));
     const std::size_t i = o / J % I, j = o % J;
-    const int first = offset_at(offsets, e, rows), end = offset_at(offsets, e + 1, rows);
+    const int first = first_row(offsets, e, rows), end = max(first, offset_at(offsets, e + 1, rows));
     float s = 0.0F;
     for (int r = first; r < end; ++r) s = __builtin_fmaf(static_cast<float>(a[r * I + i]), static_cast<float>(b[r * J + j]), s);
     dw[o] = static_cast<T>(s);

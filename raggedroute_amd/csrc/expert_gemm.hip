@@ -180,6 +180,24 @@ __host__ __device__ constexpr int slices_of(int rows, int slice) { return rows >
 static_assert(slices_of(0, 64) == 1 && slices_of(64, 64) == 1 && slices_of(65, 64) == 2);
 static_assert(slices_of(0x7FFFFFFF, 64) == 1 << 25, "a sum with the slice would pass 31 bits");
 
+// The offsets in s_off[0 .. experts] to the segments' bounds: the largest of each and those
+// before it. By one whole wave, whose own reads afterwards see them.
+__device__ __forceinline__ void raise_offsets(int32_t* s_off, int experts, int lane) {
+  const int per = experts / 64 + 1;  // entries of a lane
+  int32_t most = 0;
+  for (int j = 0; j < per; ++j) {
+    const int e = lane * per + j;
+    if (e <= experts) most = max(most, s_off[e]);
+  }
+  const int32_t before = __shfl_up(rr::dev::wave_inclusive_max(most), 1, 64);
+  most = lane > 0 ? before : 0;
+  for (int j = 0; j < per; ++j) {
+    const int e = lane * per + j;
+    if (e <= experts) s_off[e] = most = max(most, s_off[e]);
+  }
+  rr::dev::wave_lds_sync();
+}
+
 // An output tile (uniform).
 struct Tile {
   int e;           // expert
@@ -209,10 +227,11 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
 
   for (int e = tid; e <= experts; e += kThreads) s_off[e] = rr::dev::offset_at(prm.offsets, e, prm.rows);
   __syncthreads();
-  if constexpr (!P::kWeights) {
-    if (wave == 0) build_tile_prefix<P::kTileRows, true>(s_off, s_pre, s_pre2, experts, lane);
-    __syncthreads();
+  if (wave == 0) {
+    raise_offsets(s_off, experts, lane);
+    if constexpr (!P::kWeights) build_tile_prefix<P::kTileRows, true>(s_off, s_pre, s_pre2, experts, lane);
   }
+  __syncthreads();
   const int col_tiles = (prm.N + P::kCols - 1) / P::kCols;
   const int m_tiles = P::kWeights ? (prm.M + P::kTileRows - 1) / P::kTileRows : 0;
   const int full_rows = P::kWeights ? 0 : __builtin_amdgcn_readfirstlane(s_pre[experts]);
@@ -328,8 +347,7 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
     const char* b = static_cast<const char*>(P::kDual ? (half == 0 ? prm.b : prm.b_up) : part == 0 ? prm.b : prm.b_up);
     const int n = next.n0 + (P::kDual ? 0 : half * 128);
     if constexpr (P::kWeights) {
-      const int count = s_off[next.e + 1] - next.first;
-      const int64_t rows = __builtin_amdgcn_readfirstlane(count > 0 ? count : 0);
+      const int64_t rows = __builtin_amdgcn_readfirstlane(s_off[next.e + 1] - next.first);
       const int m = next.row0 + a_half * 128;
       a_at = a + (static_cast<int64_t>(next.first) * prm.lda + m) * S;
       a_left = m < prm.M ? (rows * prm.lda - m) * S : 0;

@@ -25,6 +25,7 @@
 #include <type_traits>
 
 #include "expert_gemm.h"
+#include "wave.h"
 
 namespace rr::kern {
 namespace {
@@ -106,13 +107,18 @@ __device__ __forceinline__ i4 load16(const T* base, uint32_t offset, uint32_t la
 // The `index`-th expert that has rows (-1: there are fewer), by one wave's lanes.
 __device__ __forceinline__ int find_expert(const Product& p, int index, int* first, int* count) {
   const int lane = static_cast<int>(threadIdx.x) & 63;
+  int most = 0;  // bound of the experts before
   for (int e0 = 0; e0 < p.experts; e0 += 64) {
     const int e = e0 + lane;
-    int from = 0, rows = 0;
+    int from = 0, to = 0;
     if (e < p.experts) {
       from = rr::dev::offset_at(p.offsets, e, p.rows);
-      rows = rr::dev::offset_at(p.offsets, e + 1, p.rows) - from;
+      to = rr::dev::offset_at(p.offsets, e + 1, p.rows);
     }
+    from = max(most, rr::dev::wave_inclusive_max(from));
+    to = max(from, to);
+    const int rows = to - from;
+    most = __builtin_amdgcn_readlane(to, 63);
     uint64_t some = __ballot(rows > 0);
     const int here = __popcll(some);
     if (index < here) {
@@ -324,16 +330,20 @@ __global__ __launch_bounds__(64 * W, Epi::kDual ? 2 : 3) void rr_expert_rows_ker
   }
 }
 
-// The splits' parts added in order, eight columns a thread.
+// The splits' parts added in order, eight columns a thread, for the rows from the first
+// expert's to the last one's.
 template <class Epi>
 __global__ __launch_bounds__(256) void rr_expert_rows_sum_kernel(Product prm, const float* parts, int splits) {
   constexpr int B = Epi::kDual ? 2 : 1;
   const int eights = (prm.N + 7) / 8;
-  const int rows = rr::dev::offset_at(prm.offsets, prm.experts, prm.rows);
-  const std::size_t total = static_cast<std::size_t>(rows) * eights;
+  const int first = rr::dev::offset_at(prm.offsets, 0, prm.rows);
+  int end = 0;
+  for (int e = static_cast<int>(threadIdx.x) & 63; e <= prm.experts; e += 64) end = max(end, rr::dev::offset_at(prm.offsets, e, prm.rows));
+  end = __builtin_amdgcn_readlane(rr::dev::wave_inclusive_max(end), 63);
+  const std::size_t total = static_cast<std::size_t>(end - first) * eights;
   for (std::size_t t = static_cast<std::size_t>(blockIdx.x) * 256 + threadIdx.x; t < total;
        t += static_cast<std::size_t>(gridDim.x) * 256) {
-    const std::size_t row = t / eights;
+    const std::size_t row = first + t / eights;
     const int n = static_cast<int>(t % eights) * 8;
     float v[B][8] = {};
     for (int s = 0; s < splits; ++s) {

@@ -70,4 +70,16 @@ __device__ __forceinline__ int32_t wave_inclusive_scan(int32_t v) {
   return static_cast<int32_t>(x);
 }
 
+// Inclusive wave maxima of values of 0 and more, by the same moves (0 where there is no source).
+__device__ __forceinline__ int32_t wave_inclusive_max(int32_t v) {
+  uint32_t x = static_cast<uint32_t>(v);
+  x = max(x, dpp_move<kDppRowShr1>(x));
+  x = max(x, dpp_move<kDppRowShr2>(x));
+  x = max(x, dpp_move<kDppRowShr4>(x));
+  x = max(x, dpp_move<kDppRowShr8>(x));
+  x = max(x, dpp_move<kDppRowBcast15, 0xa>(x));
+  x = max(x, dpp_move<kDppRowBcast31, 0xc>(x));
+  return static_cast<int32_t>(x);
+}
+
 }  // namespace rr::dev
