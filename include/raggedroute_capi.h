@@ -543,7 +543,9 @@ typedef struct rr_block_norm_args {
  *   dgate = sum over the gate row's tokens of residual_scale * N(block) * dx,
  *   dpre_weight = sum dn * h / rms(h),  dpost_weight = sum db * block / rms(block).
  * dblock, dgate, dpre_weight and dpost_weight may be NULL where they are not
- * wanted. dx may be dh, dblock may be block where their types agree. Sums over
+ * wanted. Without tokens dpre_weight and dpost_weight are zeros, whatever the other
+ * pointers are; without dn or a post norm theirs is; dblock without a block and dgate
+ * without a gate are left alone. dx may be dh, dblock may be block where their types agree. Sums over
  * tokens go by fixed parts in a fixed order: equal calls give equal bits.
  * Workspace: rr_block_norm_backward_workspace_size, 16-byte aligned.
  */

@@ -113,7 +113,7 @@ kern::NormParams norm_params(const rr_block_norm_backward_args& a) noexcept {
   p.dblock = p.block != nullptr ? a.dblock : nullptr;
   p.dgate = p.gate != nullptr ? a.dgate : nullptr;
   p.dpre_weight = a.dpre_weight;
-  p.dpost_weight = p.post_weight != nullptr ? a.dpost_weight : nullptr;
+  p.dpost_weight = a.dpost_weight;  // (zeros without a post norm)
   p.scale = a.residual_scale;
   p.eps = a.eps;
   p.gate_tokens = a.gate_tokens;
@@ -313,7 +313,7 @@ rr_status rr_block_norm_backward(const rr_block_norm_backward_args* args, const 
   if (status.code != RR_STATUS_SUCCESS) return status;
   const rr::kern::NormParams p = rr::norm_params(a);
   if (a.tokens == 0) {
-    // no tokens: the sums over them are zero
+    // no tokens: the sums over them are zero (and tensors of none may have no address)
     return rr::device_status(rr::kern::block_norm_backward(p, context->stream), "block_norm_backward: a kernel did not launch");
   }
   if (a.h == nullptr || a.dx == nullptr || (a.dh == nullptr && a.dn == nullptr) ||

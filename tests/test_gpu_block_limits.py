@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import raggedroute_amd as rr
-from block_helpers import CODES, context
+from block_helpers import CODES, TYPES, Buf, context
 
 pytestmark = pytest.mark.gpu
 MOST = 2 ** 31 - 1
@@ -85,3 +85,37 @@ def test_quantize_most_rows(device):
     one = torch.tensor(1.0, device="cuda:0") / torch.tensor(127.0, device="cuda:0")
     for piece in pieces():
         assert torch.equal(q[piece], 127 * sign[piece]) and (scale[piece] == one).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("hidden", [1, 520, 20001])
+def test_norm_gradients_of_no_tokens(device, dtype, hidden):
+    """As an empty step calls it: tensors without tokens have no address, the weights' gradients
+    are zero."""
+    empty = torch.empty(0, hidden, dtype=TYPES[dtype], device="cuda:0")
+    assert empty.data_ptr() == 0
+    sums = {name: Buf(torch.full((hidden,), float("nan"), dtype=TYPES[dtype], device="cuda:0"))
+            for name in ("dpre_weight", "dpost_weight")}
+    weight = Buf(torch.ones(hidden, dtype=TYPES[dtype], device="cuda:0"))
+    none = {name: empty.data_ptr() for name in ("h", "block", "gate", "dh", "dn", "dx", "dblock", "dgate")}
+    args = rr.BlockNormBackwardArgs(**none, **{name: b.ptr for name, b in sums.items()}, pre_weight=weight.ptr,
+                                    post_weight=weight.ptr, gate_tokens=1, tokens=0, hidden=hidden, dtype=CODES[dtype])
+    ctx, _ = context(rr.get_block_norm_backward_workspace_size(args))
+    status = rr.block_norm_backward(args, ctx)
+    assert status.ok(), status.message
+    for name, b in sums.items():
+        assert b.intact() and (b.t == 0).all(), name
+
+
+@pytest.mark.parametrize("hidden", [264, 20001])
+@pytest.mark.parametrize("block", [False, True])
+def test_norm_gradient_of_an_absent_post_weight(device, hidden, block):
+    """Nothing depends on it: zeros."""
+    rows = {name: Buf(torch.ones(7, hidden, dtype=BF16, device="cuda:0")) for name in ("h", "dh", "block")}
+    dx, dpost = Buf(shape=(7, hidden), dtype=BF16), Buf(torch.full((hidden,), 3.0, dtype=BF16, device="cuda:0"))
+    args = rr.BlockNormBackwardArgs(h=rows["h"].ptr, dh=rows["dh"].ptr, block=rows["block"].ptr if block else None,
+                                    dx=dx.ptr, dpost_weight=dpost.ptr, tokens=7, hidden=hidden, dtype=CODES["bf16"])
+    ctx, ws = context(rr.get_block_norm_backward_workspace_size(args))
+    status = rr.block_norm_backward(args, ctx)
+    assert status.ok(), status.message
+    assert ws.intact() and dpost.intact() and (dpost.t == 0).all() and torch.equal(dx.t, rows["dh"].t)
