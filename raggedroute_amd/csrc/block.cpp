@@ -314,6 +314,9 @@ rr_status rr_block_norm_backward(const rr_block_norm_backward_args* args, const 
   const rr::kern::NormParams p = rr::norm_params(a);
   if (a.tokens == 0) {
     // no tokens: the sums over them are zero (and tensors of none may have no address)
+    if (!rr::all_aligned({a.dpre_weight, a.dpost_weight}, rr::type_size(a.dtype))) {
+      return rr::invalid_argument("block_norm_backward: every buffer must be aligned to its element type");
+    }
     return rr::device_status(rr::kern::block_norm_backward(p, context->stream), "block_norm_backward: a kernel did not launch");
   }
   if (a.h == nullptr || a.dx == nullptr || (a.dh == nullptr && a.dn == nullptr) ||

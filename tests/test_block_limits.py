@@ -26,3 +26,10 @@ def test_norm_workspace_of_many_tokens(tokens, gate_tokens):
     else:
         parts = divide(tokens, most // group * group)
     assert rr.get_block_norm_backward_workspace_size(args) == parts * 3 * 4
+
+
+@pytest.mark.parametrize("field", ["dpre_weight", "dpost_weight"])
+def test_norm_sums_of_no_tokens_are_aligned(field):
+    args = rr.BlockNormBackwardArgs(**{field: P + 1}, tokens=0, hidden=8)
+    status = rr.block_norm_backward(args, rr.RuntimeContext(architecture=int(rr.DeviceArchitecture.kGfx950)))
+    assert status.code == rr.StatusCode.kInvalidArgument and "aligned" in status.message
