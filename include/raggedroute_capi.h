@@ -574,7 +574,8 @@ typedef struct rr_block_norm_backward_args {
 
 /*
  * Rows to 8-bit integers with a scale each: scale = max|x| / 127 and q =
- * round(x / scale), both divisions in FP32, halves to even; a row of zeros has
+ * round(x / scale), both divisions in FP32, halves to even, q cut to [-127, 127] (a
+ * row of FP32 subnormals may have a scale that was rounded down); a row of zeros has
  * scale 0 and q 0. A row with an infinity or a NaN has that scale and q 0, so that
  * its products are NaN. Also lays weights out for rr_int8_grouped_gemm: one row
  * per expert and output channel.

@@ -552,9 +552,11 @@ __device__ __forceinline__ uint32_t reduce_max(uint32_t v, uint32_t* lds) {
   return v;
 }
 
-// The scale is finite and not zero.
+// The scale is finite and not zero. Cut to +-127: where an FP32 row's largest value is below
+// 127^2 2^-149 its scale is a subnormal of so few bits that it may be up to 1.5 times 127 of
+// them (16-bit rows have no such values).
 __device__ __forceinline__ int8_t quantize(float v, float scale) {
-  return static_cast<int8_t>(static_cast<int>(__builtin_rintf(__fdiv_rn(v, scale))));
+  return static_cast<int8_t>(static_cast<int>(__builtin_amdgcn_fmed3f(__builtin_rintf(__fdiv_rn(v, scale)), -127.0F, 127.0F)));
 }
 
 template <typename T, int G, int NV>

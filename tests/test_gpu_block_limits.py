@@ -1,6 +1,7 @@
 """The expert block's operators at the ends of their ranges: row counts next to 2^31."""
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
 
@@ -119,3 +120,33 @@ def test_norm_gradient_of_an_absent_post_weight(device, hidden, block):
     status = rr.block_norm_backward(args, ctx)
     assert status.ok(), status.message
     assert ws.intact() and dpost.intact() and (dpost.t == 0).all() and torch.equal(dx.t, rows["dh"].t)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("hidden", [5, 20003])
+def test_quantize_subnormal_rows(device, dtype, hidden):
+    """Rows whose scale is zero or a subnormal FP32 number, by the bits of their largest values:
+    FP32 2^-149 to 2^-134 in steps of 2^-149 (wide rows: 2^-140), BF16 2^-133 to 2^-125 in
+    steps of 2^-133. FP32 scales of few bits are rounded down so far that quotients pass
+    127."""
+    last, step = (1 << 15, 512) if dtype == "f32" else (1 << 8, 9)
+    top = torch.arange(1, last, device="cuda:0") if hidden < 100 else torch.arange(150, last, step, device="cuda:0")
+    bits = torch.stack([top, -top, top // 3, -(top // 200), torch.zeros_like(top)], 1)
+    bits = bits.abs() + torch.where(bits < 0, torch.iinfo(torch.int32 if dtype == "f32" else torch.int16).min, 0)
+    x = torch.zeros(len(top), hidden, device="cuda:0", dtype=TYPES[dtype])
+    x[:, -5:] = bits.to(torch.int32).view(torch.float32) if dtype == "f32" else bits.to(torch.int16).view(BF16)
+    q, scale = Buf(shape=x.shape, dtype=torch.int8), Buf(shape=x.shape[:1], dtype=torch.float32)
+    buf = Buf(x)
+    ctx, _ = context()
+    status = rr.quantize_rows(rr.QuantizeRowsArgs(x=buf.ptr, q=q.ptr, scale=scale.ptr, rows=x.shape[0], hidden=hidden,
+                                                  dtype=CODES[dtype]), ctx)
+    assert status.ok(), status.message
+    host = x.cpu().float().numpy()
+    want_scale = np.abs(host).max(1) / np.float32(127.0)
+    with np.errstate(invalid="ignore", divide="ignore"):
+        quotient = np.rint(host / want_scale[:, None])
+    assert dtype == "bf16" or np.nanmax(quotient[want_scale > 0]) > 127
+    want = np.where(want_scale[:, None] > 0, np.clip(quotient, -127, 127), 0)
+    assert np.array_equal(scale.t.cpu().numpy(), want_scale)
+    assert np.array_equal(q.t.cpu().numpy(), want.astype(np.int8))
+    assert q.intact() and scale.intact()
