@@ -28,13 +28,13 @@ __device__ __forceinline__ float activation(int kind, float g) {
   return g * sigmoid(t);
 }
 
-// act(g) and act'(g) = s + g t'(g) s (1 - s), s = sigmoid(t(g)). The second term is
-// below FP32's last bit of the sum from |g| = 40 on and is formed there from 40, where no
-// square or cube overflows against 1 - s = 0.
+// act(g) and act'(g) = s + g t'(g) s (1 - s), s = sigmoid(t(g)). Past the cuts of g in the
+// second term one of its other factors is 0, and no square may overflow against it: 1 - s
+// from 18 on, s below -88 (for SiLU, whose slope there is the second term).
 __device__ __forceinline__ void activation_grad(int kind, float g, float* act, float* grad) {
   const float t = kind == RR_ACT_SILU ? g : kGelu * (g + kGeluCube * g * g * g);
   const float s = sigmoid(t);
-  const float b = g > 40.0F ? 40.0F : g < -40.0F ? -40.0F : g;
+  const float b = g > 40.0F ? 40.0F : g < -104.0F ? -104.0F : g;
   const float slope = kind == RR_ACT_SILU ? 1.0F : kGelu * (1.0F + 3.0F * kGeluCube * b * b);
   *act = g * s;
   *grad = s + b * slope * (s * (1.0F - s));

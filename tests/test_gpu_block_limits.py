@@ -6,7 +6,8 @@ import pytest
 import torch
 
 import raggedroute_amd as rr
-from block_helpers import CODES, TYPES, Buf, context
+from block_helpers import CODES, ROUNDING, TYPES, Buf, context
+from test_gpu_block_ffn import EXP, backward, make
 
 pytestmark = pytest.mark.gpu
 MOST = 2 ** 31 - 1
@@ -150,3 +151,22 @@ def test_quantize_subnormal_rows(device, dtype, hidden):
     assert np.array_equal(scale.t.cpu().numpy(), want_scale)
     assert np.array_equal(q.t.cpu().numpy(), want.astype(np.int8))
     assert q.intact() and scale.intact()
+
+
+@pytest.mark.parametrize("family", ["auto", "naive"])
+def test_slopes_of_small_sigmoids(device, family):
+    """SiLU's slope s (1 + g (1 - s)) down to g = -87, where s is still a normal FP32 number.
+    d gate is the slope itself (one output column, weights of one, up and dy one), dx eight
+    times that, exactly: one rounding to BF16, and s off by 2^-20 (1 + |g|) of itself for the
+    rounding of its exponent."""
+    g = torch.arange(-174, 40, device="cuda:0", dtype=torch.float64) / 2
+    rows, f = len(g), 8
+    v, b, _ = make([rows], 1, f, 1, "bf16")
+    values = {"gate": g[:, None].expand(rows, f), "up": torch.ones(rows, f), "dy": torch.ones(rows, 1),
+              "w_gate": torch.ones(1, 1, f), "w_up": torch.zeros(1, 1, f), "w_down": torch.ones(1, f, 1)}
+    b = {**b, **{name: Buf(t.to(device="cuda:0", dtype=BF16).contiguous()) for name, t in values.items()}}
+    dx = backward(b, [rows], rows, 1, f, 1, "bf16", "silu", family)["dx"].t.double().flatten() / f
+    s = torch.sigmoid(g)
+    want, size = s * (1 + g * (1 - s)), s * (1 + g.abs() * (1 - s))
+    bound = EXP * (1 + g.abs()) * size * 1.01 + ROUNDING["bf16"] * want.abs()
+    assert ((dx - want).abs() <= bound).all(), ((dx - want).abs() / bound).max()
