@@ -594,7 +594,8 @@ typedef struct rr_quantize_rows_args {
  * Expert products of quantised rows and weights, exact in int32:
  *   p(w)[r, n] = (sum_k q[r, k] w[e, n, k]) * q_scale[r] * w_scale[e, n];
  * y = p(w), or with w_up the gated form y = act(p(w)) * p(w_up). hidden <= 131072
- * keeps the sums inside int32.
+ * keeps the sums inside int32 but for one, 131072 products of (-128)(-128), which is
+ * taken as the 2^31 that it is.
  */
 typedef struct rr_int8_grouped_gemm_args {
   const int8_t* q;         /* [rows, hidden] */

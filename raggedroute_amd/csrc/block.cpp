@@ -363,7 +363,7 @@ rr_status rr_int8_grouped_gemm(const rr_int8_grouped_gemm_args* args, const rr_r
   if (args == nullptr) return rr::invalid_argument("int8_grouped_gemm: no argument struct was given");
   if (context == nullptr) return rr::invalid_argument("int8_grouped_gemm: no runtime context was given");
   const rr_int8_grouped_gemm_args& a = *args;
-  if (a.rows < 0 || !rr::experts_ok(a.experts) || !rr::width_ok(a.hidden) || a.hidden > 131072 ||
+  if (a.rows < 0 || !rr::experts_ok(a.experts) || !rr::width_ok(a.hidden) || a.hidden > rr::kern::kMostInt8Hidden ||
       !rr::width_ok(a.output)) {
     return rr::invalid_argument(
         "int8_grouped_gemm: needs rows >= 0, 1 <= experts <= 1024, hidden in 1..131072 and output in 1..1048576");

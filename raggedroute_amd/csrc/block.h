@@ -37,6 +37,8 @@ struct FfnParams {
   bool y_f32;  // forward: y is FP32
 };
 
+constexpr int kMostInt8Hidden = 131072;  // length of an int8 sum
+
 struct Int8Params {
   const int8_t* q;
   const float* q_scale;

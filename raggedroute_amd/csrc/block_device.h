@@ -40,6 +40,15 @@ __device__ __forceinline__ void activation_grad(int kind, float g, float* act, f
   *grad = s + b * slope * (s * (1.0F - s));
 }
 
+// Int32 sums of K int8 products, as FP32. Of at most 2^17 products the least is 2^24 above
+// -2^31, and one sum passes 31 bits: 2^17 times (-128)(-128), whose bits are those of -2^31.
+template <int V>
+__device__ __forceinline__ void mend_int8_sums(float (&v)[V], int K) {
+  if (K != 1 << 17) return;
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = v[i] == -0x1p31F ? 0x1p31F : v[i];
+}
+
 // offsets[e] cut to [0, rows]. Segments are bounded by the largest of these up to theirs: an
 // offset that falls leaves its expert empty, and no row belongs to two experts.
 __device__ __forceinline__ int offset_at(const int32_t* offsets, int e, int rows) {

@@ -154,9 +154,11 @@ __global__ void rr_int8_gemm_naive_kernel(Int8Params p) {
     const int e = expert_of(p.offsets, p.experts, p.rows, static_cast<int>(row));
     if (e < 0) return;
     auto product = [&](const int8_t* w, const float* scale) {
-      int32_t s = 0;
-      for (std::size_t k = 0; k < K; ++k) s += static_cast<int>(p.q[row * K + k]) * static_cast<int>(w[(e * N + n) * K + k]);
-      return static_cast<float>(s) * p.q_scale[row] * scale[e * N + n];
+      uint32_t s = 0;
+      for (std::size_t k = 0; k < K; ++k) s += static_cast<uint32_t>(static_cast<int>(p.q[row * K + k]) * static_cast<int>(w[(e * N + n) * K + k]));
+      float sum[1] = {static_cast<float>(static_cast<int32_t>(s))};
+      rr::dev::mend_int8_sums(sum, p.hidden);
+      return sum[0] * p.q_scale[row] * scale[e * N + n];
     };
     float v = product(p.w, p.w_scale);
     if (p.w_up != nullptr) v = activation(p.activation, v) * product(p.w_up, p.w_up_scale);

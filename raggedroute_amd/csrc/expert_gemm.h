@@ -142,12 +142,14 @@ struct EpiDGate {
 };
 
 // int32 sums (converted) times the row's and the channels' scales. in: channel scales,
-// in_up: those of the second operand, a2: row scales.
-template <typename T>
+// in_up: those of the second operand, a2: row scales. LONGEST: the one sum past int32 is mended
+// (not in the direct tile kernels, whose registers are full: the gated one would spill).
+template <typename T, bool LONGEST>
 struct EpiInt8 {
   static constexpr bool kDual = false;
   template <int V>
-  static __device__ __forceinline__ void emit(const Product& p, int e, std::size_t row, int n, int left, const float (&v)[V]) {
+  static __device__ __forceinline__ void emit(const Product& p, int e, std::size_t row, int n, int left, float (&v)[V]) {
+    if constexpr (LONGEST) rr::dev::mend_int8_sums(v, p.K);
     const float rs = static_cast<const float*>(p.a2)[row];
     float s[V], y[V];
     Cols<float, V>::load(static_cast<const float*>(p.in) + static_cast<std::size_t>(e) * p.N + n, s, left);
@@ -157,12 +159,16 @@ struct EpiInt8 {
   }
 };
 
-template <typename T>
+template <typename T, bool LONGEST>
 struct EpiInt8Gate {
   static constexpr bool kDual = true;
   template <int V>
-  static __device__ __forceinline__ void emit(const Product& p, int e, std::size_t row, int n, int left, const float (&g)[V],
-                                              const float (&u)[V]) {
+  static __device__ __forceinline__ void emit(const Product& p, int e, std::size_t row, int n, int left, float (&g)[V],
+                                              float (&u)[V]) {
+    if constexpr (LONGEST) {
+      rr::dev::mend_int8_sums(g, p.K);
+      rr::dev::mend_int8_sums(u, p.K);
+    }
     const float rs = static_cast<const float*>(p.a2)[row];
     const std::size_t channel = static_cast<std::size_t>(e) * p.N + n;
     float sg[V], su[V], y[V];

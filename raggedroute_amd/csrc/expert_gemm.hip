@@ -707,9 +707,9 @@ using DwPair = Kind<T, false, false, true, EpiPair<T>, DIRECT, ROWS>;  // x^T [d
 template <typename T, bool DIRECT, int ROWS>
 using Dw = Kind<T, false, false, true, EpiStore<T>, DIRECT, ROWS>;  // a^T dy
 template <typename T, bool DIRECT, int ROWS>
-using Int8 = Kind<int8_t, true, true, false, EpiInt8<T>, DIRECT, ROWS>;
+using Int8 = Kind<int8_t, true, true, false, EpiInt8<T, !DIRECT>, DIRECT, ROWS>;
 template <typename T, bool DIRECT, int ROWS>
-using Int8Gate = Kind<int8_t, true, true, false, EpiInt8Gate<T>, DIRECT, ROWS>;
+using Int8Gate = Kind<int8_t, true, true, false, EpiInt8Gate<T, !DIRECT>, DIRECT, ROWS>;
 
 // Loads straight into LDS need every row of every operand on a 16-byte boundary.
 bool aligned16(std::initializer_list<const void*> pointers) {
@@ -854,8 +854,8 @@ hipError_t int8_product(const Int8Params& f, hipStream_t stream) {
   p.K = f.hidden;
   p.lda = p.ldb = f.hidden;
   if (expert_rows_ok(f.rows, f.experts, true)) {
-    return f.w_up != nullptr ? expert_rows<int8_t, EpiInt8Gate<T>>(p, nullptr, 1, stream)
-                             : expert_rows<int8_t, EpiInt8<T>>(p, nullptr, 1, stream);
+    return f.w_up != nullptr ? expert_rows<int8_t, EpiInt8Gate<T, true>>(p, nullptr, 1, stream)
+                             : expert_rows<int8_t, EpiInt8<T, true>>(p, nullptr, 1, stream);
   }
   return f.w_up != nullptr ? launch_kind<T, DIRECT, Int8Gate>(p, stream)
                            : launch_kind<T, DIRECT, Int8>(p, stream);
@@ -884,7 +884,8 @@ hipError_t gated_ffn_backward(const FfnParams& f, hipStream_t stream) {
 }
 
 hipError_t int8_grouped_gemm(const Int8Params& f, hipStream_t stream) {
-  const bool direct = f.hidden % 16 == 0 && aligned16({f.q, f.w, f.w_up});
+  // (the longest sums need the other form's epilogue)
+  const bool direct = f.hidden % 16 == 0 && f.hidden != kMostInt8Hidden && aligned16({f.q, f.w, f.w_up});
   if (f.dtype == RR_DTYPE_FP32) return direct ? int8_product<float, true>(f, stream) : int8_product<float, false>(f, stream);
   if (f.dtype == RR_DTYPE_BF16) return direct ? int8_product<bf16, true>(f, stream) : int8_product<bf16, false>(f, stream);
   return direct ? int8_product<f16, true>(f, stream) : int8_product<f16, false>(f, stream);

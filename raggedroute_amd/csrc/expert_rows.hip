@@ -420,11 +420,11 @@ template hipError_t expert_rows<bf16, EpiGate<bf16>>(const Product&, float*, int
 template hipError_t expert_rows<bf16, EpiStore<bf16>>(const Product&, float*, int, hipStream_t);
 template hipError_t expert_rows<f16, EpiGate<f16>>(const Product&, float*, int, hipStream_t);
 template hipError_t expert_rows<f16, EpiStore<f16>>(const Product&, float*, int, hipStream_t);
-template hipError_t expert_rows<int8_t, EpiInt8<float>>(const Product&, float*, int, hipStream_t);
-template hipError_t expert_rows<int8_t, EpiInt8<bf16>>(const Product&, float*, int, hipStream_t);
-template hipError_t expert_rows<int8_t, EpiInt8<f16>>(const Product&, float*, int, hipStream_t);
-template hipError_t expert_rows<int8_t, EpiInt8Gate<float>>(const Product&, float*, int, hipStream_t);
-template hipError_t expert_rows<int8_t, EpiInt8Gate<bf16>>(const Product&, float*, int, hipStream_t);
-template hipError_t expert_rows<int8_t, EpiInt8Gate<f16>>(const Product&, float*, int, hipStream_t);
+template hipError_t expert_rows<int8_t, EpiInt8<float, true>>(const Product&, float*, int, hipStream_t);
+template hipError_t expert_rows<int8_t, EpiInt8<bf16, true>>(const Product&, float*, int, hipStream_t);
+template hipError_t expert_rows<int8_t, EpiInt8<f16, true>>(const Product&, float*, int, hipStream_t);
+template hipError_t expert_rows<int8_t, EpiInt8Gate<float, true>>(const Product&, float*, int, hipStream_t);
+template hipError_t expert_rows<int8_t, EpiInt8Gate<bf16, true>>(const Product&, float*, int, hipStream_t);
+template hipError_t expert_rows<int8_t, EpiInt8Gate<f16, true>>(const Product&, float*, int, hipStream_t);
 
 }  // namespace rr::kern

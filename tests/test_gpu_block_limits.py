@@ -8,6 +8,7 @@ import torch
 import raggedroute_amd as rr
 from block_helpers import CODES, ROUNDING, TYPES, Buf, context
 from test_gpu_block_ffn import EXP, backward, make
+from test_gpu_block_int8 import product
 
 pytestmark = pytest.mark.gpu
 MOST = 2 ** 31 - 1
@@ -170,3 +171,21 @@ def test_slopes_of_small_sigmoids(device, family):
     want, size = s * (1 + g * (1 - s)), s * (1 + g.abs() * (1 - s))
     bound = EXP * (1 + g.abs()) * size * 1.01 + ROUNDING["bf16"] * want.abs()
     assert ((dx - want).abs() <= bound).all(), ((dx - want).abs() / bound).max()
+
+
+@pytest.mark.parametrize("family", ["auto", "naive"])
+@pytest.mark.parametrize("counts", [[1], [1, 40], [300]])
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("gated", [False, True])
+def test_largest_int8_sum(device, counts, offset, gated, family):
+    """131072 products of (-128)(-128) are 2^31, one past int32, those of (-128) 127 the least sum.
+    Scales of 2^-31 and 1: p is 1 and -127 / 128, exactly."""
+    k, n, rows = 131072, 3, sum(counts)
+    q = torch.full((rows, k), -128, dtype=torch.int8, device="cuda:0")
+    w = torch.full((len(counts), n, k), -128, dtype=torch.int8, device="cuda:0")
+    w[:, 1] = 127
+    qs, ws = torch.full((rows,), 2.0 ** -31, device="cuda:0"), torch.ones(len(counts), n, device="cuda:0")
+    y = product(q, qs, [w, w][:1 + gated], [ws, ws][:1 + gated], counts, n, "f32", "silu", family, offset).t.double()
+    want = torch.tensor([1.0, -127.0 / 128.0, 1.0], dtype=torch.float64, device="cuda:0")
+    want = want * want * torch.sigmoid(want) if gated else want
+    assert ((y - want).abs() <= (2.0 ** -20 if gated else 0.0) * want.abs()).all()
