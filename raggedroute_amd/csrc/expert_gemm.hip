@@ -42,6 +42,7 @@
 #include <type_traits>
 
 #include "expert_gemm.h"
+#include "launchers.h"
 #include "tiles.h"
 #include "wave.h"
 
@@ -667,18 +668,6 @@ __global__ __launch_bounds__(kThreads, 2) void rr_expert_gemm_kernel(Product prm
   if constexpr (P::kDirect) wait_loads<0>();  // (the stream's last loads bring nothing, but they write LDS)
 }
 
-int cu_count() {
-  static const int cus = [] {
-    int device = 0, count = 0;
-    if (hipGetDevice(&device) != hipSuccess ||
-        hipDeviceGetAttribute(&count, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || count <= 0) {
-      return 256;
-    }
-    return count;
-  }();
-  return cus;
-}
-
 template <class P>
 hipError_t launch(const Product& prm, hipStream_t stream) {
   static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(rr_expert_gemm_kernel<P>),
@@ -687,7 +676,7 @@ hipError_t launch(const Product& prm, hipStream_t stream) {
   const long cols = (prm.N + P::kCols - 1) / P::kCols;
   const long rows = P::kWeights ? static_cast<long>(prm.experts) * ((prm.M + 63) / 64)
                                 : prm.rows / 64 + std::min<long>(prm.experts, prm.rows);
-  long grid = std::min<long>(cols * rows, cu_count());
+  long grid = std::min<long>(cols * rows, device_cu_count());
   if (grid >= kXcds) grid = grid / kXcds * kXcds;
   const std::size_t lds = P::kStages * P::kStageBytes + 3 * static_cast<std::size_t>(prm.experts + 1) * sizeof(int32_t);
   rr_expert_gemm_kernel<P><<<dim3(static_cast<unsigned>(grid)), kThreads, lds, stream>>>(prm);

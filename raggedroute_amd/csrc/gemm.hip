@@ -34,6 +34,28 @@
 #include "wave.h"
 
 namespace rr::kern {
+
+namespace {
+constexpr int kMaxDevices = 64;
+std::atomic<int> g_cu_count[kMaxDevices] = {};
+}  // namespace
+
+int device_cu_count() {
+  int device = 0;
+  if (hipGetDevice(&device) != hipSuccess) return 256;
+  if (device >= 0 && device < kMaxDevices) {
+    const int cached = g_cu_count[device].load(std::memory_order_relaxed);
+    if (cached > 0) return cached;
+  }
+  int cus = 0;
+  if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess ||
+      cus <= 0) {
+    cus = 256;
+  }
+  if (device >= 0 && device < kMaxDevices) g_cu_count[device].store(cus, std::memory_order_relaxed);
+  return cus;
+}
+
 namespace {
 
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -743,25 +765,6 @@ __global__ __launch_bounds__(S::kThreads, 2) void rr_gemm_mfma_kernel(GemmParams
       run_tile(WaveLayout<S::kTM, S::kTN, S>{});
     }
   }
-}
-
-constexpr int kMaxDevices = 64;
-std::atomic<int> g_cu_count[kMaxDevices] = {};
-
-int device_cu_count() {
-  int device = 0;
-  if (hipGetDevice(&device) != hipSuccess) return 256;
-  if (device >= 0 && device < kMaxDevices) {
-    const int cached = g_cu_count[device].load(std::memory_order_relaxed);
-    if (cached > 0) return cached;
-  }
-  int cus = 0;
-  if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess ||
-      cus <= 0) {
-    cus = 256;
-  }
-  if (device >= 0 && device < kMaxDevices) g_cu_count[device].store(cus, std::memory_order_relaxed);
-  return cus;
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<std::uintptr_t>(p) & 15u) == 0; }

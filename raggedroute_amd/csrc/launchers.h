@@ -9,6 +9,9 @@
 
 namespace rr::kern {
 
+// Compute units of the current device (gemm.hip).
+int device_cu_count();
+
 // ---- dense / grouped GEMM on FP32 MFMA (gemm.hip) ----
 // c[m, n] = a[m, k] * b[k, n]
 hipError_t dense_gemm_mfma(const float* a, const float* b, float* c, int m, int n, int k,
