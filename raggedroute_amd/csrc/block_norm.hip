@@ -85,6 +85,13 @@ __device__ __forceinline__ void reduce(float (&v)[M], float* lds, int slot) {
   }
 }
 
+// 1 / sqrt(v) for v > 0. v_rsq_f32 takes a subnormal v (eps may be one) for 0.
+__device__ __forceinline__ float inverse_root(float v) {
+  const bool small = v < 0x1p-100F;
+  const float r = __builtin_amdgcn_rsqf(small ? v * 0x1p64F : v);
+  return small ? r * 0x1p32F : r;
+}
+
 template <int G, int M>
 constexpr int kReduceFloats = G > 64 ? 2 * (G / 64) * M : 1;
 
@@ -144,7 +151,7 @@ __global__ __launch_bounds__(G) void rr_block_norm_kernel(NormParams p) {
         for (int i = 0; i < V; ++i) ss[0] = __builtin_fmaf(rb[c][i], rb[c][i], ss[0]);
       });
       reduce<G>(ss, lds, 0);
-      scale *= __frsqrt_rn(__builtin_fmaf(ss[0], inv, p.eps));
+      scale *= inverse_root(__builtin_fmaf(ss[0], inv, p.eps));
     }
     float ss[1] = {0.0F};
     for_chunks<V, G, NV>(D, [&](int c, int col, int left) {
@@ -170,7 +177,7 @@ __global__ __launch_bounds__(G) void rr_block_norm_kernel(NormParams p) {
     }
     if (p.n != nullptr) {
       reduce<G>(ss, lds, 1);
-      const float r = __frsqrt_rn(__builtin_fmaf(ss[0], inv, p.eps));
+      const float r = inverse_root(__builtin_fmaf(ss[0], inv, p.eps));
       for_chunks<V, G, NV>(D, [&](int c, int col, int left) {
         Raw<T, V> out;
         for (int i = 0; i < V; ++i) out.set(i, h[c][i] * r * wpre[c][i]);
@@ -201,7 +208,7 @@ __global__ __launch_bounds__(1024) void rr_block_norm_wide_kernel(NormParams p) 
         ss[0] = __builtin_fmaf(b, b, ss[0]);
       }
       reduce<G>(ss, lds, 0);
-      scale *= __frsqrt_rn(__builtin_fmaf(ss[0], inv, p.eps));
+      scale *= inverse_root(__builtin_fmaf(ss[0], inv, p.eps));
     }
     auto value = [&](int col) {
       float v = static_cast<float>(static_cast<const T*>(p.x)[row + col]);
@@ -220,7 +227,7 @@ __global__ __launch_bounds__(1024) void rr_block_norm_wide_kernel(NormParams p) 
         ss[0] = __builtin_fmaf(v, v, ss[0]);
       }
       reduce<G>(ss, lds, 1);
-      r = __frsqrt_rn(__builtin_fmaf(ss[0], inv, p.eps));
+      r = inverse_root(__builtin_fmaf(ss[0], inv, p.eps));
     }
     for (int col = threadIdx.x; col < D; col += G) {
       const float v = value(col);  // (before h, which may be x)
@@ -349,9 +356,9 @@ __global__ __launch_bounds__(G) void rr_block_norm_backward_kernel(NormParams p,
       }
     });
     reduce<G>(s, lds, 0);
-    const float r = __frsqrt_rn(__builtin_fmaf(s[0], inv, p.eps));
+    const float r = inverse_root(__builtin_fmaf(s[0], inv, p.eps));
     const float back = s[1] * inv * r * r;  // mean(dn pre_weight h) / rms^2
-    const float rb_scale = post ? __frsqrt_rn(__builtin_fmaf(s[2], inv, p.eps)) : 1.0F;
+    const float rb_scale = post ? inverse_root(__builtin_fmaf(s[2], inv, p.eps)) : 1.0F;
     float dx[NV][V];
     float s2[1] = {0.0F};  // db post_weight block
     for_chunks<V, G, NV>(D, [&](int c, int col, int left) {
@@ -460,9 +467,9 @@ __global__ __launch_bounds__(1024) void rr_block_norm_backward_wide_kernel(NormP
       }
     }
     reduce<G>(s, lds, 0);
-    const float r = __frsqrt_rn(__builtin_fmaf(s[0], inv, p.eps));
+    const float r = inverse_root(__builtin_fmaf(s[0], inv, p.eps));
     const float back = s[1] * inv * r * r;
-    const float rb_scale = post ? __frsqrt_rn(__builtin_fmaf(s[2], inv, p.eps)) : 1.0F;
+    const float rb_scale = post ? inverse_root(__builtin_fmaf(s[2], inv, p.eps)) : 1.0F;
     auto dx_at = [&](int col) {
       float v = dh != nullptr ? static_cast<float>(dh[row + col]) : 0.0F;
       if (dn != nullptr) {

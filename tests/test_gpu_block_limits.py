@@ -189,3 +189,40 @@ def test_largest_int8_sum(device, counts, offset, gated, family):
     want = torch.tensor([1.0, -127.0 / 128.0, 1.0], dtype=torch.float64, device="cuda:0")
     want = want * want * torch.sigmoid(want) if gated else want
     assert ((y - want).abs() <= (2.0 ** -20 if gated else 0.0) * want.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("hidden", [64, 2000, 20001])
+def test_norms_with_a_subnormal_eps(device, dtype, hidden):
+    """Rows of one value, 0 and more, and eps = 1e-40: 1 / sqrt(mean + eps) is at most 1e20. Squares
+    and their mean are 71362 units of 2^-149 and more where they matter, each rounded to one:
+    2^-15 of the result together, next to D / 4 + 8 steps of FP32."""
+    eps, v = 1e-40, 2.0 ** -23
+    values = torch.tensor([0.0, 1e-20, 3e-20, 1e-19, 1e-18, 1.0], device="cuda:0").to(TYPES[dtype])
+    t = len(values)
+    rows = values[:, None].expand(t, hidden).contiguous()
+    h, w, dn = Buf(rows), Buf(torch.ones_like(rows[0])), Buf(torch.ones_like(rows))
+    n, dx = Buf(shape=rows.shape, dtype=rows.dtype), Buf(shape=rows.shape, dtype=rows.dtype)
+    dpre, dpost = (Buf(shape=(hidden,), dtype=rows.dtype) for _ in range(2))
+    dblock = Buf(shape=rows.shape, dtype=rows.dtype)
+    common = dict(pre_weight=w.ptr, eps=eps, tokens=t, hidden=hidden, dtype=CODES[dtype])
+    ctx, _ = context()
+    status = rr.block_norm(rr.BlockNormArgs(x=h.ptr, n=n.ptr, **common), ctx)
+    assert status.ok(), status.message
+    # the block is h, too, scaled by 0: dblock and dpost_weight are 0, through its own 1 / rms
+    args = rr.BlockNormBackwardArgs(h=h.ptr, dn=dn.ptr, dx=dx.ptr, dpre_weight=dpre.ptr, block=h.ptr, post_weight=w.ptr,
+                                    dblock=dblock.ptr, dpost_weight=dpost.ptr, residual_scale=0.0, **common)
+    ctx, _ = context(rr.get_block_norm_backward_workspace_size(args))
+    status = rr.block_norm_backward(args, ctx)
+    assert status.ok(), status.message
+    x = rows.double()
+    r = (x * x + eps).rsqrt()
+    error = (hidden / 4 + 8) * v + 2.0 ** -15
+    u = ROUNDING[dtype]
+    assert ((n.t.double() - x * r).abs() <= (error + u) * (x * r)).all()
+    # dx = r (1 - x^2 r^2): of r times the error of its terms
+    want = r * (1 - x * x * r * r)
+    assert ((dx.t.double() - want).abs() <= r * 4 * error + u * (want + r * 4 * error)).all()
+    total = (x * r).sum(0)
+    assert ((dpre.t.double() - total).abs() <= (error + u) * total).all()
+    assert (dblock.t == 0).all() and (dpost.t == 0).all()
