@@ -1,9 +1,11 @@
 // Grouped products of the expert block for few rows an expert (decoding): the weights are
 // read once from memory, straight into registers in matrix-operand order.
 //
-// A workgroup of W waves takes 128 columns (int8: 64) of one expert (of each right operand) and its
-// rows 16 at a time; the waves share the sum's length and add up through LDS in a
-// fixed order. What bounds it is memory: a wave has 8 to 16 loads of 1 KB in flight and
+// A workgroup of W waves takes 128 columns (int8: 64) of one expert (of each right operand) and 16 of
+// its rows; the waves share the sum's length and add up through LDS in a fixed order. An
+// expert's groups of 16 rows are side by side, so that rows which crowd on one expert
+// share the card (one workgroup after the other: 640 rows on one of 128 experts, K = 2048, F =
+// 768, 1130 us; here 41, and on tiles the same). What bounds it is memory: a wave has 8 to 16 loads of 1 KB in flight and
 // never passes weights through LDS (one token, two experts, K = 4096, F = 14336: 470 MB of
 // gate and up in 84 us = 5.6 TB/s, of a pure read's 7.1; the same rows on tiles of 128 rows
 // 558 us for all eight experts' forward pass, here 463).
@@ -104,8 +106,11 @@ __device__ __forceinline__ i4 load16(const T* base, uint32_t offset, uint32_t la
   return __builtin_bit_cast(i4, v);
 }
 
-// The `index`-th expert that has rows (-1: there are fewer), by one wave's lanes.
-__device__ __forceinline__ int find_expert(const Product& p, int index, int* first, int* count) {
+constexpr int kGroup = 16;  // rows of a workgroup
+
+// The `index`-th group of rows, counted through the experts (-1: there are fewer): its expert,
+// first row and rows. By one wave's lanes.
+__device__ __forceinline__ int find_group(const Product& p, int index, int* first, int* count) {
   const int lane = static_cast<int>(threadIdx.x) & 63;
   int most = 0;  // bound of the experts before
   for (int e0 = 0; e0 < p.experts; e0 += 64) {
@@ -117,15 +122,15 @@ __device__ __forceinline__ int find_expert(const Product& p, int index, int* fir
     }
     from = max(most, rr::dev::wave_inclusive_max(from));
     to = max(from, to);
-    const int rows = to - from;
     most = __builtin_amdgcn_readlane(to, 63);
-    uint64_t some = __ballot(rows > 0);
-    const int here = __popcll(some);
+    const int groups = (to - from + kGroup - 1) / kGroup;
+    const int through = rr::dev::wave_inclusive_scan(groups);
+    const int here = __builtin_amdgcn_readlane(through, 63);
     if (index < here) {
-      for (int i = 0; i < index; ++i) some &= some - 1;
-      const int at = __builtin_ctzll(some);
-      *first = __builtin_amdgcn_readlane(from, at);
-      *count = __builtin_amdgcn_readlane(rows, at);
+      const int at = __builtin_ctzll(__ballot(through > index));
+      const int r0 = (index - __builtin_amdgcn_readlane(through - groups, at)) * kGroup;
+      *first = __builtin_amdgcn_readlane(from, at) + r0;
+      *count = min(__builtin_amdgcn_readlane(to, at) - *first, kGroup);
       return e0 + at;
     }
     index -= here;
@@ -151,7 +156,7 @@ __global__ __launch_bounds__(64 * W, Epi::kDual ? 2 : 3) void rr_expert_rows_ker
   const int block = static_cast<int>(blockIdx.x) % blocks;
   const int split = static_cast<int>(blockIdx.x) / blocks % splits;
   int first, count;
-  const int e = find_expert(prm, static_cast<int>(blockIdx.x) / blocks / splits, &first, &count);
+  const int e = find_group(prm, static_cast<int>(blockIdx.x) / blocks / splits, &first, &count);
   if (e < 0) return;
   const int n0 = block * M::kCols;
   const int K = prm.K, N = prm.N;
@@ -166,166 +171,162 @@ __global__ __launch_bounds__(64 * W, Epi::kDual ? 2 : 3) void rr_expert_rows_ker
   const bool aligned = ((reinterpret_cast<uintptr_t>(prm.a) | reinterpret_cast<uintptr_t>(weights[0]) |
                          reinterpret_cast<uintptr_t>(weights[1]) | sizeof(T) * K | (kKC ? 0 : sizeof(T) * N)) & 3) == 0;
 
-#pragma unroll 1
-  for (int r0 = 0; r0 < count; r0 += 16) {
-    Acc acc[B][C] = {};
-    // byte offsets of the lane: of its rows (rows past the last repeat it: their results
-    // are not stored) and in the weights
-    constexpr uint32_t S = sizeof(T);
-    const T* x = static_cast<const T*>(prm.a) + static_cast<std::size_t>(first + r0) * K;
-    const uint32_t x_at = S * (static_cast<uint32_t>(min(li, count - 1 - r0)) * static_cast<uint32_t>(K) + g * V);
-    uint32_t w_at[kKC ? 4 : 1];
+  Acc acc[B][C] = {};
+  // byte offsets of the lane: of its rows (rows past the last repeat it: their results
+  // are not stored) and in the weights
+  constexpr uint32_t S = sizeof(T);
+  const T* x = static_cast<const T*>(prm.a) + static_cast<std::size_t>(first) * K;
+  const uint32_t x_at = S * (static_cast<uint32_t>(min(li, count - 1)) * static_cast<uint32_t>(K) + g * V);
+  uint32_t w_at[kKC ? 4 : 1];
 #pragma unroll
-    for (int j = 0; j < (kKC ? 4 : 1); ++j) {
-      w_at[j] = kKC ? S * (static_cast<uint32_t>(min(16 * j + li, N - 1 - n0)) * static_cast<uint32_t>(K) + g * V)
-                    : S * (static_cast<uint32_t>(8 * g) * static_cast<uint32_t>(N) + 8 * li);
+  for (int j = 0; j < (kKC ? 4 : 1); ++j) {
+    w_at[j] = kKC ? S * (static_cast<uint32_t>(min(16 * j + li, N - 1 - n0)) * static_cast<uint32_t>(K) + g * V)
+                  : S * (static_cast<uint32_t>(8 * g) * static_cast<uint32_t>(N) + 8 * li);
+  }
+  struct Rows {
+    i4 v[X];
+  };
+  struct Weights {
+    i4 v[8];
+  };
+  // what a step multiplies; `whole`: neither the columns nor the step are cut
+  auto load_rows = [&](Rows& o, int s, auto whole) {
+#pragma unroll
+    for (int h = 0; h < X; ++h) {
+      o.v[h] = load16<decltype(whole)::value, kCached>(x + s * M::kK, S * 4 * h * V, x_at, K - s * M::kK - (4 * h + g) * V);
     }
-    struct Rows {
-      i4 v[X];
-    };
-    struct Weights {
-      i4 v[8];
-    };
-    // what a step multiplies; `whole`: neither the columns nor the step are cut
-    auto load_rows = [&](Rows& o, int s, auto whole) {
+  };
+  auto load_weights = [&](Weights& o, int b, int s, auto whole) {
+    constexpr bool kWhole = decltype(whole)::value;
+    if constexpr (kKC) {  // [fragment][half]: columns 16 j + li, k of half h
+      const T* at = weights[b] + static_cast<std::size_t>(n0) * K + s * M::kK;  // (uniform, as below)
 #pragma unroll
-      for (int h = 0; h < X; ++h) {
-        o.v[h] = load16<decltype(whole)::value, kCached>(x + s * M::kK, S * 4 * h * V, x_at, K - s * M::kK - (4 * h + g) * V);
+      for (int q = 0; q < 8; ++q) {
+        o.v[q] = load16<kWhole, POLICY>(at, S * 4 * (q & 1) * V, w_at[q >> 1], K - s * M::kK - (4 * (q & 1) + g) * V);
+        if (!kWhole) __builtin_amdgcn_sched_barrier(0);  // (the pieces of all eight at once would fill the registers)
       }
-    };
-    auto load_weights = [&](Weights& o, int b, int s, auto whole) {
-      constexpr bool kWhole = decltype(whole)::value;
-      if constexpr (kKC) {  // [fragment][half]: columns 16 j + li, k of half h
-        const T* at = weights[b] + static_cast<std::size_t>(n0) * K + s * M::kK;  // (uniform, as below)
+    } else {  // k 8 g + q: columns 8 li .. + 7
+      const T* at = weights[b] + static_cast<std::size_t>(s * M::kK) * N + n0;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          o.v[q] = load16<kWhole, POLICY>(at, S * 4 * (q & 1) * V, w_at[q >> 1], K - s * M::kK - (4 * (q & 1) + g) * V);
-          if (!kWhole) __builtin_amdgcn_sched_barrier(0);  // (the pieces of all eight at once would fill the registers)
-        }
-      } else {  // k 8 g + q: columns 8 li .. + 7
-        const T* at = weights[b] + static_cast<std::size_t>(s * M::kK) * N + n0;
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          o.v[q] = load16<kWhole, POLICY>(at, S * static_cast<uint32_t>(q) * static_cast<uint32_t>(N), w_at[0],
-                                  s * M::kK + 8 * g + q < K ? N - n0 - 8 * li : 0);
-          if (!kWhole) __builtin_amdgcn_sched_barrier(0);
-        }
-      }
-    };
-    auto multiply = [&](const Weights& w, const Rows& r, int b) {
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        if constexpr (kKC) {
-#pragma unroll
-          for (int h = 0; h < X; ++h) acc[b][c] = M::mul(w.v[2 * c + h], r.v[h], acc[b][c]);
-        } else {
-          i4 column;
-#pragma unroll
-          for (int m = 0; m < 4; ++m) {
-            column[m] = static_cast<int>(__builtin_amdgcn_perm(static_cast<uint32_t>(w.v[2 * m + 1][c >> 1]),
-                                                               static_cast<uint32_t>(w.v[2 * m][c >> 1]),
-                                                               (c & 1) != 0 ? 0x07060302U : 0x05040100U));
-          }
-          acc[b][c] = M::mul(column, r.v[0], acc[b][c]);
-        }
-      }
-    };
-    // Two sets of weights in registers: while one is multiplied the other is on its way.
-    // Dual products hold one step's gate and up weights, others two steps.
-    const std::integral_constant<bool, true> whole;
-    const std::integral_constant<bool, false> cut;
-    int s = s0;
-    const int end = n0 + M::kCols > N || !aligned ? s0 : max(s0, min(s1, K / M::kK));  // of the whole steps
-    constexpr int D = Epi::kDual ? 1 : 2;                                 // steps in the two sets
-    if (s + D <= end) {
-      Weights w0, w1;
-      Rows r0v, r1v;
-      load_rows(r0v, s, whole);
-      load_weights(w0, 0, s, whole);
-      if constexpr (!Epi::kDual) load_rows(r1v, s + 1, whole);
-      load_weights(w1, B - 1, s + D - 1, whole);
-#pragma unroll 1
-      for (; s + 2 * D <= end; s += D) {
-        __builtin_amdgcn_sched_barrier(0);
-        Rows next;
-        multiply(w0, r0v, 0);
-        __builtin_amdgcn_sched_barrier(0);  // (loads hoisted over the products would need registers of their own)
-        if constexpr (Epi::kDual) {
-          load_rows(next, s + 1, whole);
-        } else {
-          load_rows(r0v, s + 2, whole);
-        }
-        load_weights(w0, 0, s + D, whole);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(w1, Epi::kDual ? r0v : r1v, B - 1);
-        __builtin_amdgcn_sched_barrier(0);
-        if constexpr (Epi::kDual) {
-          r0v = next;
-        } else {
-          load_rows(r1v, s + 3, whole);
-        }
-        load_weights(w1, B - 1, s + 2 * D - 1, whole);
-      }
-      multiply(w0, r0v, 0);
-      multiply(w1, Epi::kDual ? r0v : r1v, B - 1);
-      s += D;
-    }
-#pragma unroll 1
-    for (; s < s1; ++s) {
-      Rows r;
-      Weights w;
-      load_rows(r, s, cut);
-#pragma unroll
-      for (int b = 0; b < B; ++b) {
-        load_weights(w, b, s, cut);
-        multiply(w, r, b);
+      for (int q = 0; q < 8; ++q) {
+        o.v[q] = load16<kWhole, POLICY>(at, S * static_cast<uint32_t>(q) * static_cast<uint32_t>(N), w_at[0],
+                                s * M::kK + 8 * g + q < K ? N - n0 - 8 * li : 0);
+        if (!kWhole) __builtin_amdgcn_sched_barrier(0);
       }
     }
-
-    // the waves' sums, halved round by round
+  };
+  auto multiply = [&](const Weights& w, const Rows& r, int b) {
 #pragma unroll
-    for (int half = W / 2; half >= 1; half /= 2) {
-      if (wave >= half && wave < 2 * half) {
+    for (int c = 0; c < C; ++c) {
+      if constexpr (kKC) {
 #pragma unroll
-        for (int q = 0; q < B * C; ++q) {
-          lds[((wave - half) * B * C + q) * 64 + lane] = __builtin_bit_cast(i4, acc[q / C][q % C]);
-        }
-      }
-      __syncthreads();
-      if (wave < half) {
-#pragma unroll
-        for (int q = 0; q < B * C; ++q) {
-          acc[q / C][q % C] += __builtin_bit_cast(Acc, lds[(wave * B * C + q) * 64 + lane]);
-        }
-      }
-      __syncthreads();
-    }
-    if (wave != 0) continue;
-    // lane: row li; columns 32 g + 8 r + 0..7 (KC: 16 j + 4 g + 0..3)
-    const int r = r0 + li;
-    if (r >= count) continue;
-    const std::size_t row = static_cast<std::size_t>(first) + r;
-    constexpr int E = kKC ? 4 : 8;  // columns of a store
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      const int n = n0 + (kKC ? 16 * p + 4 * g : 32 * g + 8 * p);
-      if (n >= N) continue;
-      float v[B][E];
-#pragma unroll
-      for (int b = 0; b < B; ++b) {
-#pragma unroll
-        for (int q = 0; q < E; ++q) v[b][q] = static_cast<float>(kKC ? acc[b][p][q] : acc[b][q][p]);
-      }
-      if (parts != nullptr) {
-#pragma unroll
-        for (int b = 0; b < B; ++b) {
-          Cols<float, E>::store(parts + (static_cast<std::size_t>(b * splits + split) * prm.rows + row) * N + n, v[b], N - n);
-        }
-      } else if constexpr (Epi::kDual) {
-        Epi::template emit<E>(prm, e, row, n, N - n, v[0], v[1]);
+        for (int h = 0; h < X; ++h) acc[b][c] = M::mul(w.v[2 * c + h], r.v[h], acc[b][c]);
       } else {
-        Epi::template emit<E>(prm, e, row, n, N - n, v[0]);
+        i4 column;
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          column[m] = static_cast<int>(__builtin_amdgcn_perm(static_cast<uint32_t>(w.v[2 * m + 1][c >> 1]),
+                                                             static_cast<uint32_t>(w.v[2 * m][c >> 1]),
+                                                             (c & 1) != 0 ? 0x07060302U : 0x05040100U));
+        }
+        acc[b][c] = M::mul(column, r.v[0], acc[b][c]);
       }
+    }
+  };
+  // Two sets of weights in registers: while one is multiplied the other is on its way.
+  // Dual products hold one step's gate and up weights, others two steps.
+  const std::integral_constant<bool, true> whole;
+  const std::integral_constant<bool, false> cut;
+  int s = s0;
+  const int end = n0 + M::kCols > N || !aligned ? s0 : max(s0, min(s1, K / M::kK));  // of the whole steps
+  constexpr int D = Epi::kDual ? 1 : 2;                                 // steps in the two sets
+  if (s + D <= end) {
+    Weights w0, w1;
+    Rows r0v, r1v;
+    load_rows(r0v, s, whole);
+    load_weights(w0, 0, s, whole);
+    if constexpr (!Epi::kDual) load_rows(r1v, s + 1, whole);
+    load_weights(w1, B - 1, s + D - 1, whole);
+#pragma unroll 1
+    for (; s + 2 * D <= end; s += D) {
+      __builtin_amdgcn_sched_barrier(0);
+      Rows next;
+      multiply(w0, r0v, 0);
+      __builtin_amdgcn_sched_barrier(0);  // (loads hoisted over the products would need registers of their own)
+      if constexpr (Epi::kDual) {
+        load_rows(next, s + 1, whole);
+      } else {
+        load_rows(r0v, s + 2, whole);
+      }
+      load_weights(w0, 0, s + D, whole);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(w1, Epi::kDual ? r0v : r1v, B - 1);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (Epi::kDual) {
+        r0v = next;
+      } else {
+        load_rows(r1v, s + 3, whole);
+      }
+      load_weights(w1, B - 1, s + 2 * D - 1, whole);
+    }
+    multiply(w0, r0v, 0);
+    multiply(w1, Epi::kDual ? r0v : r1v, B - 1);
+    s += D;
+  }
+#pragma unroll 1
+  for (; s < s1; ++s) {
+    Rows r;
+    Weights w;
+    load_rows(r, s, cut);
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      load_weights(w, b, s, cut);
+      multiply(w, r, b);
+    }
+  }
+
+  // the waves' sums, halved round by round
+#pragma unroll
+  for (int half = W / 2; half >= 1; half /= 2) {
+    if (wave >= half && wave < 2 * half) {
+#pragma unroll
+      for (int q = 0; q < B * C; ++q) {
+        lds[((wave - half) * B * C + q) * 64 + lane] = __builtin_bit_cast(i4, acc[q / C][q % C]);
+      }
+    }
+    __syncthreads();
+    if (wave < half) {
+#pragma unroll
+      for (int q = 0; q < B * C; ++q) {
+        acc[q / C][q % C] += __builtin_bit_cast(Acc, lds[(wave * B * C + q) * 64 + lane]);
+      }
+    }
+    __syncthreads();
+  }
+  if (wave != 0) return;
+  // lane: row li; columns 32 g + 8 r + 0..7 (KC: 16 j + 4 g + 0..3)
+  if (li >= count) return;
+  const std::size_t row = static_cast<std::size_t>(first) + li;
+  constexpr int E = kKC ? 4 : 8;  // columns of a store
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const int n = n0 + (kKC ? 16 * p + 4 * g : 32 * g + 8 * p);
+    if (n >= N) continue;
+    float v[B][E];
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+#pragma unroll
+      for (int q = 0; q < E; ++q) v[b][q] = static_cast<float>(kKC ? acc[b][p][q] : acc[b][q][p]);
+    }
+    if (parts != nullptr) {
+#pragma unroll
+      for (int b = 0; b < B; ++b) {
+        Cols<float, E>::store(parts + (static_cast<std::size_t>(b * splits + split) * prm.rows + row) * N + n, v[b], N - n);
+      }
+    } else if constexpr (Epi::kDual) {
+      Epi::template emit<E>(prm, e, row, n, N - n, v[0], v[1]);
+    } else {
+      Epi::template emit<E>(prm, e, row, n, N - n, v[0]);
     }
   }
 }
@@ -368,7 +369,9 @@ hipError_t launch(const Product& prm, float* parts, int splits, hipStream_t stre
   constexpr std::size_t lds = static_cast<std::size_t>(W / 2) * (Epi::kDual ? 2 : 1) * (Step<T>::kKC ? 4 : 8) * 64 * sizeof(i4);
   static_assert(lds <= 64 * 1024, "no attribute raises the limit");
   const int blocks = (prm.N + Step<T>::kCols - 1) / Step<T>::kCols;
-  const std::size_t grid = static_cast<std::size_t>(std::min(prm.experts, prm.rows)) * blocks * splits;
+  // (the most groups: of n rows an expert has (n - 1) / kGroup + 1 at most)
+  const int busy = std::min(prm.experts, prm.rows);
+  const std::size_t grid = static_cast<std::size_t>((prm.rows - busy) / kGroup + busy) * blocks * splits;
   rr_expert_rows_kernel<T, Epi, W, POLICY><<<dim3(static_cast<unsigned>(grid)), 64 * W, lds, stream>>>(prm, parts, splits, blocks);
   if (splits > 1) {
     if constexpr (sizeof(T) == 2) {
@@ -392,10 +395,12 @@ hipError_t launch_waves(const Product& prm, float* parts, int splits, hipStream_
 }  // namespace
 
 // Five rows an expert on average, of int8 three: tiles then multiply 64 rows for every few,
-// but an expert's weights are read once however many rows it has, and here again for every
-// 16 (E = 128, K = 2048, F = 768, skewed: 512 rows 233 us, tiles 248; 768 rows 270, tiles
-// 250; 1024 rows 293, tiles 249; E = 8, K = 4096, F = 14336: 16 rows 463, tiles 558; int8,
-// E = 128, K = 2048, N = 768: 384 rows 115, tiles 114; 640 rows 127, tiles 113).
+// but read an expert's weights once however many rows it has, and here every 16 rows read them
+// again (E = 128, K = 2048, F = 768: 640 rows 194 us without skew and 216 with Zipf's 1, 641
+// on tiles 209 and 210; E = 8, K = 4096, F = 14336: 40 rows 457, 41 on tiles 522; int8, E = 128,
+// K = 2048, N = 768: 384 rows 37 to 39, 385 on tiles 37). Rows that all go to one expert cost up to
+// twice the tiles' time (5120 rows on one of 1024 experts, K = 1024, F = 256: 89 us, 5121 on
+// tiles 41).
 bool expert_rows_ok(int rows, int experts, bool int8) {
   return rows <= 16 || rows <= (int8 ? 3 : 5) * std::min(rows, experts);
 }
