@@ -438,7 +438,8 @@ void rr_chain_graph_cache_destroy(rr_chain_graph_cache* cache);
  * <= rows; larger or negative ones are cut to [0, rows], and one that falls counts as
  * the largest before it, so that its expert is empty and no row belongs to two. Rows
  * before the first expert's and past the last one's are neither read nor written. The
- * kernel families of the other operators apply: auto and optimized (id 950) run the gfx950 kernels, naive one thread per output. Entries allocate and
+ * kernel families of the other operators apply: auto and optimized (id 950) run the
+ * gfx950 kernels, naive (the products only) one thread per output. Entries allocate and
  * synchronise nothing and may be captured into graphs.
  */
 enum { RR_ACT_SILU = 0, RR_ACT_GELU_TANH = 1 };

@@ -27,12 +27,12 @@
 //    ones; the workgroup meets once or twice a slice.
 //
 // What bounds it: large products the slices' loads that miss an XCD's L2 (8192 skewed rows of
-// eight experts, K = 4096, F = 14336: gate and up 1853 us = 1.04 PFLOP/s, 0.69 of a dense
+// eight experts, K = 4096, F = 14336: gate and up 1922 us = 1.00 PFLOP/s, 0.67 of a dense
 // library product of that size; without its loads 1426, the products alone 1052; data
-// gradients 2040, weight gradients 1905 and 900 us); int8 the power that the products draw
-// (16384 rows, K = 4096, N = 14336: 2.1 POP/s, the library's rate); experts of a hundred
-// rows the weights from HBM and what a few tiles a CU leave idle (8192 rows of 64
-// experts, K = 1024, F = 512, forward and backward: 273 us).
+// gradients 2072, weight gradients 1973 and 937 us); int8 the power that the products draw
+// (16384 rows of eight experts, K = 4096, N = 14336: 917 us = 2.1 POP/s, a dense library product
+// of that size 819); experts of a hundred rows the weights from HBM and what a few tiles a
+// CU leave idle (8192 rows of 64 experts, K = 1024, F = 512, forward and backward: 275 us).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -5,10 +5,12 @@
 // its rows; the waves share the sum's length and add up through LDS in a fixed order. An
 // expert's groups of 16 rows are side by side, so that rows which crowd on one expert
 // share the card (one workgroup after the other: 640 rows on one of 128 experts, K = 2048, F =
-// 768, 1130 us; here 41, and on tiles the same). What bounds it is memory: a wave has 8 to 16 loads of 1 KB in flight and
-// never passes weights through LDS (one token, two experts, K = 4096, F = 14336: 470 MB of
-// gate and up in 84 us = 5.6 TB/s, of a pure read's 7.1; the same rows on tiles of 128 rows
-// 558 us for all eight experts' forward pass, here 463).
+// 768, 1130 us; here 41, and on tiles the same). What bounds it is memory: a wave has 8 to 16
+// loads of 1 KB in flight and never passes weights through LDS (one token, two experts, K =
+// 4096, F = 14336: 470 MB of gate and up in 81 us = 5.8 TB/s, of a pure read's 7.1; two rows on
+// each of eight experts, forward: 454 us, on tiles of 128 rows 558). Rows of odd widths, and
+// the last 128 columns of others, are loaded a step at a time with nothing in flight (the
+// token at K = 4095, F = 14335: 873 us, at the even widths 121).
 //  - 16-bit weights lie [K, N]: a lane (i, g) loads 8 columns 8 i .. + 7 of the k rows 8 g .. + 7
 //    of a 32-k step and turns that 8 x 8 block (32 byte permutes); register c then holds
 //    eight k of column 8 i + c, the operand of one v_mfma_f32_16x16x32: the order of the
@@ -40,10 +42,10 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 
 constexpr int kBufferFlags = 0x00027000;  // raw 32-bit buffer
 // Policies of the weights' loads: past the caches where the weights are larger than the
-// caches keep from one call to the next (one token of E = 8, K = 4096, F = 14336 143 -> 125 us;
-// but E = 64, K = 256, F = 128 13.1 -> 15.2). int8 rows are loaded 64 bytes at a time, whose
-// lines the next load needs again (E = 128, K = 2048, N = 768, 128 rows: 46 us, past the
-// caches 59), 16-bit rows a whole line and more.
+// caches keep from one call to the next (one token of E = 8, K = 4096, F = 14336 134 -> 123 us;
+// but E = 64, K = 256, F = 128 11.0 -> 11.7). int8 rows are loaded 64 bytes at a time, whose
+// lines the next load needs again (E = 128, K = 2048, N = 768, 128 rows, with their
+// quantisation: 52.4 us, past the caches 53.0), 16-bit rows a whole line and more.
 constexpr int kStreamed = 2, kCached = 0;
 constexpr std::size_t kStreamedBytes = std::size_t{64} << 20;
 
