@@ -1,4 +1,5 @@
-"""The expert block's operators at the ends of their ranges: row counts next to 2^31."""
+"""The expert block's operators at the ends of their ranges: row counts next to 2^31, the widest
+rows, the smallest and the largest numbers."""
 from __future__ import annotations
 
 import numpy as np
@@ -7,8 +8,13 @@ import torch
 
 import raggedroute_amd as rr
 from block_helpers import CODES, ROUNDING, TYPES, Buf, context
-from test_gpu_block_ffn import EXP, backward, make
+from test_gpu_block_ffn import EXP, backward, check_backward, check_forward, forward, make
 from test_gpu_block_int8 import product
+from test_gpu_block_norm import backward as norm_backward
+from test_gpu_block_norm import check_backward as check_norm_backward
+from test_gpu_block_norm import check_forward as check_norm_forward
+from test_gpu_block_norm import forward as norm_forward
+from test_gpu_block_norm import make as make_norm
 
 pytestmark = pytest.mark.gpu
 MOST = 2 ** 31 - 1
@@ -226,3 +232,64 @@ def test_norms_with_a_subnormal_eps(device, dtype, hidden):
     total = (x * r).sum(0)
     assert ((dpre.t.double() - total).abs() <= (error + u) * total).all()
     assert (dblock.t == 0).all() and (dpost.t == 0).all()
+
+
+WIDEST = 1 << 20
+
+
+@pytest.mark.parametrize("counts,k,f,n", [([2, 0, 1], WIDEST, 8, 16), ([1, 2], 8, WIDEST, 8), ([130], 16, WIDEST, 8),
+                                          ([300], WIDEST, 8, 16), ([300], 8, 16, WIDEST), ([2, 1], WIDEST - 1, 3, 5),
+                                          ([130], 5, WIDEST - 1, 3)])
+def test_widest_ffn(device, counts, k, f, n):
+    v, b, rows = make(counts, k, f, n, "bf16", seed=1)
+    check_forward(v, forward(b, counts, rows, k, f, n, "bf16"), counts, "bf16", "silu")
+    check_backward(v, backward(b, counts, rows, k, f, n, "bf16"), counts, "bf16", "silu")
+
+
+@pytest.mark.parametrize("d", [WIDEST, WIDEST - 1])
+def test_widest_norm(device, d):
+    v = make_norm(3, d, "bf16", "bf16", 2, seed=2)
+    check_norm_forward(v, norm_forward(v, 3, d, "bf16", "bf16", 2), "bf16", 2)
+    v["h"] = v.pop("x")
+    check_norm_backward(v, norm_backward(v, 3, d, "bf16", "bf16", 2), "bf16", "bf16", 2)
+
+
+class Part:
+    """Some rows (or experts) of an output."""
+
+    def __init__(self, buf, part):
+        self.t = buf.t[part].clone()
+
+
+def last_expert(v, rows, count):
+    """The inputs of the last expert, which has the last `count` rows."""
+    weights = {name: v[name][-1:] for name in ("w_gate", "w_up", "w_down")}
+    return {**weights, **{name: v[name][rows - count:] for name in ("x", "dy", "gate", "up", "act")}}
+
+
+# rows from 2^32 bytes on; weights of the last expert from 2^32 bytes on, few and many rows
+@pytest.mark.parametrize("counts,k,f,n", [([1100000, 1000], 2048, 16, 24), ([0] * 63 + [3], 8192, 4200, 16),
+                                          ([0] * 63 + [700], 4200, 8192, 8), ([0] * 63 + [11000], 8200, 4200, 8),
+                                          ([1100000, 300], 2047, 3, 5)])
+def test_far_rows_and_experts(device, counts, k, f, n):
+    v, b, rows = make(counts, k, f, n, "bf16", seed=4)
+    mine, count = last_expert(v, rows, counts[-1]), counts[-1]
+    out = forward(b, counts, rows, k, f, n, "bf16")
+    check_forward(mine, {name: Part(buf, slice(rows - count, rows)) for name, buf in out.items()}, [count], "bf16", "silu")
+    del out
+    grad = backward(b, counts, rows, k, f, n, "bf16")
+    got = {name: Part(buf, slice(rows - count, rows) if name == "dx" else slice(-1, None)) for name, buf in grad.items()}
+    check_backward(mine, got, [count], "bf16", "silu")
+    if counts[0] == 0:
+        assert all((grad[name].t[0] == 0).all() for name in ("dw_gate", "dw_up", "dw_down"))
+
+
+@pytest.mark.parametrize("count", [3, 700, 11000])
+def test_far_int8_experts(device, count):
+    """Weights past 2^31 bytes: of the last of 64 experts, 3 in every place; rows of ones."""
+    counts, k, n = [0] * 63 + [count], 4208, 8200
+    q, w = torch.ones(count, k, dtype=torch.int8, device="cuda:0"), torch.ones(64, n, k, dtype=torch.int8, device="cuda:0")
+    w[-1] = 3
+    y = product(q, torch.ones(count, device="cuda:0"), [w], [torch.ones(64, n, device="cuda:0")], counts, n, "f32", "silu",
+                "auto").t
+    assert (y == 3.0 * k).all()
