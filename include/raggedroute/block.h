@@ -1,6 +1,6 @@
 // raggedroute/block.h - the expert block around the routing chain: gated
-// feed-forward with its gradients, the norms before and after it, and 8-bit
-// integer products. New entries (no reference counterpart); inline forwarders to
+// feed-forward with its gradients, the norms before and after it, 8-bit integer and
+// 4-bit floating-point products, tokens to their experts and back with gradients. New entries (no reference counterpart); inline forwarders to
 // raggedroute_capi.h, which states formulas, shapes and optional buffers.
 #pragma once
 
@@ -133,6 +133,104 @@ struct Int8GroupedGemmArgs {
   KernelSelection kernel;
 };
 
+struct SortTokensArgs {
+  const void* x = nullptr;
+  const std::int32_t* expert_ids = nullptr;
+  std::int32_t* offsets = nullptr;
+  std::int32_t* route_pos = nullptr;
+  std::int32_t* sorted_route = nullptr;
+  void* x_sorted = nullptr;
+  int tokens = 0;
+  int experts = 0;
+  int top_k = 2;
+  int hidden = 0;
+  ScalarType dtype = ScalarType::kBf16;
+  ScalarType x_dtype = ScalarType::kBf16;
+  KernelSelection kernel;
+};
+
+struct SortTokensBackwardArgs {
+  const void* dx_sorted = nullptr;
+  const std::int32_t* route_pos = nullptr;
+  void* dx = nullptr;
+  int tokens = 0;
+  int top_k = 2;
+  int hidden = 0;
+  ScalarType dtype = ScalarType::kBf16;
+  ScalarType x_dtype = ScalarType::kBf16;
+  KernelSelection kernel;
+};
+
+struct CombineTokensArgs {
+  const void* y_sorted = nullptr;
+  const std::int32_t* route_pos = nullptr;
+  const float* route_weights = nullptr;
+  void* y = nullptr;
+  int tokens = 0;
+  int top_k = 2;
+  int hidden = 0;
+  ScalarType dtype = ScalarType::kBf16;
+  ScalarType y_dtype = ScalarType::kBf16;
+  KernelSelection kernel;
+};
+
+struct CombineTokensBackwardArgs {
+  const void* dy = nullptr;
+  const void* y_sorted = nullptr;
+  const std::int32_t* route_pos = nullptr;
+  const float* route_weights = nullptr;
+  void* dy_sorted = nullptr;
+  float* droute_weights = nullptr;
+  int tokens = 0;
+  int top_k = 2;
+  int hidden = 0;
+  ScalarType dtype = ScalarType::kBf16;
+  ScalarType y_dtype = ScalarType::kBf16;
+  KernelSelection kernel;
+};
+
+struct TopKGateBackwardArgs {
+  const std::int32_t* expert_ids = nullptr;
+  const float* weights = nullptr;
+  const float* dweights = nullptr;
+  float* dlogits = nullptr;
+  int tokens = 0;
+  int experts = 0;
+  int top_k = 2;
+  KernelSelection kernel;
+};
+
+struct QuantizeRowsMxfp4Args {
+  const void* x = nullptr;
+  const std::int32_t* sorted_route = nullptr;
+  std::uint8_t* q = nullptr;
+  std::uint8_t* scale = nullptr;
+  int rows = 0;
+  int hidden = 0;
+  int tokens = 0;
+  int top_k = 2;
+  ScalarType dtype = ScalarType::kBf16;
+  KernelSelection kernel;
+};
+
+struct Mxfp4GroupedGemmArgs {
+  const std::uint8_t* q = nullptr;
+  const std::uint8_t* q_scale = nullptr;
+  const std::uint8_t* w = nullptr;
+  const std::uint8_t* w_scale = nullptr;
+  const std::uint8_t* w_up = nullptr;
+  const std::uint8_t* w_up_scale = nullptr;
+  const std::int32_t* offsets = nullptr;
+  void* y = nullptr;
+  int rows = 0;
+  int experts = 0;
+  int hidden = 0;
+  int output = 0;
+  Activation activation = Activation::kSilu;
+  ScalarType dtype = ScalarType::kBf16;
+  KernelSelection kernel;
+};
+
 namespace detail {
 
 inline rr_gated_ffn_args to_c(const GatedFfnArgs& a) noexcept {
@@ -164,6 +262,37 @@ inline rr_int8_grouped_gemm_args to_c(const Int8GroupedGemmArgs& a) noexcept {
           a.experts, a.hidden, a.output, static_cast<int32_t>(a.activation),
           static_cast<int32_t>(a.dtype), to_c(a.kernel)};
 }
+inline rr_sort_tokens_args to_c(const SortTokensArgs& a) noexcept {
+  return {a.x, a.expert_ids, a.offsets, a.route_pos, a.sorted_route, a.x_sorted, a.tokens,
+          a.experts, a.top_k, a.hidden, static_cast<int32_t>(a.dtype),
+          static_cast<int32_t>(a.x_dtype), to_c(a.kernel)};
+}
+inline rr_sort_tokens_backward_args to_c(const SortTokensBackwardArgs& a) noexcept {
+  return {a.dx_sorted, a.route_pos, a.dx, a.tokens, a.top_k, a.hidden,
+          static_cast<int32_t>(a.dtype), static_cast<int32_t>(a.x_dtype), to_c(a.kernel)};
+}
+inline rr_combine_tokens_args to_c(const CombineTokensArgs& a) noexcept {
+  return {a.y_sorted, a.route_pos, a.route_weights, a.y, a.tokens, a.top_k, a.hidden,
+          static_cast<int32_t>(a.dtype), static_cast<int32_t>(a.y_dtype), to_c(a.kernel)};
+}
+inline rr_combine_tokens_backward_args to_c(const CombineTokensBackwardArgs& a) noexcept {
+  return {a.dy, a.y_sorted, a.route_pos, a.route_weights, a.dy_sorted, a.droute_weights, a.tokens,
+          a.top_k, a.hidden, static_cast<int32_t>(a.dtype), static_cast<int32_t>(a.y_dtype),
+          to_c(a.kernel)};
+}
+inline rr_topk_gate_backward_args to_c(const TopKGateBackwardArgs& a) noexcept {
+  return {a.expert_ids, a.weights, a.dweights, a.dlogits, a.tokens, a.experts, a.top_k,
+          to_c(a.kernel)};
+}
+inline rr_quantize_rows_mxfp4_args to_c(const QuantizeRowsMxfp4Args& a) noexcept {
+  return {a.x, a.sorted_route, a.q, a.scale, a.rows, a.hidden, a.tokens, a.top_k,
+          static_cast<int32_t>(a.dtype), to_c(a.kernel)};
+}
+inline rr_mxfp4_grouped_gemm_args to_c(const Mxfp4GroupedGemmArgs& a) noexcept {
+  return {a.q, a.q_scale, a.w, a.w_scale, a.w_up, a.w_up_scale, a.offsets, a.y, a.rows, a.experts,
+          a.hidden, a.output, static_cast<int32_t>(a.activation), static_cast<int32_t>(a.dtype),
+          to_c(a.kernel)};
+}
 
 }  // namespace detail
 
@@ -190,6 +319,35 @@ inline std::size_t get_quantize_rows_workspace_size(const QuantizeRowsArgs& args
 inline std::size_t get_int8_grouped_gemm_workspace_size(const Int8GroupedGemmArgs& args) noexcept {
   const auto c = detail::to_c(args);
   return rr_int8_grouped_gemm_workspace_size(&c);
+}
+
+inline std::size_t get_sort_tokens_workspace_size(const SortTokensArgs& args) noexcept {
+  const auto c = detail::to_c(args);
+  return rr_sort_tokens_workspace_size(&c);
+}
+inline std::size_t get_sort_tokens_backward_workspace_size(const SortTokensBackwardArgs& args) noexcept {
+  const auto c = detail::to_c(args);
+  return rr_sort_tokens_backward_workspace_size(&c);
+}
+inline std::size_t get_combine_tokens_workspace_size(const CombineTokensArgs& args) noexcept {
+  const auto c = detail::to_c(args);
+  return rr_combine_tokens_workspace_size(&c);
+}
+inline std::size_t get_combine_tokens_backward_workspace_size(const CombineTokensBackwardArgs& args) noexcept {
+  const auto c = detail::to_c(args);
+  return rr_combine_tokens_backward_workspace_size(&c);
+}
+inline std::size_t get_topk_gate_backward_workspace_size(const TopKGateBackwardArgs& args) noexcept {
+  const auto c = detail::to_c(args);
+  return rr_topk_gate_backward_workspace_size(&c);
+}
+inline std::size_t get_quantize_rows_mxfp4_workspace_size(const QuantizeRowsMxfp4Args& args) noexcept {
+  const auto c = detail::to_c(args);
+  return rr_quantize_rows_mxfp4_workspace_size(&c);
+}
+inline std::size_t get_mxfp4_grouped_gemm_workspace_size(const Mxfp4GroupedGemmArgs& args) noexcept {
+  const auto c = detail::to_c(args);
+  return rr_mxfp4_grouped_gemm_workspace_size(&c);
 }
 
 inline Status gated_ffn(const GatedFfnArgs& args, const RuntimeContext& context) noexcept {
@@ -225,6 +383,41 @@ inline Status int8_grouped_gemm(const Int8GroupedGemmArgs& args,
   const auto a = detail::to_c(args);
   const auto c = detail::to_c(context);
   return detail::from_c(rr_int8_grouped_gemm(&a, &c));
+}
+inline Status sort_tokens(const SortTokensArgs& args, const RuntimeContext& context) noexcept {
+  const auto a = detail::to_c(args);
+  const auto c = detail::to_c(context);
+  return detail::from_c(rr_sort_tokens(&a, &c));
+}
+inline Status sort_tokens_backward(const SortTokensBackwardArgs& args, const RuntimeContext& context) noexcept {
+  const auto a = detail::to_c(args);
+  const auto c = detail::to_c(context);
+  return detail::from_c(rr_sort_tokens_backward(&a, &c));
+}
+inline Status combine_tokens(const CombineTokensArgs& args, const RuntimeContext& context) noexcept {
+  const auto a = detail::to_c(args);
+  const auto c = detail::to_c(context);
+  return detail::from_c(rr_combine_tokens(&a, &c));
+}
+inline Status combine_tokens_backward(const CombineTokensBackwardArgs& args, const RuntimeContext& context) noexcept {
+  const auto a = detail::to_c(args);
+  const auto c = detail::to_c(context);
+  return detail::from_c(rr_combine_tokens_backward(&a, &c));
+}
+inline Status topk_gate_backward(const TopKGateBackwardArgs& args, const RuntimeContext& context) noexcept {
+  const auto a = detail::to_c(args);
+  const auto c = detail::to_c(context);
+  return detail::from_c(rr_topk_gate_backward(&a, &c));
+}
+inline Status quantize_rows_mxfp4(const QuantizeRowsMxfp4Args& args, const RuntimeContext& context) noexcept {
+  const auto a = detail::to_c(args);
+  const auto c = detail::to_c(context);
+  return detail::from_c(rr_quantize_rows_mxfp4(&a, &c));
+}
+inline Status mxfp4_grouped_gemm(const Mxfp4GroupedGemmArgs& args, const RuntimeContext& context) noexcept {
+  const auto a = detail::to_c(args);
+  const auto c = detail::to_c(context);
+  return detail::from_c(rr_mxfp4_grouped_gemm(&a, &c));
 }
 
 }  // namespace raggedroute

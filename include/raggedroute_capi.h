@@ -636,6 +636,203 @@ rr_status rr_quantize_rows(const rr_quantize_rows_args* args, const rr_runtime_c
 rr_status rr_int8_grouped_gemm(const rr_int8_grouped_gemm_args* args,
                                const rr_runtime_context* context);
 
+/* ---- tokens to their experts and back, with gradients (no reference counterpart) ----
+ *
+ * What token_permute and unpermute do in FP32, for the types of the expert block, and
+ * every gradient of it. The conventions of the expert block hold; the kernels are the
+ * gfx950 ones alone (no naive family). A token has top_k routes (1..64; tokens * top_k
+ * within 31 bits), route r = token * top_k + rank, and the same expert may stand in
+ * several of them. A 16-bit `dtype` of the sorted rows may go with FP32 rows on the
+ * tokens' side (x_dtype, y_dtype): the norms and the router then compute in FP32.
+ * Every sum has a fixed order: equal calls give equal bits.
+ */
+#define RR_MAX_SORT_TOP_K 64
+
+/*
+ * Routes in order of their experts, by route index inside an expert:
+ *   offsets[e] = #{r: 0 <= ids[r] < e},
+ *   route_pos[r] = offsets[ids[r]] + #{q < r: ids[q] = ids[r]},  sorted_route[route_pos[r]] = r,
+ *   x_sorted[route_pos[r]] = x[r / top_k].
+ * A route whose id is none of 0..experts-1 (padding) is not placed: its route_pos is -1, and
+ * the last entries of sorted_route are -1. Rows of x_sorted past offsets[experts] are left
+ * alone. x_sorted NULL: the maps alone (x is not read). Without tokens offsets is zeros.
+ */
+typedef struct rr_sort_tokens_args {
+  const void* x;             /* [tokens, hidden] of x_dtype */
+  const int32_t* expert_ids; /* [tokens, top_k] */
+  int32_t* offsets;          /* [experts + 1] */
+  int32_t* route_pos;        /* [tokens * top_k] */
+  int32_t* sorted_route;     /* [tokens * top_k], optional */
+  void* x_sorted;            /* [tokens * top_k, hidden] of dtype, optional */
+  int32_t tokens;
+  int32_t experts;
+  int32_t top_k;
+  int32_t hidden;
+  int32_t dtype;   /* FP32, FP16 or BF16 */
+  int32_t x_dtype; /* dtype, or RR_DTYPE_FP32 */
+  rr_kernel_selection kernel;
+} rr_sort_tokens_args;
+
+/*
+ * Gradient of the rows' copies: dx[t] = sum over t's routes of dx_sorted[route_pos], in
+ * rank order and FP32, rounded once. Routes whose position is none of 0..tokens*top_k-1 have
+ * no part; a token without any gets zeros.
+ */
+typedef struct rr_sort_tokens_backward_args {
+  const void* dx_sorted;    /* [tokens * top_k, hidden] of dtype */
+  const int32_t* route_pos; /* [tokens * top_k] */
+  void* dx;                 /* [tokens, hidden] of x_dtype */
+  int32_t tokens;
+  int32_t top_k;
+  int32_t hidden;
+  int32_t dtype;
+  int32_t x_dtype;
+  rr_kernel_selection kernel;
+} rr_sort_tokens_backward_args;
+
+/*
+ * Sorted rows back to their tokens: y[t] = sum over t's routes of route_weights[r] *
+ * y_sorted[route_pos[r]], in rank order and FP32, rounded once. route_weights NULL: all 1.
+ * Positions as in rr_sort_tokens_backward.
+ */
+typedef struct rr_combine_tokens_args {
+  const void* y_sorted;       /* [tokens * top_k, hidden] of dtype */
+  const int32_t* route_pos;   /* [tokens * top_k] */
+  const float* route_weights; /* [tokens * top_k], optional */
+  void* y;                    /* [tokens, hidden] of y_dtype */
+  int32_t tokens;
+  int32_t top_k;
+  int32_t hidden;
+  int32_t dtype;   /* FP32, FP16 or BF16 */
+  int32_t y_dtype; /* dtype, or RR_DTYPE_FP32 */
+  rr_kernel_selection kernel;
+} rr_combine_tokens_args;
+
+/*
+ * Gradients of rr_combine_tokens:
+ *   dy_sorted[route_pos[r]] = route_weights[r] * dy[t],
+ *   droute_weights[r] = sum over the columns of dy[t] * y_sorted[route_pos[r]] (FP32),
+ * 0 for routes without a position. Rows of dy_sorted that no position names are left
+ * alone; the positions of a map differ from each other. dy_sorted and droute_weights
+ * may be NULL where they are not wanted (y_sorted is read for the latter only), and dy_sorted
+ * may be y_sorted.
+ */
+typedef struct rr_combine_tokens_backward_args {
+  const void* dy;             /* [tokens, hidden] of y_dtype */
+  const void* y_sorted;       /* as in the forward call, with droute_weights */
+  const int32_t* route_pos;
+  const float* route_weights; /* optional */
+  void* dy_sorted;            /* [tokens * top_k, hidden] of dtype, optional */
+  float* droute_weights;      /* [tokens * top_k], optional */
+  int32_t tokens;
+  int32_t top_k;
+  int32_t hidden;
+  int32_t dtype;
+  int32_t y_dtype;
+  rr_kernel_selection kernel;
+} rr_combine_tokens_backward_args;
+
+/*
+ * Gradient of the gate's logits from that of its weights, w = softmax over the chosen
+ * logits, whose sum is 1:
+ *   dlogits[t, ids[j]] = w[j] * sum over i of w[i] * (dw[j] - dw[i]),
+ * 0 for the experts that were not chosen (for every one of a token whose ids are none of
+ * 0..experts-1; of ids of which some are, the others have no part in the sums). An expert
+ * chosen twice gets the sum of both.
+ */
+typedef struct rr_topk_gate_backward_args {
+  const int32_t* expert_ids; /* [tokens, top_k] */
+  const float* weights;      /* [tokens, top_k] */
+  const float* dweights;     /* [tokens, top_k] */
+  float* dlogits;            /* [tokens, experts] */
+  int32_t tokens;
+  int32_t experts;
+  int32_t top_k;
+  rr_kernel_selection kernel;
+} rr_topk_gate_backward_args;
+
+/* ---- the experts' products in microscaled 4-bit floating point ----
+ *
+ * Blocks of 32 elements of a row share a power of two: an element is E2M1 (0, 0.5, 1, 1.5, 2, 3, 4,
+ * 6 and their negatives), its block's scale E8M0 (2^(byte - 127); 255 is NaN). With blocks =
+ * ceil(hidden / 32) and slices = ceil(hidden / 256):
+ *   q     [rows, 16 * blocks] bytes, element k of a row in the low (even k) or high half of its
+ *         byte k / 2; elements past hidden in the last block are zeros;
+ *   scale [slices, rows, 8] bytes, block b of a row at [b / 8][row][b % 8], so that the scales
+ *         which a tile of a product reads lie side by side. Bytes past the last block are
+ *         not looked at.
+ * q starts on a 16-byte boundary, scale on an 8-byte one. Scales [rows, blocks] as a
+ * checkpoint holds them come into this order by padding a row to 8 * slices bytes and a
+ * transposed copy.
+ */
+
+/*
+ * Rows to blocks of 4-bit elements: with m the block's largest magnitude, X = floor(log2 m) - 2
+ * (-127 at least, and for m = 0), the scale is 2^X and an element x / 2^X rounded to the
+ * nearest of the values, ties to even, and cut to [-6, 6]. A block with an infinity or a NaN
+ * has scale NaN and elements 0, so that its row's products are NaN. With sorted_route row r is
+ * that of token sorted_route[r] / top_k (x is not copied in between), and rows whose route is
+ * none of 0..tokens*top_k-1 are left alone. Scale bytes past the last block are written 0.
+ * Also lays weights out for rr_mxfp4_grouped_gemm: a row per expert and output channel.
+ */
+typedef struct rr_quantize_rows_mxfp4_args {
+  const void* x;               /* [rows, hidden] ([tokens, hidden] with sorted_route) of dtype */
+  const int32_t* sorted_route; /* [rows], optional */
+  uint8_t* q;                  /* [rows, 16 * blocks] */
+  uint8_t* scale;              /* [slices, rows, 8] */
+  int32_t rows;
+  int32_t hidden;
+  int32_t tokens; /* with sorted_route, as top_k */
+  int32_t top_k;
+  int32_t dtype;  /* FP32, FP16 or BF16 */
+  rr_kernel_selection kernel;
+} rr_quantize_rows_mxfp4_args;
+
+/*
+ * Expert products of such rows and weights, sums in FP32:
+ *   p(w)[r, n] = sum over the blocks of 2^(Xq + Xw) * sum over k of q[r, k] w[e, n, k];
+ * y = p(w), or with w_up the gated form y = act(p(w)) * p(w_up), rounded once. Workspace:
+ * rr_mxfp4_grouped_gemm_workspace_size, 16-byte aligned.
+ */
+typedef struct rr_mxfp4_grouped_gemm_args {
+  const uint8_t* q;          /* [rows, 16 * blocks] */
+  const uint8_t* q_scale;    /* [slices, rows, 8] */
+  const uint8_t* w;          /* [experts, output, 16 * blocks] */
+  const uint8_t* w_scale;    /* [slices, experts * output, 8] */
+  const uint8_t* w_up;       /* as w, optional */
+  const uint8_t* w_up_scale; /* with w_up */
+  const int32_t* offsets;    /* [experts + 1] */
+  void* y;                   /* [rows, output] of dtype (FP32, FP16 or BF16) */
+  int32_t rows;
+  int32_t experts;
+  int32_t hidden;
+  int32_t output;
+  int32_t activation; /* with w_up */
+  int32_t dtype;
+  rr_kernel_selection kernel;
+} rr_mxfp4_grouped_gemm_args;
+
+size_t rr_sort_tokens_workspace_size(const rr_sort_tokens_args* args);
+size_t rr_sort_tokens_backward_workspace_size(const rr_sort_tokens_backward_args* args);
+size_t rr_combine_tokens_workspace_size(const rr_combine_tokens_args* args);
+size_t rr_combine_tokens_backward_workspace_size(const rr_combine_tokens_backward_args* args);
+size_t rr_topk_gate_backward_workspace_size(const rr_topk_gate_backward_args* args);
+size_t rr_quantize_rows_mxfp4_workspace_size(const rr_quantize_rows_mxfp4_args* args);
+size_t rr_mxfp4_grouped_gemm_workspace_size(const rr_mxfp4_grouped_gemm_args* args);
+
+rr_status rr_sort_tokens(const rr_sort_tokens_args* args, const rr_runtime_context* context);
+rr_status rr_sort_tokens_backward(const rr_sort_tokens_backward_args* args,
+                                  const rr_runtime_context* context);
+rr_status rr_combine_tokens(const rr_combine_tokens_args* args, const rr_runtime_context* context);
+rr_status rr_combine_tokens_backward(const rr_combine_tokens_backward_args* args,
+                                     const rr_runtime_context* context);
+rr_status rr_topk_gate_backward(const rr_topk_gate_backward_args* args,
+                                const rr_runtime_context* context);
+rr_status rr_quantize_rows_mxfp4(const rr_quantize_rows_mxfp4_args* args,
+                                 const rr_runtime_context* context);
+rr_status rr_mxfp4_grouped_gemm(const rr_mxfp4_grouped_gemm_args* args,
+                                const rr_runtime_context* context);
+
 /* Static device scratch of rr_chain_from_tokens_noalloc: one copy per GPU,
  * held until the process ends. */
 #define RR_CHAIN_NOALLOC_SCRATCH_BYTES (1u << 20)

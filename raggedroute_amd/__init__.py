@@ -39,6 +39,8 @@ from ._capi import (  # noqa: F401  (re-exported vocabulary)
     BlockNormBackwardArgs,
     ChainArgs,
     ChainGraphCacheStats,
+    CombineTokensArgs,
+    CombineTokensBackwardArgs,
     ConstTensorView,
     DenseGemmArgs,
     DeviceArchitecture,
@@ -54,19 +56,24 @@ from ._capi import (  # noqa: F401  (re-exported vocabulary)
     KernelFamily,
     KernelSelection,
     MutableTensorView,
+    Mxfp4GroupedGemmArgs,
     OperatorKind,
     OperatorSignature,
     QuantizeRowsArgs,
+    QuantizeRowsMxfp4Args,
     RouteChainArgs,
     RouteTraceInfo,
     RuntimeContext,
     ScalarType,
+    SortTokensArgs,
+    SortTokensBackwardArgs,
     Status,
     StatusCode,
     TensorLayout,
     TensorSpec,
     TokenPermuteArgs,
     TopKGateArgs,
+    TopKGateBackwardArgs,
     UnpermuteArgs,
     bind,
 )
@@ -197,6 +204,43 @@ def quantize_rows(args: QuantizeRowsArgs, context: RuntimeContext | None = None)
 def int8_grouped_gemm(args: Int8GroupedGemmArgs, context: RuntimeContext | None = None) -> Status:
     """Expert products of 8-bit rows and weights with scales per row and output channel."""
     return lib.rr_int8_grouped_gemm(byref(args), byref(_ctx(context)))
+
+
+# ---- tokens to their experts and back, 4-bit products (no reference counterpart) ----
+
+def sort_tokens(args: SortTokensArgs, context: RuntimeContext | None = None) -> Status:
+    """Routes in order of their experts, and the tokens' rows in that order."""
+    return lib.rr_sort_tokens(byref(args), byref(_ctx(context)))
+
+
+def sort_tokens_backward(args: SortTokensBackwardArgs, context: RuntimeContext | None = None) -> Status:
+    """Gradient of sort_tokens: the sum of a token's sorted rows."""
+    return lib.rr_sort_tokens_backward(byref(args), byref(_ctx(context)))
+
+
+def combine_tokens(args: CombineTokensArgs, context: RuntimeContext | None = None) -> Status:
+    """Sorted rows back to their tokens, with the routes' weights applied."""
+    return lib.rr_combine_tokens(byref(args), byref(_ctx(context)))
+
+
+def combine_tokens_backward(args: CombineTokensBackwardArgs, context: RuntimeContext | None = None) -> Status:
+    """Gradients of combine_tokens: of the sorted rows and of the weights."""
+    return lib.rr_combine_tokens_backward(byref(args), byref(_ctx(context)))
+
+
+def topk_gate_backward(args: TopKGateBackwardArgs, context: RuntimeContext | None = None) -> Status:
+    """Gradient of the gate's logits from that of its weights."""
+    return lib.rr_topk_gate_backward(byref(args), byref(_ctx(context)))
+
+
+def quantize_rows_mxfp4(args: QuantizeRowsMxfp4Args, context: RuntimeContext | None = None) -> Status:
+    """Rows (gathered through sorted_route, if given) to 4-bit blocks of 32 with a power of two each."""
+    return lib.rr_quantize_rows_mxfp4(byref(args), byref(_ctx(context)))
+
+
+def mxfp4_grouped_gemm(args: Mxfp4GroupedGemmArgs, context: RuntimeContext | None = None) -> Status:
+    """Expert products of 4-bit rows and weights."""
+    return lib.rr_mxfp4_grouped_gemm(byref(args), byref(_ctx(context)))
 
 
 # ---- chain graphs (rr_chain_graph_*, rr_chain_graph_cache_*) ----
@@ -343,6 +387,34 @@ def get_quantize_rows_workspace_size(args: QuantizeRowsArgs) -> int:
 
 def get_int8_grouped_gemm_workspace_size(args: Int8GroupedGemmArgs) -> int:
     return lib.rr_int8_grouped_gemm_workspace_size(byref(args))
+
+
+def get_sort_tokens_workspace_size(args: SortTokensArgs) -> int:
+    return lib.rr_sort_tokens_workspace_size(byref(args))
+
+
+def get_sort_tokens_backward_workspace_size(args: SortTokensBackwardArgs) -> int:
+    return lib.rr_sort_tokens_backward_workspace_size(byref(args))
+
+
+def get_combine_tokens_workspace_size(args: CombineTokensArgs) -> int:
+    return lib.rr_combine_tokens_workspace_size(byref(args))
+
+
+def get_combine_tokens_backward_workspace_size(args: CombineTokensBackwardArgs) -> int:
+    return lib.rr_combine_tokens_backward_workspace_size(byref(args))
+
+
+def get_topk_gate_backward_workspace_size(args: TopKGateBackwardArgs) -> int:
+    return lib.rr_topk_gate_backward_workspace_size(byref(args))
+
+
+def get_quantize_rows_mxfp4_workspace_size(args: QuantizeRowsMxfp4Args) -> int:
+    return lib.rr_quantize_rows_mxfp4_workspace_size(byref(args))
+
+
+def get_mxfp4_grouped_gemm_workspace_size(args: Mxfp4GroupedGemmArgs) -> int:
+    return lib.rr_mxfp4_grouped_gemm_workspace_size(byref(args))
 
 
 # ---- dispatch (reference include/raggedroute/dispatch.h:32-46) ----

@@ -458,6 +458,155 @@ class Int8GroupedGemmArgs(ctypes.Structure):
         super().__init__(**kw)
 
 
+class SortTokensArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", c_void_p),
+        ("expert_ids", c_void_p),
+        ("offsets", c_void_p),
+        ("route_pos", c_void_p),
+        ("sorted_route", c_void_p),
+        ("x_sorted", c_void_p),
+        ("tokens", c_int32),
+        ("experts", c_int32),
+        ("top_k", c_int32),
+        ("hidden", c_int32),
+        ("dtype", c_int32),
+        ("x_dtype", c_int32),
+        ("kernel", KernelSelection),
+    ]
+
+    def __init__(self, **kw):
+        kw.setdefault("dtype", ScalarType.kBf16)
+        kw.setdefault("x_dtype", kw["dtype"])
+        kw.setdefault("top_k", 2)
+        super().__init__(**kw)
+
+
+class SortTokensBackwardArgs(ctypes.Structure):
+    _fields_ = [
+        ("dx_sorted", c_void_p),
+        ("route_pos", c_void_p),
+        ("dx", c_void_p),
+        ("tokens", c_int32),
+        ("top_k", c_int32),
+        ("hidden", c_int32),
+        ("dtype", c_int32),
+        ("x_dtype", c_int32),
+        ("kernel", KernelSelection),
+    ]
+
+    def __init__(self, **kw):
+        kw.setdefault("dtype", ScalarType.kBf16)
+        kw.setdefault("x_dtype", kw["dtype"])
+        kw.setdefault("top_k", 2)
+        super().__init__(**kw)
+
+
+class CombineTokensArgs(ctypes.Structure):
+    _fields_ = [
+        ("y_sorted", c_void_p),
+        ("route_pos", c_void_p),
+        ("route_weights", c_void_p),
+        ("y", c_void_p),
+        ("tokens", c_int32),
+        ("top_k", c_int32),
+        ("hidden", c_int32),
+        ("dtype", c_int32),
+        ("y_dtype", c_int32),
+        ("kernel", KernelSelection),
+    ]
+
+    def __init__(self, **kw):
+        kw.setdefault("dtype", ScalarType.kBf16)
+        kw.setdefault("y_dtype", kw["dtype"])
+        kw.setdefault("top_k", 2)
+        super().__init__(**kw)
+
+
+class CombineTokensBackwardArgs(ctypes.Structure):
+    _fields_ = [
+        ("dy", c_void_p),
+        ("y_sorted", c_void_p),
+        ("route_pos", c_void_p),
+        ("route_weights", c_void_p),
+        ("dy_sorted", c_void_p),
+        ("droute_weights", c_void_p),
+        ("tokens", c_int32),
+        ("top_k", c_int32),
+        ("hidden", c_int32),
+        ("dtype", c_int32),
+        ("y_dtype", c_int32),
+        ("kernel", KernelSelection),
+    ]
+
+    def __init__(self, **kw):
+        kw.setdefault("dtype", ScalarType.kBf16)
+        kw.setdefault("y_dtype", kw["dtype"])
+        kw.setdefault("top_k", 2)
+        super().__init__(**kw)
+
+
+class TopKGateBackwardArgs(ctypes.Structure):
+    _fields_ = [
+        ("expert_ids", c_void_p),
+        ("weights", c_void_p),
+        ("dweights", c_void_p),
+        ("dlogits", c_void_p),
+        ("tokens", c_int32),
+        ("experts", c_int32),
+        ("top_k", c_int32),
+        ("kernel", KernelSelection),
+    ]
+
+    def __init__(self, **kw):
+        kw.setdefault("top_k", 2)
+        super().__init__(**kw)
+
+
+class QuantizeRowsMxfp4Args(ctypes.Structure):
+    _fields_ = [
+        ("x", c_void_p),
+        ("sorted_route", c_void_p),
+        ("q", c_void_p),
+        ("scale", c_void_p),
+        ("rows", c_int32),
+        ("hidden", c_int32),
+        ("tokens", c_int32),
+        ("top_k", c_int32),
+        ("dtype", c_int32),
+        ("kernel", KernelSelection),
+    ]
+
+    def __init__(self, **kw):
+        kw.setdefault("dtype", ScalarType.kBf16)
+        kw.setdefault("top_k", 2)
+        super().__init__(**kw)
+
+
+class Mxfp4GroupedGemmArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", c_void_p),
+        ("q_scale", c_void_p),
+        ("w", c_void_p),
+        ("w_scale", c_void_p),
+        ("w_up", c_void_p),
+        ("w_up_scale", c_void_p),
+        ("offsets", c_void_p),
+        ("y", c_void_p),
+        ("rows", c_int32),
+        ("experts", c_int32),
+        ("hidden", c_int32),
+        ("output", c_int32),
+        ("activation", c_int32),
+        ("dtype", c_int32),
+        ("kernel", KernelSelection),
+    ]
+
+    def __init__(self, **kw):
+        kw.setdefault("dtype", ScalarType.kBf16)
+        super().__init__(**kw)
+
+
 class OperatorSignature(ctypes.Structure):
     _fields_ = [
         ("has_input", c_int32),
@@ -504,6 +653,13 @@ _OP_ENTRIES = [
     ("block_norm_backward", BlockNormBackwardArgs),
     ("quantize_rows", QuantizeRowsArgs),
     ("int8_grouped_gemm", Int8GroupedGemmArgs),
+    ("sort_tokens", SortTokensArgs),
+    ("sort_tokens_backward", SortTokensBackwardArgs),
+    ("combine_tokens", CombineTokensArgs),
+    ("combine_tokens_backward", CombineTokensBackwardArgs),
+    ("topk_gate_backward", TopKGateBackwardArgs),
+    ("quantize_rows_mxfp4", QuantizeRowsMxfp4Args),
+    ("mxfp4_grouped_gemm", Mxfp4GroupedGemmArgs),
 ]
 
 PROTOTYPES: list[tuple[str, object, list]] = []

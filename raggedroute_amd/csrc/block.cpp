@@ -7,74 +7,13 @@
 
 #include <cstddef>
 #include <cstdint>
-#include <initializer_list>
 
 #include "block.h"
+#include "block_checks.h"
 #include "common.h"
 
 namespace rr {
 namespace {
-
-constexpr std::size_t kWorkspaceAlignment = 16;
-
-bool is_16bit(int32_t dtype) noexcept { return dtype == RR_DTYPE_FP16 || dtype == RR_DTYPE_BF16; }
-bool is_block_type(int32_t dtype) noexcept { return dtype == RR_DTYPE_FP32 || is_16bit(dtype); }
-std::size_t type_size(int32_t dtype) noexcept { return dtype == RR_DTYPE_FP32 ? 4 : 2; }
-
-bool width_ok(int32_t width) noexcept { return width >= 1 && width <= RR_MAX_BLOCK_WIDTH; }
-bool experts_ok(int32_t experts) noexcept { return experts >= 1 && experts <= RR_MAX_EXPERTS; }
-bool activation_ok(int32_t activation) noexcept {
-  return activation == RR_ACT_SILU || activation == RR_ACT_GELU_TANH;
-}
-
-bool any_null(std::initializer_list<const void*> pointers) noexcept {
-  for (const void* p : pointers) {
-    if (p == nullptr) return true;
-  }
-  return false;
-}
-
-bool all_aligned(std::initializer_list<const void*> pointers, std::size_t alignment) noexcept {
-  for (const void* p : pointers) {
-    if (!is_aligned(p, alignment)) return false;
-  }
-  return true;
-}
-
-// These operators run on gfx950; id 950 is the one optimized implementation and, unless
-// `naive` is null, the naive family has kernels.
-rr_status choose_family(rr_kernel_selection kernel, int32_t architecture, bool* naive) noexcept {
-  int32_t resolved = RR_ARCH_OTHER;
-  const rr_status status = rr_resolve_device_architecture(architecture, &resolved);
-  if (status.code != RR_STATUS_SUCCESS) return status;
-  if (resolved != RR_ARCH_GFX950) {
-    return make_status(RR_STATUS_UNSUPPORTED_ARCHITECTURE, "expert block: kernels exist for gfx950 (MI355X) only");
-  }
-  const bool native = (kernel.family == RR_FAMILY_AUTO && kernel.implementation_id == 0) ||
-                      (kernel.family == RR_FAMILY_OPTIMIZED && kernel.implementation_id == RR_IMPL_GFX950_NATIVE);
-  const bool plain = naive != nullptr && kernel.family == RR_FAMILY_NAIVE && kernel.implementation_id == 0;
-  if (!native && !plain) {
-    return make_status(RR_STATUS_UNSUPPORTED_KERNEL_VARIANT,
-                       "expert block: no kernel has that family and implementation id");
-  }
-  if (naive != nullptr) *naive = plain;
-  return ok_status();
-}
-
-rr_status check_workspace(const rr_runtime_context* context, std::size_t bytes, const char* message) noexcept {
-  if (bytes == 0) return ok_status();
-  if (context->workspace == nullptr || context->workspace_bytes < bytes) {
-    return make_status(RR_STATUS_INSUFFICIENT_WORKSPACE, message);
-  }
-  if (!is_aligned(context->workspace, kWorkspaceAlignment)) {
-    return invalid_argument("expert block: the workspace must start on a 16-byte boundary");
-  }
-  return ok_status();
-}
-
-std::size_t round_up(std::size_t bytes) noexcept {
-  return (bytes + kWorkspaceAlignment - 1) / kWorkspaceAlignment * kWorkspaceAlignment;
-}
 
 // One of the backward pass's two [rows, inner] parts.
 std::size_t ffn_part_bytes(const rr_gated_ffn_backward_args& a) noexcept {

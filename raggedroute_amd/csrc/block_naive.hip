@@ -7,6 +7,7 @@
 
 #include "block.h"
 #include "block_device.h"
+#include "mxfp4.h"
 
 namespace rr::kern {
 namespace {
@@ -172,6 +173,46 @@ __global__ void rr_int8_gemm_naive_kernel(Int8Params p) {
   });
 }
 
+// An E2M1 number.
+__device__ float e2m1(int code) {
+  const int e = (code >> 1) & 3, m = code & 1;
+  const float v = e == 0 ? 0.5F * m : 0.5F * static_cast<float>((2 + m) << (e - 1));
+  return (code & 8) != 0 ? -v : v;
+}
+
+__global__ void rr_mxfp4_gemm_naive_kernel(MxGemmParams p) {
+  const std::size_t N = p.output, blocks = mx_blocks(p.hidden);
+  const std::size_t channels = static_cast<std::size_t>(p.experts) * N;
+  for_outputs(p.rows * N, [&](std::size_t i) {
+    const std::size_t row = i / N, n = i % N;
+    const int e = expert_of(p.offsets, p.experts, p.rows, static_cast<int>(row));
+    if (e < 0) return;
+    const std::size_t channel = e * N + n;
+    auto product = [&](const uint8_t* w, const uint8_t* w_scale) {
+      float sum = 0.0F;
+      for (std::size_t b = 0; b < blocks; ++b) {
+        float part = 0.0F;  // (exact: quarters up to 32 * 36)
+        for (std::size_t k = 0; k < 16; ++k) {
+          const int x = p.q[(row * blocks + b) * 16 + k], y = w[(channel * blocks + b) * 16 + k];
+          part += e2m1(x & 15) * e2m1(y & 15) + e2m1(x >> 4) * e2m1(y >> 4);
+        }
+        const int xs = p.q_scale[(b / 8 * p.rows + row) * 8 + b % 8], ys = w_scale[(b / 8 * channels + channel) * 8 + b % 8];
+        sum += xs == 255 || ys == 255 ? __builtin_nanf("") : ldexpf(part, xs + ys - 254);
+      }
+      return sum;
+    };
+    float v = product(p.w, p.w_scale);
+    if (p.w_up != nullptr) v = activation(p.activation, v) * product(p.w_up, p.w_up_scale);
+    if (p.dtype == RR_DTYPE_FP32) {
+      static_cast<float*>(p.y)[i] = v;
+    } else if (p.dtype == RR_DTYPE_BF16) {
+      static_cast<rr::dev::bf16*>(p.y)[i] = static_cast<rr::dev::bf16>(v);
+    } else {
+      static_cast<rr::dev::f16*>(p.y)[i] = static_cast<rr::dev::f16>(v);
+    }
+  });
+}
+
 template <typename T>
 hipError_t ffn_forward(const FfnParams& p, hipStream_t stream) {
   const std::size_t rows = p.rows;
@@ -210,6 +251,11 @@ hipError_t gated_ffn_backward_naive(const FfnParams& p, hipStream_t stream) {
 hipError_t int8_grouped_gemm_naive(const Int8Params& p, hipStream_t stream) {
   if (p.rows == 0) return hipSuccess;
   rr_int8_gemm_naive_kernel<<<grid_for(static_cast<std::size_t>(p.rows) * p.output), kThreads, 0, stream>>>(p);
+  return hipGetLastError();
+}
+
+hipError_t mxfp4_grouped_gemm_naive(const MxGemmParams& p, hipStream_t stream) {
+  rr_mxfp4_gemm_naive_kernel<<<grid_for(static_cast<std::size_t>(p.rows) * p.output), kThreads, 0, stream>>>(p);
   return hipGetLastError();
 }
 

@@ -29,6 +29,7 @@
 #include <type_traits>
 
 #include "expert_gemm.h"
+#include "row_groups.h"
 #include "wave.h"
 
 namespace rr::kern {
@@ -106,38 +107,6 @@ __device__ __forceinline__ i4 load16(const T* base, uint32_t offset, uint32_t la
     }
   }
   return __builtin_bit_cast(i4, v);
-}
-
-constexpr int kGroup = 16;  // rows of a workgroup
-
-// The `index`-th group of rows, counted through the experts (-1: there are fewer): its expert,
-// first row and rows. By one wave's lanes.
-__device__ __forceinline__ int find_group(const Product& p, int index, int* first, int* count) {
-  const int lane = static_cast<int>(threadIdx.x) & 63;
-  int most = 0;  // bound of the experts before
-  for (int e0 = 0; e0 < p.experts; e0 += 64) {
-    const int e = e0 + lane;
-    int from = 0, to = 0;
-    if (e < p.experts) {
-      from = rr::dev::offset_at(p.offsets, e, p.rows);
-      to = rr::dev::offset_at(p.offsets, e + 1, p.rows);
-    }
-    from = max(most, rr::dev::wave_inclusive_max(from));
-    to = max(from, to);
-    most = __builtin_amdgcn_readlane(to, 63);
-    const int groups = (to - from + kGroup - 1) / kGroup;
-    const int through = rr::dev::wave_inclusive_scan(groups);
-    const int here = __builtin_amdgcn_readlane(through, 63);
-    if (index < here) {
-      const int at = __builtin_ctzll(__ballot(through > index));
-      const int r0 = (index - __builtin_amdgcn_readlane(through - groups, at)) * kGroup;
-      *first = __builtin_amdgcn_readlane(from, at) + r0;
-      *count = min(__builtin_amdgcn_readlane(to, at) - *first, kGroup);
-      return e0 + at;
-    }
-    index -= here;
-  }
-  return -1;
 }
 
 // (waves a SIMD: what the accumulators and the two sets of weights leave room for)
@@ -371,9 +340,7 @@ hipError_t launch(const Product& prm, float* parts, int splits, hipStream_t stre
   constexpr std::size_t lds = static_cast<std::size_t>(W / 2) * (Epi::kDual ? 2 : 1) * (Step<T>::kKC ? 4 : 8) * 64 * sizeof(i4);
   static_assert(lds <= 64 * 1024, "no attribute raises the limit");
   const int blocks = (prm.N + Step<T>::kCols - 1) / Step<T>::kCols;
-  // (the most groups: of n rows an expert has (n - 1) / kGroup + 1 at most)
-  const int busy = std::min(prm.experts, prm.rows);
-  const std::size_t grid = static_cast<std::size_t>((prm.rows - busy) / kGroup + busy) * blocks * splits;
+  const std::size_t grid = most_groups(prm.rows, prm.experts) * blocks * splits;
   rr_expert_rows_kernel<T, Epi, W, POLICY><<<dim3(static_cast<unsigned>(grid)), 64 * W, lds, stream>>>(prm, parts, splits, blocks);
   if (splits > 1) {
     if constexpr (sizeof(T) == 2) {

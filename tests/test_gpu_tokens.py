@@ -1,0 +1,285 @@
+"""sort_tokens, combine_tokens, their gradients and the gate's against their definitions.
+
+Maps and copies are exact. Sums of k products in FP32 are off by k half units of the products'
+magnitudes (one rounding each of the fused multiply-add) and the result's own half unit; a
+dot product over n columns by n of them. The gate's gradient has a subtraction and a
+multiply-add for each route and a last product: (top_k + 3) half units of the sum of its
+terms' magnitudes.
+"""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import raggedroute_amd as rr
+from block_helpers import CODES, LEAST, ROUNDING, TYPES, Buf, assert_within, context
+
+pytestmark = pytest.mark.gpu
+
+PAIRS = [("f32", "f32"), ("bf16", "bf16"), ("f16", "f16"), ("bf16", "f32"), ("f16", "f32")]
+
+
+def run(entry, args, size=None):
+    ctx, ws = context(size(args) if size else 0)
+    status = entry(args, ctx)
+    assert status.ok(), status.message
+    assert ws.intact()
+
+
+def routes(tokens, top_k, experts, seed, kind="any"):
+    """Expert ids with padding and repeated experts among them."""
+    gen = torch.Generator().manual_seed(seed)
+    if kind == "one":
+        return torch.full((tokens, top_k), experts - 1, dtype=torch.int32)
+    if kind == "none":
+        return torch.full((tokens, top_k), -1, dtype=torch.int32)
+    ids = torch.randint(0, experts, (tokens, top_k), generator=gen, dtype=torch.int32)
+    if kind == "any":
+        bad = torch.rand(tokens, top_k, generator=gen)
+        ids[bad < 0.1] = -1
+        ids[bad > 0.95] = experts  # one past the last
+        ids[(bad > 0.9) & (bad < 0.92)] = -2 ** 31
+        ids[(bad > 0.92) & (bad < 0.94)] = 2 ** 31 - 1
+    return ids
+
+
+def maps(ids, experts):
+    flat = ids.reshape(-1).long()
+    order = torch.cat([torch.nonzero(flat == e).reshape(-1) for e in range(experts)])
+    counts = torch.tensor([int((flat == e).sum()) for e in range(experts)])
+    offsets = torch.cat([torch.zeros(1, dtype=torch.long), counts.cumsum(0)]).int()
+    pos = torch.full((flat.numel(),), -1, dtype=torch.int32)
+    pos[order] = torch.arange(order.numel(), dtype=torch.int32)
+    route = torch.full((flat.numel(),), -1, dtype=torch.int32)
+    route[:order.numel()] = order.int()
+    return offsets, pos, route
+
+
+def sort(ids, x, experts, dtype, x_dtype, offset=0, rows=True, inverse=True):
+    tokens, top_k = ids.shape
+    hidden = x.shape[1]
+    count = tokens * top_k
+    i32 = dict(dtype=torch.int32)
+    b = dict(ids=Buf(ids.cuda(), offset=offset), x=Buf(x, offset=offset), offsets=Buf(shape=(experts + 1,), offset=offset, **i32),
+             pos=Buf(shape=(count,), offset=offset, **i32), route=Buf(shape=(count,), offset=offset, **i32),
+             out=Buf(shape=(count, hidden), dtype=TYPES[dtype], offset=offset))
+    run(rr.sort_tokens, rr.SortTokensArgs(
+        x=b["x"].ptr, expert_ids=b["ids"].ptr, offsets=b["offsets"].ptr, route_pos=b["pos"].ptr,
+        sorted_route=b["route"].ptr if inverse else None, x_sorted=b["out"].ptr if rows else None, tokens=tokens,
+        experts=experts, top_k=top_k, hidden=hidden, dtype=CODES[dtype], x_dtype=CODES[x_dtype]),
+        rr.get_sort_tokens_workspace_size)
+    assert all(buf.intact() for buf in b.values())
+    return b
+
+
+def check_sort(ids, x, experts, dtype, b):
+    offsets, pos, route = maps(ids, experts)
+    assert torch.equal(b["offsets"].t.cpu(), offsets)
+    assert torch.equal(b["pos"].t.cpu(), pos)
+    assert torch.equal(b["route"].t.cpu(), route)
+    placed = int(offsets[-1])
+    want = x.cpu()[(route[:placed] // ids.shape[1]).long()].to(TYPES[dtype])
+    got = b["out"].t[:placed].cpu()
+    assert torch.equal(got.contiguous().view(torch.uint8), want.contiguous().view(torch.uint8))
+    assert b["out"].untouched(slice(placed, None))
+
+
+SHAPES = [(1, 1, 1, 1), (1, 8, 128, 64), (3, 2, 5, 7), (5, 64, 3, 33), (64, 8, 128, 200), (128, 8, 300, 96),
+          (513, 2, 9, 1023), (700, 3, 1024, 40), (2100, 8, 64, 264), (4097, 1, 257, 65), (333, 5, 1000, 2050)]
+
+
+@pytest.mark.parametrize("kind", ["any", "all", "one", "none"])
+@pytest.mark.parametrize("tokens,top_k,experts,hidden", SHAPES)
+def test_sort(device, tokens, top_k, experts, hidden, kind):
+    ids = routes(tokens, top_k, experts, tokens * top_k, kind)
+    x = torch.randn(tokens, hidden, device="cuda:0").bfloat16()
+    x[0, 0], x[-1, -1] = float("nan"), float("-inf")
+    for offset in (0, 1):
+        check_sort(ids, x, experts, "bf16", sort(ids, x, experts, "bf16", "bf16", offset))
+
+
+@pytest.mark.parametrize("dtype,x_dtype", PAIRS)
+@pytest.mark.parametrize("tokens,hidden", [(2, 5), (40, 4100), (1500, 130)])
+def test_sort_types(device, tokens, hidden, dtype, x_dtype):
+    ids = routes(tokens, 2, 7, tokens)
+    x = (torch.randn(tokens, hidden, device="cuda:0") * 3).to(TYPES[x_dtype])
+    check_sort(ids, x, 7, dtype, sort(ids, x, 7, dtype, x_dtype, 3))
+
+
+@pytest.mark.parametrize("tokens", [9, 3000])
+def test_sort_maps_alone(device, tokens):
+    ids = routes(tokens, 3, 11, tokens)
+    x = torch.zeros(tokens, 16, device="cuda:0")
+    b = sort(ids, x, 11, "f32", "f32", rows=False, inverse=False)
+    offsets, pos, _ = maps(ids, 11)
+    assert torch.equal(b["offsets"].t.cpu(), offsets) and torch.equal(b["pos"].t.cpu(), pos)
+    assert b["route"].untouched(slice(None)) and b["out"].untouched(slice(None))
+
+
+def test_sort_no_tokens(device):
+    offsets = Buf(shape=(301,), dtype=torch.int32)
+    run(rr.sort_tokens, rr.SortTokensArgs(offsets=offsets.ptr, tokens=0, experts=300, hidden=8))
+    assert offsets.intact() and not offsets.t.any()
+
+
+def inputs(tokens, top_k, experts, hidden, dtype, seed, kind="any"):
+    gen = torch.Generator(device="cuda:0")
+    gen.manual_seed(seed)
+    ids = routes(tokens, top_k, experts, seed, kind)
+    _, pos, _ = maps(ids, experts)
+    rows = torch.randn(tokens * top_k, hidden, device="cuda:0", generator=gen).to(TYPES[dtype])
+    weights = torch.softmax(torch.randn(tokens, top_k, device="cuda:0", generator=gen), 1)
+    return ids, pos, rows, weights
+
+
+def combined(pos, rows, weights, tokens, top_k):
+    """The sums in 64 bits and the sums of the terms' magnitudes."""
+    p = pos.view(tokens, top_k).cuda().long()
+    term = rows.double()[p.clamp(min=0)] * weights.double()[:, :, None]
+    term = torch.where((p >= 0)[:, :, None], term, torch.zeros((), dtype=torch.float64, device="cuda:0"))
+    return term.sum(1), term.abs().sum(1)
+
+
+CASES = [(1, 1, 1, 1, "any"), (1, 8, 16, 64, "all"), (3, 2, 5, 7, "any"), (5, 64, 3, 33, "any"), (64, 8, 128, 2048, "all"),
+         (130, 9, 40, 515, "any"), (700, 2, 9, 1023, "any"), (40, 2, 4, 8200, "any"), (300, 17, 20, 100, "any"),
+         (21, 3, 6, 260, "none")]
+
+
+@pytest.mark.parametrize("dtype,y_dtype", PAIRS)
+@pytest.mark.parametrize("tokens,top_k,experts,hidden,kind", CASES)
+def test_combine(device, tokens, top_k, experts, hidden, kind, dtype, y_dtype):
+    _, pos, rows, weights = inputs(tokens, top_k, experts, hidden, dtype, tokens + top_k, kind)
+    for offset in (0, 1):
+        for weighted in (True, False):
+            b = [Buf(rows, offset=offset), Buf(pos.cuda(), offset=offset), Buf(weights, offset=offset),
+                 Buf(shape=(tokens, hidden), dtype=TYPES[y_dtype], offset=offset)]
+            common = dict(route_pos=b[1].ptr, tokens=tokens, top_k=top_k, hidden=hidden, dtype=CODES[dtype])
+            if weighted:
+                run(rr.combine_tokens, rr.CombineTokensArgs(y_sorted=b[0].ptr, route_weights=b[2].ptr, y=b[3].ptr,
+                                                            y_dtype=CODES[y_dtype], **common),
+                    rr.get_combine_tokens_workspace_size)
+            else:
+                run(rr.sort_tokens_backward, rr.SortTokensBackwardArgs(dx_sorted=b[0].ptr, dx=b[3].ptr,
+                                                                       x_dtype=CODES[y_dtype], **common),
+                    rr.get_sort_tokens_backward_workspace_size)
+            assert all(buf.intact() for buf in b)
+            want, size = combined(pos, rows, weights if weighted else torch.ones_like(weights), tokens, top_k)
+            bound = top_k * ROUNDING["f32"] * size * 1.01
+            bound = bound + ROUNDING[y_dtype] * (want.abs() + bound) + LEAST[y_dtype]
+            assert_within(b[3].t, want, bound, "y")
+
+
+@pytest.mark.parametrize("dtype,y_dtype", PAIRS)
+@pytest.mark.parametrize("tokens,top_k,experts,hidden,kind", CASES)
+def test_combine_backward(device, tokens, top_k, experts, hidden, kind, dtype, y_dtype):
+    _, pos, rows, weights = inputs(tokens, top_k, experts, hidden, dtype, 3 * tokens + top_k, kind)
+    dy = torch.randn(tokens, hidden, device="cuda:0").to(TYPES[y_dtype])
+    p = pos.cuda().long()
+    placed = p >= 0
+    token = torch.arange(tokens, device="cuda:0").repeat_interleave(top_k)
+    want_rows = torch.zeros(rows.shape, dtype=torch.float64, device="cuda:0")
+    want_rows[p[placed]] = (dy.double()[token] * weights.double().reshape(-1, 1))[placed]
+    products = torch.where(placed[:, None], dy.double()[token] * rows.double()[p.clamp(min=0)],
+                           torch.zeros((), dtype=torch.float64, device="cuda:0"))
+    count = int(placed.sum())
+    for what in ("both", "rows", "weights", "in place"):
+        b = [Buf(rows, offset=1), Buf(pos.cuda(), offset=1), Buf(weights, offset=1), Buf(dy, offset=1),
+             Buf(shape=rows.shape, dtype=TYPES[dtype], offset=1), Buf(shape=(tokens * top_k,), dtype=torch.float32, offset=1)]
+        out = b[0] if what == "in place" else b[4]
+        run(rr.combine_tokens_backward, rr.CombineTokensBackwardArgs(
+            dy=b[3].ptr, y_sorted=b[0].ptr if what != "rows" else None, route_pos=b[1].ptr, route_weights=b[2].ptr,
+            dy_sorted=out.ptr if what != "weights" else None, droute_weights=b[5].ptr if what != "rows" else None,
+            tokens=tokens, top_k=top_k, hidden=hidden, dtype=CODES[dtype], y_dtype=CODES[y_dtype]),
+            rr.get_combine_tokens_backward_workspace_size)
+        assert all(buf.intact() for buf in b)
+        if what == "weights":
+            assert b[4].untouched(slice(None))
+        else:
+            # one product, rounded in FP32 and then to the type
+            bound = (ROUNDING[dtype] + 2 * ROUNDING["f32"]) * want_rows.abs() + LEAST[dtype]
+            assert_within(out.t[:count], want_rows[:count], bound[:count], "dy_sorted")
+            if what != "in place":
+                assert b[4].untouched(slice(count, None))
+        if what == "rows":
+            assert b[5].untouched(slice(None))
+        else:
+            bound = (hidden + 1) * ROUNDING["f32"] * products.abs().sum(1) + LEAST["f32"]
+            assert_within(b[5].t, products.sum(1), bound, "droute_weights")
+
+
+def test_rows_that_no_route_names_do_not_enter(device):
+    """NaN in rows without a route, NaN weights of routes without a row, positions past the end."""
+    rows = torch.full((6, 40), float("nan"), device="cuda:0")
+    rows[2], rows[4] = 1.0, 2.0
+    pos = torch.tensor([2, -1, 6, 4, -7, 2 ** 31 - 1], dtype=torch.int32, device="cuda:0")
+    weights = torch.tensor([0.5, float("nan"), float("inf"), 0.25, float("nan"), 1.0], device="cuda:0")
+    y = Buf(shape=(3, 40), dtype=torch.float32)
+    run(rr.combine_tokens, rr.CombineTokensArgs(y_sorted=rows.data_ptr(), route_pos=pos.data_ptr(),
+                                                route_weights=weights.data_ptr(), y=y.ptr, tokens=3, top_k=2, hidden=40,
+                                                dtype=CODES["f32"]))
+    assert (y.t[0] == 0.5).all() and (y.t[1] == 0.5).all() and (y.t[2] == 0.0).all()
+    dw = Buf(shape=(6,), dtype=torch.float32)
+    dy = torch.ones(3, 40, device="cuda:0")
+    run(rr.combine_tokens_backward, rr.CombineTokensBackwardArgs(
+        dy=dy.data_ptr(), y_sorted=rows.data_ptr(), route_pos=pos.data_ptr(), route_weights=weights.data_ptr(),
+        droute_weights=dw.ptr, tokens=3, top_k=2, hidden=40, dtype=CODES["f32"]))
+    assert dw.t.tolist() == [40.0, 0.0, 0.0, 80.0, 0.0, 0.0]
+
+
+@pytest.mark.parametrize("tokens,experts,top_k", [(1, 1, 1), (3, 5, 2), (200, 64, 2), (77, 130, 8), (33, 1024, 64),
+                                                  (9, 7, 33), (1000, 3, 3)])
+def test_gate_backward(device, tokens, experts, top_k):
+    """Weights near 1 included: the gradient is then far below its terms without differences."""
+    ids = routes(tokens, top_k, experts, tokens)
+    gen = torch.Generator(device="cuda:0")
+    gen.manual_seed(tokens)
+    w = torch.softmax(8 * torch.randn(tokens, top_k, device="cuda:0", generator=gen), 1)
+    dw = torch.randn(tokens, top_k, device="cuda:0", generator=gen)
+    b = [Buf(ids.cuda(), offset=1), Buf(w, offset=1), Buf(dw, offset=1), Buf(shape=(tokens, experts), dtype=torch.float32, offset=1)]
+    run(rr.topk_gate_backward, rr.TopKGateBackwardArgs(
+        expert_ids=b[0].ptr, weights=b[1].ptr, dweights=b[2].ptr, dlogits=b[3].ptr, tokens=tokens, experts=experts,
+        top_k=top_k), rr.get_topk_gate_backward_workspace_size)
+    assert all(buf.intact() for buf in b)
+    valid = (ids >= 0) & (ids < experts)
+    w64 = w.double().cpu() * valid
+    d64 = dw.double().cpu()
+    terms = w64[:, :, None] * w64[:, None, :] * (d64[:, :, None] - d64[:, None, :])
+    want, size = (torch.zeros(tokens, experts, dtype=torch.float64) for _ in range(2))
+    at = ids.clamp(0, experts - 1).long()
+    want.scatter_add_(1, at, terms.sum(2))
+    size.scatter_add_(1, at, terms.abs().sum(2))
+    bound = (2 * top_k + 3) * ROUNDING["f32"] * size + LEAST["f32"]
+    assert_within(b[3].t.cpu(), want, bound, "dlogits")
+
+
+def test_gate_backward_is_the_gates(device):
+    """Against differences of topk_gate's own weights."""
+    tokens, experts = 40, 9
+    gen = torch.Generator(device="cuda:0")
+    gen.manual_seed(5)
+    logits = torch.randn(tokens, experts, device="cuda:0", generator=gen)
+    ids, w = torch.empty(tokens, 2, dtype=torch.int32, device="cuda:0"), torch.empty(tokens, 2, device="cuda:0")
+
+    def gate(at):
+        run(rr.topk_gate, rr.TopKGateArgs(logits=rr.cview(at.data_ptr()), expert_ids=ids.data_ptr(),
+                                          weights=rr.mview(w.data_ptr()), tokens=tokens, experts=experts))
+        torch.cuda.synchronize()
+        return ids.clone(), w.clone()
+
+    first, weights = gate(logits)
+    dw = torch.randn(tokens, 2, device="cuda:0", generator=gen)
+    grad = torch.empty(tokens, experts, device="cuda:0")
+    run(rr.topk_gate_backward, rr.TopKGateBackwardArgs(
+        expert_ids=first.data_ptr(), weights=weights.data_ptr(), dweights=dw.data_ptr(), dlogits=grad.data_ptr(),
+        tokens=tokens, experts=experts))
+    step = 2.0 ** -8
+    for e in range(experts):
+        shift = torch.zeros_like(logits)
+        shift[:, e] = step
+        (ids_up, up), (ids_down, down) = gate(logits + shift), gate(logits - shift)
+        same = (ids_up == first).all(1) & (ids_down == first).all(1)  # (no other expert was chosen)
+        assert same.sum() > tokens // 2
+        difference = ((up - down).double() * dw.double()).sum(1) / (2 * step)
+        # a third derivative of the softmax is below 1/8; weights are good to 2^-22 over the step
+        bound = dw.abs().double().sum(1) * (step ** 2 / 6 + 2.0 ** -22 / step)
+        assert ((difference - grad[:, e].double()).abs() <= bound)[same].all()
