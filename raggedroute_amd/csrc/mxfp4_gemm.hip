@@ -1,5 +1,5 @@
 // Grouped products of 4-bit rows and weights with a power of two for every 32 elements:
-// 256-column tiles of 256 or 128 rows on v_mfma_scale_f32_16x16x128_f8f6f4, sums in FP32.
+// 256-column tiles of 256 or 128 rows on v_mfma_scale_f32_32x32x64_f8f6f4, sums in FP32.
 //
 //   C[r, n] = sum over blocks b of 2^(Xa[r, b] + Xw[n, b]) sum over k of A[r, k] W[n, k]
 //
@@ -10,11 +10,12 @@
 // 128 bytes (256 elements, eight blocks) of every row of both operands straight from memory into
 // LDS, that many slices ahead of the products and across the end of a tile. A slice's scales
 // (eight bytes a row, side by side in memory) come the same way, a word a lane.
-//  - Lane group g (of 16 lanes) multiplies blocks 2 g and 2 g + 1 of a slice, so that its two
-//    scales lie side by side; the two are the low bytes of one register, and the instruction's
-//    selector takes the one or the other.
-//  - Scales of blocks past the row's last are replaced by 0 (2^-127 times elements that are
-//    zeros: the bytes may be NaN's).
+//  - Lane group g (of 32 lanes) multiplies blocks 4 g .. 4 g + 3 of a slice, so that its four
+//    scales are one register, of which the instruction's selector takes a byte.
+//  - The weights are the instruction's first operand and their rows are dealt to its 32 so
+//    that a lane ends with 16 adjacent columns of a row.
+//  - Scales of blocks past the row's last, whatever their bytes are, are replaced by 0 on both
+//    sides: the elements there, the next row's, then add 2^-254 times 36 at most, nothing.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -37,7 +38,7 @@ namespace {
 using rr::dev::bf16;
 using rr::dev::f16;
 
-typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
 
 constexpr int kThreads = 512;
 constexpr int kScaleBytes = 8;  // of a row's slice
@@ -55,24 +56,26 @@ struct MxKind {
   static constexpr int kBScales = kAScales + ROWS * kScaleBytes;
   static constexpr int kStageBytes = kBScales + kTileCols * kScaleBytes;
   static constexpr int kCols = kDual ? kTileCols / 2 : kTileCols;
+  static_assert(kStageBytes % kSliceBytes == 0, "a chunk's number is bits 4 to 6 of its LDS address");
 };
 
-// Chunk permutations of a row's eight chunks, as in expert_gemm.hip.
-template <bool DUAL>
-__device__ __forceinline__ int swizzle_b(int r) {
-  return (r & 3) | ((r >> (DUAL ? 3 : 4)) & 1) << 2;
-}
+// Column of a fragment's row m: the sums of rows 8 i + 4 g + r are registers 4 i + r of lane group g.
+__device__ __forceinline__ int dealt_column(int m) { return ((m >> 2) & 1) << 4 | (m >> 3) << 2 | (m & 3); }
 
-// HALF: which of the scales' two low bytes counts.
-template <int HALF>
-__device__ __forceinline__ f4 multiply(i4 a, i4 b, f4 c, int a_scale, int b_scale) {
+// Chunk permutation of a weight row's eight chunks: the rows that lanes read together differ
+// in the bits used.
+__device__ __forceinline__ int swizzle_b(int r) { return ((r >> 1) & 3) | ((r >> 4) & 1) << 2; }
+
+// BYTE: which of the scales' counts.
+template <int BYTE>
+__device__ __forceinline__ f16v multiply(i4 a, i4 b, f16v c, int a_scale, int b_scale) {
   typedef int i8 __attribute__((ext_vector_type(8)));
   const i8 a8 = {a[0], a[1], a[2], a[3], 0, 0, 0, 0}, b8 = {b[0], b[1], b[2], b[3], 0, 0, 0, 0};
   constexpr int kE2M1 = 4;
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a8, b8, c, kE2M1, kE2M1, HALF, a_scale, HALF, b_scale);
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a8, b8, c, kE2M1, kE2M1, BYTE, a_scale, BYTE, b_scale);
 }
 
-__device__ __forceinline__ int read_scales(uint32_t at) { return *reinterpret_cast<RR_LDS const uint16_t*>(at); }
+__device__ __forceinline__ int read_word(uint32_t at) { return *reinterpret_cast<RR_LDS const int*>(at); }
 
 // An output tile (uniform).
 struct MxTile {
@@ -85,7 +88,7 @@ struct MxTile {
 // weights, p.a2: of the rows. p.K: blocks of a row.
 template <class P>
 __global__ __launch_bounds__(kThreads, 2) void rr_mxfp4_gemm_kernel(Product prm) {
-  extern __shared__ __align__(16) char smem[];
+  extern __shared__ __align__(128) char smem[];
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((RR_LDS char*)smem));
   int32_t* s_off = reinterpret_cast<int32_t*>(smem + P::kStages * P::kStageBytes);  // [E + 1]
   int32_t* s_pre = s_off + prm.experts + 1;                             // [E + 1] full row tiles before expert e
@@ -94,7 +97,7 @@ __global__ __launch_bounds__(kThreads, 2) void rr_mxfp4_gemm_kernel(Product prm)
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave >> 2, wn = wave & 3;
-  const int li = lane & 15, g = lane >> 4;
+  const int li = lane & 31, g = lane >> 5;
   const int experts = prm.experts;
 
   for (int e = tid; e <= experts; e += kThreads) s_off[e] = rr::dev::offset_at(prm.offsets, e, prm.rows);
@@ -154,26 +157,21 @@ __global__ __launch_bounds__(kThreads, 2) void rr_mxfp4_gemm_kernel(Product prm)
   constexpr int QA = P::kTileRows / 64;  // loads of A
   constexpr int kLoads = QA + 6;         // of a slice
   const int half = wave >> 2;
-  uint32_t a_lane[QA], b_lane[4], a_chunk, b_chunk[2];
-  constexpr int b_bit = P::kDual ? 0 : 1;  // the bit of q that B's chunk depends on
-  const uint32_t row_bytes = static_cast<uint32_t>(prm.lda);
+  // Lane offsets inside eight rows; which eight is the buffer's start.
+  uint32_t a_lane, b_lane[2];
+  const int64_t row_bytes = prm.lda;
+  {
+    const int r = lane >> 3;
+    a_lane = static_cast<uint32_t>(r * prm.lda) + (static_cast<uint32_t>((lane & 7) ^ r) << 4);
 #pragma unroll
-  for (int q = 0; q < QA; ++q) {
-    const int r = (QA == 4 ? 128 * half + 64 * (q >> 1) + 16 * wn + 8 * (q & 1) : 16 * wave + 8 * q) + (lane >> 3);
-    a_chunk = static_cast<uint32_t>((lane & 7) ^ (r & 7)) << 4;
-    a_lane[q] = static_cast<uint32_t>(r) * row_bytes + a_chunk;
+    for (int q = 0; q < 2; ++q) b_lane[q] = static_cast<uint32_t>(r * prm.lda) + (static_cast<uint32_t>((lane & 7) ^ swizzle_b(16 * q + r)) << 4);
   }
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int r = 32 * wn + 8 * q + (lane >> 3);
-    const uint32_t chunk = static_cast<uint32_t>((lane & 7) ^ swizzle_b<P::kDual>(r)) << 4;
-    b_chunk[(q >> b_bit) & 1] = chunk;
-    b_lane[q] = static_cast<uint32_t>(r) * row_bytes + chunk;
-  }
+  const int a_first = QA == 4 ? 128 * half + 16 * wn : 16 * wave;  // the wave's first rows
+  const int b_first = 32 * wn;
   const uint32_t a_scale_lane = static_cast<uint32_t>((QA == 4 ? 32 : 16) * wave * kScaleBytes + lane * 4);
   const uint32_t b_scale_lane = static_cast<uint32_t>(32 * wn * kScaleBytes + lane * 4);
   const uint32_t to_a = lds0 + (QA == 4 ? half * kHalfBytes + wn * 2048 : wave * 2048);
-  auto a_to = [&](int q) -> uint32_t { return (q >> 1) * 8192 + (q & 1) * 1024; };
+  auto a_to = [](int q) -> uint32_t { return (q >> 1) * 8192 + (q & 1) * 1024; };
   const uint32_t to_b = lds0 + P::kABytes + wave * 4096;
   const uint32_t to_a_scale = lds0 + P::kAScales + (QA == 4 ? 32 : 16) * wave * kScaleBytes;
   const uint32_t to_b_scale = lds0 + P::kBScales + 32 * wave * kScaleBytes;
@@ -183,8 +181,8 @@ __global__ __launch_bounds__(kThreads, 2) void rr_mxfp4_gemm_kernel(Product prm)
   bool open;            // there is one
   int slice = 0;        // its slice to be loaded
   const char *a_at, *b_at, *as_at, *bs_at;  // the slice of each operand, and the bytes to the operand's end from there
-  int64_t a_left, b_left, as_left, bs_left;
-  int k_left;  // bytes of a row from the slice on
+  int64_t a_left, b_left;
+  int as_left, bs_left;
   const int64_t a_scale_slice = static_cast<int64_t>(prm.rows) * kScaleBytes;  // bytes between slices
   const int64_t b_scale_slice = static_cast<int64_t>(experts) * prm.N * kScaleBytes;
   auto start_tile = [&]() {
@@ -202,19 +200,20 @@ __global__ __launch_bounds__(kThreads, 2) void rr_mxfp4_gemm_kernel(Product prm)
     a_at = static_cast<const char*>(prm.a) + static_cast<int64_t>(next.row0) * prm.lda;
     a_left = static_cast<int64_t>(next.rows) * prm.lda;
     as_at = static_cast<const char*>(prm.a2) + static_cast<int64_t>(next.row0) * kScaleBytes;
-    as_left = static_cast<int64_t>(next.rows) * kScaleBytes;
+    as_left = next.rows * kScaleBytes;
     b_at = b + channel * prm.lda;
     b_left = static_cast<int64_t>(columns) * prm.lda;
     bs_at = bs + channel * kScaleBytes;
-    bs_left = static_cast<int64_t>(columns) * kScaleBytes;
-    k_left = prm.lda;
+    bs_left = columns * kScaleBytes;
   };
-  auto cut = [&](uint32_t offset, uint32_t chunk) { return static_cast<int>(chunk) < k_left ? offset : kPast; };
+  // (what lies past a row's end in its last slice is the next row's: its scales count as 2^-127)
   auto load_a = [&](uint32_t stage, int q) {
-    load_to_lds(make_buffer(a_at, a_left), cut(a_lane[q], a_chunk), to_a + stage + a_to(q));
+    const int64_t from = (a_first + 64 * (q >> 1) + 8 * (q & 1)) * row_bytes;
+    load_to_lds(make_buffer(a_at + from, a_left - from), a_lane, to_a + stage + a_to(q));
   };
   auto load_b = [&](uint32_t stage, int q) {
-    load_to_lds(make_buffer(b_at, b_left), cut(b_lane[q], b_chunk[(q >> b_bit) & 1]), to_b + stage + q * 1024);
+    const int64_t from = (b_first + 8 * q) * row_bytes;
+    load_to_lds(make_buffer(b_at + from, b_left - from), b_lane[q >> 1], to_b + stage + q * 1024);
   };
   auto load_scales = [&](uint32_t stage) {
     if (QA == 4 || lane < 32) load_words_to_lds(make_buffer(as_at, as_left), a_scale_lane, to_a_scale + stage);
@@ -228,7 +227,6 @@ __global__ __launch_bounds__(kThreads, 2) void rr_mxfp4_gemm_kernel(Product prm)
     b_left -= kSliceBytes;
     as_at += a_scale_slice;
     bs_at += b_scale_slice;
-    k_left -= kSliceBytes;
     ++slice;
     if (slice == slices) {
       dealt += grid;
@@ -237,22 +235,19 @@ __global__ __launch_bounds__(kThreads, 2) void rr_mxfp4_gemm_kernel(Product prm)
   };
 
   // ---- operand reads ----
-  uint32_t b_read[2];  // per half: block 2 g, block 2 g + 1
+  uint32_t b_read;  // block 4 g; t blocks further: the address ^ (t << 4)
   uint32_t b_scale;
   {
-    const int r = (P::kDual ? 32 * wn + 8 * (li >> 2) : 64 * (wn & 1) + 16 * (li >> 2)) + (li & 3);
+    const int r = (P::kDual ? 32 * wn : 64 * (wn & 1)) + dealt_column(li);
     const uint32_t base = lds0 + P::kABytes + (P::kDual ? 0 : (wn >> 1) * kHalfBytes) + r * kSliceBytes;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) b_read[h] = base + (static_cast<uint32_t>((2 * g + h) ^ swizzle_b<P::kDual>(r)) << 4);
-    b_scale = lds0 + P::kBScales + (r + (P::kDual ? 0 : (wn >> 1) * 128)) * kScaleBytes + 2 * g;
+    b_read = base + (static_cast<uint32_t>((4 * g) ^ swizzle_b(r)) << 4);
+    b_scale = lds0 + P::kBScales + (r + (P::kDual ? 0 : (wn >> 1) * 128)) * kScaleBytes + 4 * g;
   }
-  // fragment j (0..3; dual: gate 0, 1, up 2, 3)
-  auto read_b = [&](uint32_t stage, int j, int h) -> i4 {
-    return read16(b_read[h] + stage + (P::kDual ? (j >> 1) * kHalfBytes + (j & 1) * 4 * kSliceBytes : j * 4 * kSliceBytes));
+  // fragment j (dual: of gate, of up)
+  auto read_b = [&](uint32_t stage, int j, int t) -> i4 {
+    return read16(((b_read + stage) ^ (t << 4)) + j * (P::kDual ? kHalfBytes : 32 * kSliceBytes));
   };
-  auto read_b_scale = [&](uint32_t stage, int j) {
-    return read_scales(b_scale + stage + (P::kDual ? (j >> 1) * 128 + (j & 1) * 4 : j * 4) * kScaleBytes);
-  };
+  auto read_b_scale = [&](uint32_t stage, int j) { return read_word(b_scale + stage + j * (P::kDual ? 128 : 32) * kScaleBytes); };
 
   start_tile();
   if (!open) return;
@@ -273,42 +268,41 @@ __global__ __launch_bounds__(kThreads, 2) void rr_mxfp4_gemm_kernel(Product prm)
   int round = 0;
 
   auto run_tile = [&](auto mi) {
-    constexpr int MI = decltype(mi)::value;  // 16-row fragments of a wave
-    constexpr int MA = MI < 4 ? MI : 4;      // of them in a phase
-    constexpr int PH = 2 * MI / MA;          // phases of a slice: half p % 2, fragments from MA (p / 2)
-    f4 acc[MI][4] = {};
-    const int wrow = wm * 16 * MI;
-    uint32_t a_read[2];
-    const uint32_t base = lds0 + (wrow + li) * kSliceBytes;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) a_read[h] = base + (static_cast<uint32_t>((2 * g + h) ^ (li & 7)) << 4);
-    const uint32_t a_scale = lds0 + P::kAScales + (wrow + li) * kScaleBytes + 2 * g;
-    i4 a[2][MA], b[2][4];  // of this phase and the next, of both halves
-    int as[2][MA], bs[2][4];  // scales: [0] in use, [1] fetched for the next two phases and the next slice
-    int k_blocks = prm.K;  // of a row from the slice on whose scales are fetched
-    auto mask_of = [&](int blocks) { return blocks - 2 * g >= 2 ? 0xFFFF : blocks - 2 * g == 1 ? 0xFF : 0; };
+    constexpr int MI = decltype(mi)::value;  // 32-row fragments of a wave
+    constexpr int MA = MI < 2 ? MI : 2;      // of them in a phase
+    constexpr int PH = 2 * MI / MA;          // phases of a slice: blocks 2 (p % 2) and one more, fragments from MA (p / 2)
+    constexpr int U = 2 * MA;                // pairs of products of a phase
+    f16v acc[MI][2] = {};
+    const int wrow = wm * 32 * MI;
+    const uint32_t a_read = lds0 + (wrow + li) * kSliceBytes + (static_cast<uint32_t>((4 * g) ^ (li & 7)) << 4);
+    const uint32_t a_scale = lds0 + P::kAScales + (wrow + li) * kScaleBytes + 4 * g;
+    i4 a[2][U], b[4][2];  // a of this phase and the next, b of the slice (the next one's from the last phase on)
+    int as[2][MA], bs[2][2];  // scales: [0] in use, [1] fetched for the next fragments and the next slice
+    int k_blocks = prm.K;     // of a row from the slice on that is multiplied
+    auto mask_of = [&](int blocks) {
+      const int n = blocks - 4 * g;
+      return n >= 4 ? -1 : n <= 0 ? 0 : (1 << (8 * n)) - 1;
+    };
     int mask = mask_of(k_blocks);
     // the operands of phase p, in two parts
     auto fetch = [&](uint32_t stage, int p, int part) {
-      const int h = p % 2, i0 = MA * (p / 2);
+      const int t = 2 * (p % 2) + part, i0 = MA * (p / 2);
       if (p < 2) {
 #pragma unroll
-        for (int j = 2 * part; j < 2 * part + 2; ++j) {
-          b[h][j] = read_b(stage, j, h);
-          if (p == 0) bs[1][j] = read_b_scale(stage, j);
-        }
+        for (int j = 0; j < 2; ++j) b[t][j] = read_b(stage, j, t);
+        if (p == 0) bs[1][part] = read_b_scale(stage, part);
       }
 #pragma unroll
-      for (int i = part * (MA / 2); i < (part + 1) * (MA / 2); ++i) {
-        a[p & 1][i] = read16(a_read[h] + stage + (i0 + i) * 16 * kSliceBytes);
-        if (h == 0) as[1][i] = read_scales(a_scale + stage + (i0 + i) * 16 * kScaleBytes);
+      for (int i = 0; i < MA; ++i) {
+        a[p & 1][part * MA + i] = read16(((a_read + stage) ^ (t << 4)) + (i0 + i) * 32 * kSliceBytes);
+        if (p % 2 == 0 && part == 0) as[1][i] = read_word(a_scale + stage + (i0 + i) * 32 * kScaleBytes);
       }
     };
     fetch(stage, 0, 0);
     fetch(stage, 0, 1);
     // The phases of a slice, its barriers and its loads are those of expert_gemm.hip; the
-    // scales of the next slice are loaded in the last phase, when those of this one have been
-    // read.
+    // scales of the slice after the next are loaded in the last phase, when those of this one
+    // have been read.
     constexpr bool kSpread = PH == 4;
     auto a_phase = [](int q) { return kSpread && q < 2 ? 2 : PH - 1; };
     auto b_phase = [](int q) { return !kSpread ? PH - 1 : q < 3 ? 1 : 2; };
@@ -318,12 +312,12 @@ __global__ __launch_bounds__(kThreads, 2) void rr_mxfp4_gemm_kernel(Product prm)
       const uint32_t st = stage;
 #pragma unroll
       for (int p = 0; p < PH; ++p) {
-        const int h = p % 2, i0 = MA * (p / 2);
+        const int i0 = MA * (p / 2);
         if (p == 0) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) bs[0][j] = bs[1][j] & mask;
+          for (int j = 0; j < 2; ++j) bs[0][j] = bs[1][j] & mask;
         }
-        if (h == 0) {
+        if (p % 2 == 0) {
 #pragma unroll
           for (int i = 0; i < MA; ++i) as[0][i] = as[1][i] & mask;
         }
@@ -334,25 +328,34 @@ __global__ __launch_bounds__(kThreads, 2) void rr_mxfp4_gemm_kernel(Product prm)
           if (p == PH - 1) stage = stage == (P::kStages - 1) * P::kStageBytes ? 0 : stage + P::kStageBytes;
         }
 #pragma unroll
-        for (int i = 0; i < MA; ++i) {
-          if (i < 2) {
+        for (int u = 0; u < U; ++u) {
+          if (u < 2) {
             if (p < PH - 1) {
-              fetch(stage, p + 1, i);
+              fetch(stage, p + 1, u);
             } else if (!last) {
-              fetch(stage, 0, i);
+              fetch(stage, 0, u);
             }
           }
 #pragma unroll
-          for (int q = i * 4 / MA; q < (i + 1) * 4 / MA; ++q) {
+          for (int q = u * 4 / U; q < (u + 1) * 4 / U; ++q) {
             if (q < QA && p == a_phase(q)) load_a(st, q);
             if (p == b_phase(q)) load_b(st, q);
             if (q == 3 && p == PH - 1) load_scales(st);
           }
           __builtin_amdgcn_sched_barrier(0);
+          const int i = i0 + u % MA;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            acc[i0 + i][j] = h == 0 ? multiply<0>(b[h][j], a[p & 1][i], acc[i0 + i][j], bs[0][j], as[0][i])
-                                    : multiply<1>(b[h][j], a[p & 1][i], acc[i0 + i][j], bs[0][j], as[0][i]);
+          for (int j = 0; j < 2; ++j) {
+            const i4 w = b[2 * (p % 2) + u / MA][j], x = a[p & 1][u];
+            const int ws = bs[0][j], xs = as[0][u % MA];
+            if (p % 2 == 0) {
+              acc[i][j] = u / MA == 0 ? multiply<0>(w, x, acc[i][j], ws, xs) : multiply<1>(w, x, acc[i][j], ws, xs);
+            } else {
+              acc[i][j] = u / MA == 0 ? multiply<2>(w, x, acc[i][j], ws, xs) : multiply<3>(w, x, acc[i][j], ws, xs);
+            }
+            // (the compiler takes these products for pure and would move them all behind the
+            // slice's loads, with their operands in registers until then)
+            asm volatile("" : "+v"(acc[i][j]));
           }
           __builtin_amdgcn_sched_barrier(0);
         }
@@ -361,30 +364,31 @@ __global__ __launch_bounds__(kThreads, 2) void rr_mxfp4_gemm_kernel(Product prm)
       mask = mask_of(k_blocks);
       advance();
     }
-    // lane: rows wrow + 16 i + li, 16 columns from 16 g (dual: 8 from 8 g) of the wave's
+    // lane: rows wrow + 32 i + li, 16 columns from 16 g of each fragment's 32
     const std::size_t row0 = tl.row0;
-    const int n = tl.n0 + (P::kDual ? 32 * wn + 8 * g : 64 * wn + 16 * g);
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
-      const int r = wrow + 16 * i + li;
+      const int r = wrow + 32 * i + li;
       if (r >= tl.rows) continue;
-      if constexpr (P::kDual) {
-        if (n >= prm.N) continue;
-        float v[8], u[8];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          v[q] = acc[i][q >> 2][q & 3];
-          u[q] = acc[i][2 + (q >> 2)][q & 3];
-        }
-        P::Epi::template emit<8>(prm, tl.e, row0 + r, n, prm.N - n, v, u);
-      } else {
+      for (int c = 0; c < 2; ++c) {  // eight columns of both operands, or 16 of a fragment
+        if constexpr (P::kDual) {
+          const int n = tl.n0 + 32 * wn + 16 * g + 8 * c;
+          if (n >= prm.N) continue;
+          float v[8], u[8];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          if (n + 8 * c >= prm.N) continue;
-          float v[8];
+          for (int q = 0; q < 8; ++q) {
+            v[q] = acc[i][0][8 * c + q];
+            u[q] = acc[i][1][8 * c + q];
+          }
+          P::Epi::template emit<8>(prm, tl.e, row0 + r, n, prm.N - n, v, u);
+        } else {
+          const int n = tl.n0 + 64 * wn + 32 * c + 16 * g;
+          if (n >= prm.N) continue;
+          float v[16];
 #pragma unroll
-          for (int q = 0; q < 8; ++q) v[q] = acc[i][2 * c + (q >> 2)][q & 3];
-          P::Epi::template emit<8>(prm, tl.e, row0 + r, n + 8 * c, prm.N - n - 8 * c, v);
+          for (int q = 0; q < 16; ++q) v[q] = acc[i][c][q];
+          P::Epi::template emit<16>(prm, tl.e, row0 + r, n, prm.N - n, v);
         }
       }
     }
@@ -393,11 +397,11 @@ __global__ __launch_bounds__(kThreads, 2) void rr_mxfp4_gemm_kernel(Product prm)
 #pragma unroll 1
   for (;;) {
     if (P::kTileRows == 256 && tl.rows > 128) {
-      if constexpr (P::kTileRows == 256) run_tile(std::integral_constant<int, 8>{});
+      if constexpr (P::kTileRows == 256) run_tile(std::integral_constant<int, 4>{});
     } else if (tl.rows > 64) {
-      run_tile(std::integral_constant<int, 4>{});
-    } else {
       run_tile(std::integral_constant<int, 2>{});
+    } else {
+      run_tile(std::integral_constant<int, 1>{});
     }
     round += grid;
     if (!decode(round, tl)) break;
