@@ -656,6 +656,7 @@ rr_status rr_int8_grouped_gemm(const rr_int8_grouped_gemm_args* args,
  * A route whose id is none of 0..experts-1 (padding) is not placed: its route_pos is -1, and
  * the last entries of sorted_route are -1. Rows of x_sorted past offsets[experts] are left
  * alone. x_sorted NULL: the maps alone (x is not read). Without tokens offsets is zeros.
+ * Workspace: rr_sort_tokens_workspace_size (0 for few routes), 16-byte aligned.
  */
 typedef struct rr_sort_tokens_args {
   const void* x;             /* [tokens, hidden] of x_dtype */
@@ -812,6 +813,7 @@ typedef struct rr_mxfp4_grouped_gemm_args {
   rr_kernel_selection kernel;
 } rr_mxfp4_grouped_gemm_args;
 
+/* counts of parts of the routes: many routes only, else 0 */
 size_t rr_sort_tokens_workspace_size(const rr_sort_tokens_args* args);
 size_t rr_sort_tokens_backward_workspace_size(const rr_sort_tokens_backward_args* args);
 size_t rr_combine_tokens_workspace_size(const rr_combine_tokens_args* args);

@@ -28,21 +28,33 @@ using rr::dev::f16;
 
 constexpr int kThreads = 256;
 
+// Rows of any width, of whole pieces, or those with results past the caches: where they are
+// larger than what the next kernel finds in an L2 (65536 rows of 2048 BF16 numbers: sorting 78
+// -> 69 us, combining and its gradients, which read the rows again, 185 -> 165).
+constexpr int kAny = 0, kWhole = 1, kStreamed = 2;
+constexpr std::size_t kStreamedBytes = std::size_t{16} << 20;
+
 // V elements of a row, any alignment that the type has; `left` of them exist.
 template <typename T, int V>
 struct Piece {
   typedef T vec __attribute__((ext_vector_type(V), aligned(sizeof(T))));
   vec v;
+  template <int MODE>
   __device__ __forceinline__ void load(const T* p, int left) {
-    if (left >= V) {
+    if (MODE != kAny || left >= V) {
       v = *reinterpret_cast<const vec*>(p);
       return;
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) v[i] = i < left ? p[i] : static_cast<T>(0.0F);
   }
+  template <int MODE>
   __device__ __forceinline__ void store(T* p, int left) const {
-    if (left >= V) {
+    if constexpr (MODE == kStreamed) {
+      __builtin_nontemporal_store(v, reinterpret_cast<vec*>(p));
+      return;
+    }
+    if (MODE != kAny || left >= V) {
       *reinterpret_cast<vec*>(p) = v;
       return;
     }
@@ -131,58 +143,251 @@ __global__ __launch_bounds__(kThreads) void rr_sort_few_kernel(SortParams p, int
     const int c = (chunk * kThreads + tid) * V;
     if (c >= p.hidden) return;
     Piece<TX, V> x;
-    x.load(static_cast<const TX*>(p.x) + static_cast<std::size_t>(token) * p.hidden + c, p.hidden - c);
+    x.template load<kAny>(static_cast<const TX*>(p.x) + static_cast<std::size_t>(token) * p.hidden + c, p.hidden - c);
     const Piece<T, V> o = converted<T>(x);
     for (int j = 0; j < p.top_k; ++j) {
-      if (s_pos[j] >= 0) o.store(static_cast<T*>(p.x_sorted) + static_cast<std::size_t>(s_pos[j]) * p.hidden + c, p.hidden - c);
+      if (s_pos[j] >= 0) o.template store<kAny>(static_cast<T*>(p.x_sorted) + static_cast<std::size_t>(s_pos[j]) * p.hidden + c, p.hidden - c);
     }
   }
 }
 
-// Any number of routes: a workgroup owns G experts and reads all ids twice, its 16 waves a
-// contiguous share each, four ids a lane. The first pass counts the ids below the workgroup's
-// experts and those of each; the second gives the routes of its experts their positions. No
-// workgroup waits for another and nothing is added atomically.
-constexpr int kRankWaves = 16;
+// More routes: a workgroup owns the routes of some tokens. It counts the ids before its own and
+// those from there on (LDS, an atomic addition for each: counts do not depend on their order),
+// or, COUNTED, sums the counts of the chunks, which a launch before it made, and counts the ids of
+// its own chunk alone; a scan over the experts then gives where each begins, and one wave
+// ranks the workgroup's routes by ballots, 64 at a time in their order. No workgroup waits for
+// another.
+//  - Up to kCountedRoutes every workgroup counts all ids and copies its tokens' rows, too: one
+//    launch (6002 routes of nine experts, rows of 1023: 10.5 us, in two launches 13.5).
+//  - Above, the rows are another launch's, a workgroup a token in the tokens' order, which
+//    writes a row behind the other in every expert's segment (32768 rows of 4096 BF16 numbers of
+//    eight experts: 80 us; 512 workgroups that copy what they own, spread over the segments, 88).
+//    Maps of 65536 routes of 128 experts 8.3 us; by workgroups that own an expert and read all
+//    ids 15.
+constexpr int kOwnedRoutes = 512;  // of a workgroup at most
+constexpr int kOwners = 512;       // workgroups, or as many as routes make of kOwnedRoutes
+constexpr int kCountedRoutes = 8192;
+constexpr int kCountedExperts = 256;
+constexpr int kChunks = 32;
 
-template <int G>
+// Routes of a chunk: a multiple of 256, as few as make kChunks chunks or fewer.
+__host__ __device__ inline int64_t chunk_routes(int64_t routes) { return (routes + kChunks * 256 - 1) / (kChunks * 256) * 256; }
+
+// Adds the ids [begin, end) to the counts of LDS, `threads` at a time.
+template <int THREADS>
+__device__ __forceinline__ void count_ids(int32_t* counts, const int32_t* ids, int64_t begin, int64_t end, int experts, int tid) {
+  constexpr int kBatchIds = 4;
+  for (int64_t from = begin; from < end; from += THREADS * kBatchIds) {
+    int id[kBatchIds];
+#pragma unroll
+    for (int i = 0; i < kBatchIds; ++i) {
+      const int64_t at = from + i * THREADS + tid;
+      id[i] = at < end ? ids[at] : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < kBatchIds; ++i) {
+      if (static_cast<unsigned>(id[i]) < static_cast<unsigned>(experts)) atomicAdd(counts + id[i], 1);
+    }
+  }
+}
+
+__global__ __launch_bounds__(1024) void rr_sort_count_kernel(SortParams p) {
+  __shared__ int32_t s_counts[kCountedExperts];
+  const int tid = static_cast<int>(threadIdx.x);
+  const int64_t routes = static_cast<int64_t>(p.tokens) * p.top_k, chunk = chunk_routes(routes);
+  const int64_t begin = static_cast<int64_t>(blockIdx.x) * chunk;
+  if (tid < p.experts) s_counts[tid] = 0;
+  __syncthreads();
+  count_ids<1024>(s_counts, p.ids, begin, begin + chunk < routes ? begin + chunk : routes, p.experts, tid);
+  __syncthreads();
+  if (tid < p.experts) p.counts[static_cast<int>(blockIdx.x) * p.experts + tid] = s_counts[tid];
+}
+
+template <typename TX, typename T, int MODE, bool COUNTED, bool ROWS>
+__global__ __launch_bounds__(kThreads) void rr_sort_owned_kernel(SortParams p, int owned) {
+  static_assert(kCountedExperts <= kThreads, "a thread an expert");
+  __shared__ int32_t s_before[kCountedExperts], s_from[kCountedExperts];  // ids before the workgroup's own; from there on
+  __shared__ int32_t s_wave[kThreads / 64];
+  __shared__ int32_t s_pos[kOwnedRoutes];
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
+  const int64_t routes = static_cast<int64_t>(p.tokens) * p.top_k;
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * owned;
+  const int tokens = static_cast<int>(p.tokens - t0 < owned ? p.tokens - t0 : owned);
+  const int64_t r0 = t0 * p.top_k;
+  const int count = tokens * p.top_k;
+  if (tid < p.experts) s_before[tid] = s_from[tid] = 0;
+  __syncthreads();
+  if constexpr (COUNTED) {
+    const int64_t chunk = chunk_routes(routes);
+    const int mine = static_cast<int>(r0 / chunk), chunks = static_cast<int>((routes + chunk - 1) / chunk);
+    // every expert's chunks shared among as many threads as there are for it
+    const int shares = kThreads / p.experts;
+    const int e = tid % p.experts, share = tid / p.experts;
+    if (share < shares) {
+      int32_t before = 0, from = 0;
+#pragma unroll 8
+      for (int c = share; c < chunks; c += shares) {
+        const int32_t n = p.counts[c * p.experts + e];
+        before += c < mine ? n : 0;
+        from += c < mine ? 0 : n;
+      }
+      atomicAdd(s_before + e, before);
+      atomicAdd(s_from + e, from);
+    }
+    // (those of its own chunk counted as from there on so far)
+    const int64_t begin = mine * chunk;
+    for (int64_t at = begin + tid; at < r0; at += kThreads) {
+      const int id = p.ids[at];
+      if (static_cast<unsigned>(id) < static_cast<unsigned>(p.experts)) {
+        atomicAdd(s_before + id, 1);
+        atomicAdd(s_from + id, -1);
+      }
+    }
+  } else {
+    count_ids<kThreads>(s_before, p.ids, 0, r0, p.experts, tid);
+    count_ids<kThreads>(s_from, p.ids, r0, routes, p.experts, tid);
+  }
+  __syncthreads();
+  // where every expert begins, and this workgroup's first route of it
+  {
+    const int32_t all = tid < p.experts ? s_before[tid] + s_from[tid] : 0;
+    const int32_t through = rr::dev::wave_inclusive_scan(all);
+    if (lane == 63) s_wave[tid >> 6] = through;
+    __syncthreads();
+    int32_t start = through - all;
+    int32_t placed = 0;
+    for (int w = 0; w < kThreads / 64; ++w) {
+      start += w < tid >> 6 ? s_wave[w] : 0;
+      placed += s_wave[w];
+    }
+    if (tid < p.experts) s_before[tid] += start;
+    if (blockIdx.x == 0) {
+      if (tid < p.experts) p.offsets[tid] = start;
+      if (tid == 0) p.offsets[p.experts] = placed;
+    }
+    if (p.sorted_route != nullptr) {  // (the last entries, spread over the workgroups)
+      for (int64_t i = placed + static_cast<int64_t>(blockIdx.x) * kThreads + tid; i < routes; i += static_cast<int64_t>(gridDim.x) * kThreads) {
+        p.sorted_route[i] = -1;
+      }
+    }
+  }
+  __syncthreads();
+  if (tid < 64) {
+    const int bits = rr::dev::bits_for(p.experts);
+    for (int i = 0; i < count; i += 64) {
+      const int at = i + lane;
+      const int id = at < count ? p.ids[r0 + at] : -1;
+      const bool valid = static_cast<unsigned>(id) < static_cast<unsigned>(p.experts);
+      const uint64_t same = rr::dev::match_mask(valid ? id : 0, bits, __ballot(valid));
+      const int rank = __popcll(same & rr::dev::lanemask_lt());
+      int32_t pos = -1;
+      if (valid) {
+        pos = s_before[id] + rank;
+        rr::dev::wave_lds_sync();
+        if (rank == 0) s_before[id] += __popcll(same);
+      }
+      rr::dev::wave_lds_sync();
+      if (at < count) {
+        s_pos[at] = pos;
+        p.route_pos[r0 + at] = pos;
+        if (pos >= 0 && p.sorted_route != nullptr) p.sorted_route[pos] = static_cast<int32_t>(r0 + at);
+      }
+    }
+  }
+  if constexpr (ROWS) {
+    __syncthreads();
+    constexpr int V = kPiece<T>;
+    const auto* x = static_cast<const TX*>(p.x);
+    auto* out = static_cast<T*>(p.x_sorted);
+    const std::size_t H = p.hidden;
+    // Pieces of the tokens' rows in a row, several on their way together.
+    constexpr int kAhead = 4;
+    const int pieces = (p.hidden + V - 1) / V;
+    int t = tid / pieces, c = tid % pieces;  // of the next piece
+    const int t_step = kThreads / pieces, c_step = kThreads % pieces;
+    while (t < tokens) {
+      Piece<TX, V> piece[kAhead];
+      int token[kAhead], column[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        token[k] = t;
+        column[k] = c * V;
+        if (t < tokens) piece[k].template load<MODE>(x + (t0 + t) * H + column[k], p.hidden - column[k]);
+        t += t_step;
+        c += c_step;
+        if (c >= pieces) {
+          c -= pieces;
+          ++t;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        if (token[k] >= tokens) continue;
+        const Piece<T, V> o = converted<T>(piece[k]);
+        for (int j = 0; j < p.top_k; ++j) {
+          const int pos = s_pos[token[k] * p.top_k + j];
+          if (pos >= 0) o.template store<MODE>(out + pos * H + column[k], p.hidden - column[k]);
+        }
+      }
+    }
+  }
+}
+
+// Many experts: a workgroup owns G of them and reads all ids twice, its 16 waves a contiguous
+// share each, four ids a lane and load, eight loads at a time. The first pass counts the ids below the workgroup's experts
+// and those of each; the second gives the routes of its experts their positions. No workgroup
+// waits for another and nothing is added atomically.
+constexpr int kRankWaves = 16;
+constexpr int kRankLoads = 8;
+constexpr int kRankExperts = 4;  // of a workgroup
+
 __global__ __launch_bounds__(64 * kRankWaves) void rr_sort_rank_kernel(SortParams p) {
+  constexpr int G = kRankExperts;
   __shared__ int32_t s_count[G + 1][kRankWaves];  // of a wave's ids: [0] below, [1 + g] of expert e0 + g
   typedef int quad __attribute__((ext_vector_type(4), aligned(4)));
+  constexpr int kStep = 256 * kRankLoads;  // ids of a wave's step
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int e0 = static_cast<int>(blockIdx.x) * G;
   const int64_t routes = static_cast<int64_t>(p.tokens) * p.top_k;
   const int64_t share = ((routes + kRankWaves * 256 - 1) / (kRankWaves * 256)) * 256;
   const int64_t begin = share * wave, end = begin + share < routes ? begin + share : routes;
-  // (an id that is none of 0..experts-1 becomes -1: as an unsigned number above all)
-  auto load = [&](int64_t at) {
-    quad v;
-    const int64_t left = end - at;
-    if (left >= 4) {
-      v = *reinterpret_cast<const quad*>(p.ids + at);
-    } else {
+  // (as unsigned numbers, ids below 0 are above all; so is what stands for those past the end)
+  quad v[kRankLoads];
+  auto load = [&](int64_t from) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = i < left ? p.ids[at + i] : -1;
+    for (int q = 0; q < kRankLoads; ++q) {
+      const int64_t at = from + 256 * q + 4 * lane;
+      v[q] = quad{-1, -1, -1, -1};
+      if (at + 4 <= end) {
+        v[q] = *reinterpret_cast<const quad*>(p.ids + at);
+      } else if (at < end) {
+        for (int i = 0; at + i < end; ++i) {
+          const int id = p.ids[at + i];
+          v[q][0] = i == 0 ? id : v[q][0];
+          v[q][1] = i == 1 ? id : v[q][1];
+          v[q][2] = i == 2 ? id : v[q][2];
+        }
+      }
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = static_cast<unsigned>(v[i]) < static_cast<unsigned>(p.experts) ? v[i] : -1;
-    return v;
   };
   int32_t below = 0, mine[G] = {};
-  for (int64_t at = begin + 4 * lane; at - 4 * lane < end; at += 256) {
-    const quad v = load(at);
+  for (int64_t from = begin; from < end; from += kStep) {
+    load(from);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      below += __popcll(__ballot(static_cast<unsigned>(v[i]) < static_cast<unsigned>(e0)));
+    for (int q = 0; q < kRankLoads; ++q) {
 #pragma unroll
-      for (int g = 0; g < G; ++g) mine[g] += __popcll(__ballot(v[i] == e0 + g));
+      for (int i = 0; i < 4; ++i) {
+        below += __popcll(__ballot(static_cast<unsigned>(v[q][i]) < static_cast<unsigned>(e0)));
+#pragma unroll
+        for (int g = 0; g < G; ++g) mine[g] += __popcll(__ballot(v[q][i] == e0 + g));
+      }
     }
   }
   if (lane == 0) {
     s_count[0][wave] = below;
 #pragma unroll
-    for (int g = 0; g < G; ++g) s_count[1 + g][wave] = mine[g];
+    for (int g = 0; g < G; ++g) s_count[1 + g][wave] = e0 + g < p.experts ? mine[g] : 0;
   }
   __syncthreads();
   // where expert e0 + g begins, and this wave's first route of it
@@ -205,34 +410,37 @@ __global__ __launch_bounds__(64 * kRankWaves) void rr_sort_rank_kernel(SortParam
       for (int64_t i = start + tid; i < routes; i += 64 * kRankWaves) p.sorted_route[i] = -1;
     }
   }
-  for (int64_t at = begin + 4 * lane; at - 4 * lane < end; at += 256) {
-    const quad v = load(at);
-    auto place = [&](int i, int32_t pos) {
-      const int64_t r = at + i;
-      if (r >= end) return;
-      p.route_pos[r] = pos;
-      if (pos >= 0 && p.sorted_route != nullptr) p.sorted_route[pos] = static_cast<int32_t>(r);
-    };
+  const uint64_t lower = rr::dev::lanemask_lt();
+  for (int64_t from = begin; from < end; from += kStep) {
+    if (share > kStep) load(from);  // (a share of one step is still there)
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      uint64_t m[4];
+    for (int q = 0; q < kRankLoads; ++q) {
+      const int64_t at = from + 256 * q + 4 * lane;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) m[i] = __ballot(v[i] == e0 + g);
-      if ((m[0] | m[1] | m[2] | m[3]) == 0) continue;
-      int32_t pos = at_wave[g];
-      const uint64_t lower = rr::dev::lanemask_lt();
+      for (int g = 0; g < G; ++g) {
+        if (e0 + g >= p.experts) continue;
+        uint64_t m[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) pos += __popcll(m[i] & lower);
+        for (int i = 0; i < 4; ++i) m[i] = __ballot(v[q][i] == e0 + g);
+        if ((m[0] | m[1] | m[2] | m[3]) == 0) continue;
+        int32_t pos = at_wave[g];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (v[i] == e0 + g) place(i, pos++);
-        at_wave[g] += __popcll(m[i]);
+        for (int i = 0; i < 4; ++i) pos += __popcll(m[i] & lower);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (v[q][i] == e0 + g) {
+            p.route_pos[at + i] = pos;
+            if (p.sorted_route != nullptr) p.sorted_route[pos] = static_cast<int32_t>(at + i);
+            ++pos;
+          }
+          at_wave[g] += __popcll(m[i]);
+        }
       }
-    }
-    if (blockIdx.x == 0) {
+      if (blockIdx.x == 0) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (v[i] < 0) place(i, -1);
+        for (int i = 0; i < 4; ++i) {
+          if (static_cast<unsigned>(v[q][i]) >= static_cast<unsigned>(p.experts) && at + i < end) p.route_pos[at + i] = -1;
+        }
       }
     }
   }
@@ -246,7 +454,7 @@ __device__ __forceinline__ int checked(int32_t pos, int64_t routes) {
 }
 
 // G threads a token: its row read once and stored at the positions of its routes.
-template <typename TX, typename T, int G>
+template <typename TX, typename T, int G, int MODE>
 __global__ __launch_bounds__(kThreads) void rr_sort_rows_kernel(SortParams p) {
   constexpr int V = kPiece<T>;
   const int tid = static_cast<int>(threadIdx.x), lane = tid & (G - 1);
@@ -264,11 +472,11 @@ __global__ __launch_bounds__(kThreads) void rr_sort_rows_kernel(SortParams p) {
       }
       for (int c = lane * V; c < p.hidden; c += G * V) {
         Piece<TX, V> piece;
-        piece.load(x + t * H + c, p.hidden - c);
+        piece.template load<MODE>(x + t * H + c, p.hidden - c);
         const Piece<T, V> o = converted<T>(piece);
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
-          if (pos[j] >= 0) o.store(out + pos[j] * H + c, p.hidden - c);
+          if (pos[j] >= 0) o.template store<MODE>(out + pos[j] * H + c, p.hidden - c);
         }
       }
     }
@@ -276,7 +484,7 @@ __global__ __launch_bounds__(kThreads) void rr_sort_rows_kernel(SortParams p) {
 }
 
 // G threads a token: the sum of its routes' rows.
-template <typename TY, typename T, int G>
+template <typename TY, typename T, int G, int MODE>
 __global__ __launch_bounds__(kThreads) void rr_combine_kernel(CombineParams p) {
   constexpr int V = kPiece<T>;
   const int tid = static_cast<int>(threadIdx.x), lane = tid & (G - 1);
@@ -300,7 +508,7 @@ __global__ __launch_bounds__(kThreads) void rr_combine_kernel(CombineParams p) {
         }
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
-          if (j0 + j < p.top_k) row[j].load(rows + max(pos[j], 0) * H + c, p.hidden - c);
+          if (j0 + j < p.top_k) row[j].template load<MODE>(rows + max(pos[j], 0) * H + c, p.hidden - c);
         }
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
@@ -313,17 +521,18 @@ __global__ __launch_bounds__(kThreads) void rr_combine_kernel(CombineParams p) {
       Piece<TY, V> o;
 #pragma unroll
       for (int i = 0; i < V; ++i) o.v[i] = static_cast<TY>(sum[i]);
-      o.store(out + t * H + c, p.hidden - c);
+      o.template store<MODE>(out + t * H + c, p.hidden - c);
     }
   }
 }
 
 // G threads a token: the gradients of its routes' rows and weights. The columns' products are
 // added by lane, then over the lanes in a fixed order.
-template <typename TY, typename T, int G>
+template <typename TY, typename T, int G, int MODE>
 __global__ __launch_bounds__(kThreads) void rr_combine_backward_kernel(CombineParams p) {
   constexpr int V = kPiece<T>;
-  __shared__ float s_dot[kThreads / 64][kBatch];
+  __shared__ float s_dot[2][kThreads / 64][kBatch];  // by turns
+  int turn = 0;
   const int tid = static_cast<int>(threadIdx.x), lane = tid & (G - 1);
   const int64_t routes = static_cast<int64_t>(p.tokens) * p.top_k;
   const auto* dy = static_cast<const TY*>(p.dy);
@@ -331,7 +540,7 @@ __global__ __launch_bounds__(kThreads) void rr_combine_backward_kernel(CombinePa
   auto* back = static_cast<T*>(p.dy_sorted);
   const std::size_t H = p.hidden;
   const int64_t step = static_cast<int64_t>(gridDim.x) * (kThreads / G);
-  // (every thread of a workgroup takes every turn: the sums of G = 256 meet at barriers)
+  // (every thread of a workgroup takes every turn: sums of more than a wave meet at barriers)
   for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * (kThreads / G); t0 < p.tokens; t0 += step) {
     const int64_t t = t0 + tid / G;
     const bool here = t < p.tokens;
@@ -347,12 +556,12 @@ __global__ __launch_bounds__(kThreads) void rr_combine_backward_kernel(CombinePa
       }
       for (int c = lane * V; here && c < p.hidden; c += G * V) {
         Piece<TY, V> g;
-        g.load(dy + t * H + c, p.hidden - c);
+        g.template load<MODE>(dy + t * H + c, p.hidden - c);
         if (p.dweights != nullptr) {
           Piece<T, V> row[kBatch];
 #pragma unroll
           for (int j = 0; j < kBatch; ++j) {
-            if (pos[j] >= 0) row[j].load(rows + pos[j] * H + c, p.hidden - c);
+            if (pos[j] >= 0) row[j].template load<MODE>(rows + pos[j] * H + c, p.hidden - c);
           }
 #pragma unroll
           for (int j = 0; j < kBatch; ++j) {
@@ -368,7 +577,7 @@ __global__ __launch_bounds__(kThreads) void rr_combine_backward_kernel(CombinePa
             Piece<T, V> o;
 #pragma unroll
             for (int i = 0; i < V; ++i) o.v[i] = static_cast<T>(w[j] * static_cast<float>(g.v[i]));
-            o.store(back + pos[j] * H + c, p.hidden - c);
+            o.template store<MODE>(back + pos[j] * H + c, p.hidden - c);
           }
         }
       }
@@ -381,17 +590,17 @@ __global__ __launch_bounds__(kThreads) void rr_combine_backward_kernel(CombinePa
       if constexpr (G > 64) {
         if ((tid & 63) == 0) {
 #pragma unroll
-          for (int j = 0; j < kBatch; ++j) s_dot[tid >> 6][j] = dot[j];
+          for (int j = 0; j < kBatch; ++j) s_dot[turn][tid >> 6][j] = dot[j];
         }
-        __syncthreads();
-        if (tid == 0) {
+        __syncthreads();  // (the other turn's sums were read before it)
+        if (lane == 0) {
 #pragma unroll
           for (int j = 0; j < kBatch; ++j) {
             dot[j] = 0.0F;
-            for (int q = 0; q < kThreads / 64; ++q) dot[j] += s_dot[q][j];
+            for (int q = 0; q < G / 64; ++q) dot[j] += s_dot[turn][(tid >> 6) + q][j];
           }
         }
-        __syncthreads();
+        turn ^= 1;
       }
       if (here && lane == 0) {
 #pragma unroll
@@ -448,20 +657,69 @@ unsigned token_grid(int tokens, int per) {
   return static_cast<unsigned>(std::min<int64_t>((static_cast<int64_t>(tokens) + per - 1) / per, 16384));
 }
 
-// Threads of a token: as many as its row has pieces, up to a wave.
-template <typename F>
-hipError_t with_group(int hidden, int piece, F f) {
+// Threads of a token: as many as its row has pieces, up to a workgroup's (a wave for a row of 256
+// pieces: combining 65536 rows of 2048 BF16 numbers 79 us against 59, its gradients 131 against
+// 115). BACKWARD: a wave up to 128 pieces, whose sums then meet at no barrier (gradients of 6002
+// rows of 1023 10 us, with two waves a token 14).
+// `bytes`: of the rows that are written.
+template <bool BACKWARD, typename F>
+hipError_t with_group(int hidden, int piece, std::size_t bytes, F f) {
   const int pieces = (hidden + piece - 1) / piece;
-  if (pieces <= 8) return f(std::integral_constant<int, 8>{});
-  if (pieces <= 16) return f(std::integral_constant<int, 16>{});
-  if (pieces <= 32) return f(std::integral_constant<int, 32>{});
-  if (pieces <= 64) return f(std::integral_constant<int, 64>{});
-  return f(std::integral_constant<int, 256>{});
+  auto with_mode = [&](auto g) {
+    if (hidden % piece != 0) return f(g, std::integral_constant<int, kAny>{});
+    if constexpr (decltype(g)::value >= 64) {
+      if (bytes >= kStreamedBytes) return f(g, std::integral_constant<int, kStreamed>{});
+    }
+    return f(g, std::integral_constant<int, kWhole>{});
+  };
+  if (pieces <= 8) return with_mode(std::integral_constant<int, 8>{});
+  if (pieces <= 16) return with_mode(std::integral_constant<int, 16>{});
+  if (pieces <= 32) return with_mode(std::integral_constant<int, 32>{});
+  if (pieces <= (BACKWARD ? 128 : 64)) return with_mode(std::integral_constant<int, 64>{});
+  if constexpr (!BACKWARD) {
+    if (pieces <= 128) return with_mode(std::integral_constant<int, 128>{});
+  }
+  return with_mode(std::integral_constant<int, 256>{});
+}
+
+template <typename TX, typename T>
+hipError_t sort_rows(const SortParams& p, hipStream_t stream) {
+  const std::size_t bytes = sizeof(T) * p.tokens * p.top_k * p.hidden;
+  return with_group<false>(p.hidden, kPiece<T>, bytes, [&](auto g, auto mode) {
+    constexpr int G = decltype(g)::value;
+    constexpr int M = decltype(mode)::value;
+    rr_sort_rows_kernel<TX, T, G, M><<<token_grid(p.tokens, kThreads / G), kThreads, 0, stream>>>(p);
+    return hipGetLastError();
+  });
 }
 
 template <typename TX, typename T>
 hipError_t sort_typed(const SortParams& p, hipStream_t stream) {
   const int64_t routes = static_cast<int64_t>(p.tokens) * p.top_k;
+  if (routes > kFewRoutes && p.experts <= kCountedExperts) {
+    const int owned = static_cast<int>(std::min<int64_t>((p.tokens + kOwners - 1) / kOwners, kOwnedRoutes / p.top_k));
+    const unsigned grid = static_cast<unsigned>((p.tokens + owned - 1) / owned);
+    const bool counted = routes > kCountedRoutes;
+    if (counted) {
+      const int64_t chunk = chunk_routes(routes);
+      rr_sort_count_kernel<<<static_cast<unsigned>((routes + chunk - 1) / chunk), 1024, 0, stream>>>(p);
+      const hipError_t error = hipGetLastError();
+      if (error != hipSuccess) return error;
+    }
+    if (counted) {
+      rr_sort_owned_kernel<TX, T, kAny, true, false><<<grid, kThreads, 0, stream>>>(p, owned);
+      const hipError_t error = hipGetLastError();
+      return error != hipSuccess || p.x_sorted == nullptr ? error : sort_rows<TX, T>(p, stream);
+    }
+    auto run = [&](auto mode, auto rows) {
+      rr_sort_owned_kernel<TX, T, decltype(mode)::value, false, decltype(rows)::value><<<grid, kThreads, 0, stream>>>(p, owned);
+      return hipGetLastError();
+    };
+    if (p.x_sorted == nullptr) return run(std::integral_constant<int, kAny>{}, std::false_type{});
+    if (p.hidden % kPiece<T> != 0) return run(std::integral_constant<int, kAny>{}, std::true_type{});
+    if (sizeof(T) * routes * p.hidden < kStreamedBytes) return run(std::integral_constant<int, kWhole>{}, std::true_type{});
+    return run(std::integral_constant<int, kStreamed>{}, std::true_type{});
+  }
   if (routes <= kFewRoutes) {
     const int counters = (p.experts + 1 + kThreads - 1) / kThreads;
     if (p.x_sorted == nullptr) {
@@ -472,39 +730,37 @@ hipError_t sort_typed(const SortParams& p, hipStream_t stream) {
     }
     return hipGetLastError();
   }
-  if (p.experts <= 256) {
-    rr_sort_rank_kernel<1><<<p.experts, 64 * kRankWaves, 0, stream>>>(p);
-  } else {
-    rr_sort_rank_kernel<4><<<(p.experts + 3) / 4, 64 * kRankWaves, 0, stream>>>(p);
-  }
+  rr_sort_rank_kernel<<<(p.experts + kRankExperts - 1) / kRankExperts, 64 * kRankWaves, 0, stream>>>(p);
   const hipError_t error = hipGetLastError();
   if (error != hipSuccess || p.x_sorted == nullptr) return error;
-  return with_group(p.hidden, kPiece<T>, [&](auto g) {
-    constexpr int G = decltype(g)::value;
-    rr_sort_rows_kernel<TX, T, G><<<token_grid(p.tokens, kThreads / G), kThreads, 0, stream>>>(p);
-    return hipGetLastError();
-  });
+  return sort_rows<TX, T>(p, stream);
 }
 
 template <typename TY, typename T>
 hipError_t combine_typed(const CombineParams& p, hipStream_t stream) {
-  return with_group(p.hidden, kPiece<T>, [&](auto g) {
+  return with_group<false>(p.hidden, kPiece<T>, sizeof(TY) * p.tokens * p.hidden, [&](auto g, auto mode) {
     constexpr int G = decltype(g)::value;
-    rr_combine_kernel<TY, T, G><<<token_grid(p.tokens, kThreads / G), kThreads, 0, stream>>>(p);
+    constexpr int M = decltype(mode)::value;
+    rr_combine_kernel<TY, T, G, M><<<token_grid(p.tokens, kThreads / G), kThreads, 0, stream>>>(p);
     return hipGetLastError();
   });
 }
 
 template <typename TY, typename T>
 hipError_t backward_typed(const CombineParams& p, hipStream_t stream) {
-  return with_group(p.hidden, kPiece<T>, [&](auto g) {
+  return with_group<true>(p.hidden, kPiece<T>, sizeof(T) * p.tokens * p.top_k * p.hidden, [&](auto g, auto mode) {
     constexpr int G = decltype(g)::value;
-    rr_combine_backward_kernel<TY, T, G><<<token_grid(p.tokens, kThreads / G), kThreads, 0, stream>>>(p);
+    constexpr int M = decltype(mode)::value;
+    rr_combine_backward_kernel<TY, T, G, M><<<token_grid(p.tokens, kThreads / G), kThreads, 0, stream>>>(p);
     return hipGetLastError();
   });
 }
 
 }  // namespace
+
+std::size_t sort_tokens_counts(int64_t routes, int experts) {
+  return routes > kCountedRoutes && experts <= kCountedExperts ? static_cast<std::size_t>(kChunks) * experts : 0;
+}
 
 hipError_t sort_tokens(const SortParams& p, hipStream_t stream) {
   if (p.dtype == RR_DTYPE_FP32) return sort_typed<float, float>(p, stream);

@@ -28,7 +28,10 @@ bool types_ok(int32_t dtype, int32_t other) noexcept {
 
 extern "C" {
 
-size_t rr_sort_tokens_workspace_size(const rr_sort_tokens_args*) { return 0; }
+size_t rr_sort_tokens_workspace_size(const rr_sort_tokens_args* args) {
+  if (args == nullptr || !rr::routes_ok(args->tokens, args->top_k) || !rr::experts_ok(args->experts)) return 0;
+  return rr::kern::sort_tokens_counts(static_cast<int64_t>(args->tokens) * args->top_k, args->experts) * sizeof(int32_t);
+}
 size_t rr_sort_tokens_backward_workspace_size(const rr_sort_tokens_backward_args*) { return 0; }
 size_t rr_combine_tokens_workspace_size(const rr_combine_tokens_args*) { return 0; }
 size_t rr_combine_tokens_backward_workspace_size(const rr_combine_tokens_backward_args*) { return 0; }
@@ -47,7 +50,7 @@ rr_status rr_sort_tokens(const rr_sort_tokens_args* args, const rr_runtime_conte
     return rr::make_status(RR_STATUS_UNSUPPORTED_DATA_TYPE,
                            "sort_tokens: dtype must be FP32, FP16 or BF16 and x_dtype the same or FP32");
   }
-  const rr_status status = rr::choose_family(a.kernel, context->architecture, nullptr);
+  rr_status status = rr::choose_family(a.kernel, context->architecture, nullptr);
   if (status.code != RR_STATUS_SUCCESS) return status;
   // without tokens the offsets are still written (zeros)
   if (a.offsets == nullptr || (a.tokens != 0 && rr::any_null({a.expert_ids, a.route_pos})) ||
@@ -58,7 +61,11 @@ rr_status rr_sort_tokens(const rr_sort_tokens_args* args, const rr_runtime_conte
       !rr::is_aligned(a.x, rr::type_size(a.x_dtype)) || !rr::is_aligned(a.x_sorted, rr::type_size(a.dtype))) {
     return rr::invalid_argument("sort_tokens: every buffer must be aligned to its element type");
   }
+  status = rr::check_workspace(context, rr_sort_tokens_workspace_size(args),
+                               "sort_tokens: the workspace must hold the counts of parts of the routes");
+  if (status.code != RR_STATUS_SUCCESS) return status;
   rr::kern::SortParams p{};
+  p.counts = static_cast<int32_t*>(context->workspace);
   p.x = a.x;
   p.ids = a.expert_ids;
   p.offsets = a.offsets;

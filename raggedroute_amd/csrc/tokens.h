@@ -17,6 +17,7 @@ struct SortParams {
   int32_t* route_pos;
   int32_t* sorted_route;  // optional
   void* x_sorted;         // optional
+  int32_t* counts;        // workspace: sort_tokens_counts() numbers
   int tokens, experts, top_k, hidden;
   int dtype;
   bool x_f32;  // x FP32 beside a 16-bit dtype
@@ -44,6 +45,8 @@ struct GateBackwardParams {
   int tokens, experts, top_k;
 };
 
+// 32-bit numbers of workspace that sort_tokens needs.
+std::size_t sort_tokens_counts(int64_t routes, int experts);
 hipError_t sort_tokens(const SortParams& prm, hipStream_t stream);
 hipError_t combine_tokens(const CombineParams& prm, hipStream_t stream);
 hipError_t combine_tokens_backward(const CombineParams& prm, hipStream_t stream);

@@ -124,6 +124,21 @@ def test_workspaces():
         assert getattr(rr.lib, f"rr_{name}_workspace_size")(None) == 0, name
 
 
+def test_workspace_of_many_routes():
+    """The counts of 32 parts of the routes, for up to 256 experts."""
+    def args(**change):
+        return rr.SortTokensArgs(**(ENTRIES["sort_tokens"][1] | change))
+
+    for tokens, top_k, experts, need in ((4096, 2, 256, 0), (8193, 1, 256, 32 * 256 * 4), (2 ** 30, 1, 9, 32 * 9 * 4),
+                                         (2 ** 30, 1, 257, 0), (2 ** 30, 2, 9, 0), (-1, 2, 9, 0)):
+        assert rr.get_sort_tokens_workspace_size(args(tokens=tokens, top_k=top_k, experts=experts)) == need
+    many = dict(tokens=8193, top_k=1, experts=9)
+    size = 32 * 9 * 4
+    assert refusal("sort_tokens", **many) == S.kInsufficientWorkspace
+    assert refusal("sort_tokens", ctx(workspace=P, workspace_bytes=size - 1), **many) == S.kInsufficientWorkspace
+    assert refusal("sort_tokens", ctx(workspace=P + 4, workspace_bytes=size), **many) == S.kInvalidArgument
+
+
 def test_nothing_to_do():
     for name, change in (("sort_tokens_backward", dict(tokens=0)), ("combine_tokens", dict(tokens=0)),
                          ("combine_tokens_backward", dict(tokens=0)),
