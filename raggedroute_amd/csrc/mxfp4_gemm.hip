@@ -25,6 +25,7 @@
 #include <type_traits>
 
 #include "expert_gemm.h"
+#include "large_lds.h"
 #include "launchers.h"
 #include "mxfp4.h"
 #include "mxfp4_rows.h"
@@ -411,18 +412,9 @@ __global__ __launch_bounds__(kThreads, 2) void rr_mxfp4_gemm_kernel(Product prm)
 
 template <class P>
 hipError_t launch(const Product& prm, hipStream_t stream) {
-  // (once a device; a second thread's call in between sets the same again)
   static std::atomic<uint64_t> allowed{0};
-  int device = 0;
-  hipError_t error = hipGetDevice(&device);
+  const hipError_t error = allow_lds(reinterpret_cast<const void*>(rr_mxfp4_gemm_kernel<P>), 160 * 1024, &allowed);
   if (error != hipSuccess) return error;
-  const uint64_t bit = uint64_t{1} << (device & 63);
-  if ((allowed.load(std::memory_order_relaxed) & bit) == 0 || device > 63) {
-    error = hipFuncSetAttribute(reinterpret_cast<const void*>(rr_mxfp4_gemm_kernel<P>),
-                                hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-    if (error != hipSuccess) return error;
-    allowed.fetch_or(bit, std::memory_order_relaxed);
-  }
   const long cols = (prm.N + P::kCols - 1) / P::kCols;
   const long rows = prm.rows / 64 + std::min<long>(prm.experts, prm.rows);
   long grid = std::min<long>(cols * rows, device_cu_count());

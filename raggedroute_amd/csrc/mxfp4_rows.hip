@@ -1,21 +1,26 @@
 // 4-bit products for few rows an expert (decoding): the weights are read once from memory,
-// straight into registers in matrix-operand order.
+// a line at a time.
 //
-// A workgroup of W waves takes 64 columns (of each right operand) of one expert and 16 of its
-// rows; the waves share the blocks of a row and add up through LDS in a fixed order. A step is
-// a slice of 256 elements: 128 bytes of every row and eight scales. Lane group g multiplies
-// blocks g and 4 + g of it (the two loads of a row's 128 bytes follow each other); its scales
-// are the bytes g of the row's two words. What bounds it is memory.
+// A workgroup of W waves takes 64 weight rows (of one operand, or 32 of each of two) of one
+// expert and 16 of its rows; the waves share the blocks of a row and add up through LDS in a
+// fixed order. A step is a slice of 256 elements: 128 bytes of every row, which eight lanes
+// bring as one line straight into the wave's own part of LDS, and eight scales. It is read
+// from there in operand order, and the next slice is on its way before it is multiplied. What bounds it is memory: two rows
+// of two experts, K = 4096, N = 14336, gated: 125 MB in 22.7 us (5.5 TB/s; lanes that load their
+// operands themselves, 64 bytes of a row at a time, 28 us; cached 25.7).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
 #include <type_traits>
 
+#include "large_lds.h"
 #include "mxfp4.h"
 #include "mxfp4_rows.h"
 #include "row_groups.h"
+#include "tile_stream.h"
 #include "wave.h"
 
 namespace rr::kern {
@@ -24,27 +29,33 @@ namespace {
 using rr::dev::bf16;
 using rr::dev::f16;
 
-typedef int i2 __attribute__((ext_vector_type(2)));
-typedef int i4 __attribute__((ext_vector_type(4)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 
-constexpr int kBufferFlags = 0x00027000;  // raw 32-bit buffer
-constexpr uint32_t kPast = 0x80000000U;   // an offset past every record count
-constexpr int kSliceBytes = 128;  // of every row
+// Weights that are larger than the caches keep from one call to the next are loaded past them.
+constexpr std::size_t kStreamedBytes = std::size_t{64} << 20;
+constexpr int kWeightRows = 64;  // of a workgroup
+constexpr int kScaleBytes = 8;   // of a row's slice
+// A wave's part of LDS: weights, rows, their scales.
+constexpr int kRows = kWeightRows * kSliceBytes;
+constexpr int kWeightScales = kRows + 16 * kSliceBytes;
+constexpr int kRowScales = kWeightScales + kWeightRows * kScaleBytes;
+constexpr int kWaveBytes = kRowScales + 16 * kScaleBytes;
 
+// HALF: which of the scales' two low bytes counts.
+template <int HALF>
 __device__ __forceinline__ f4 multiply(i4 a, i4 b, f4 c, int a_scale, int b_scale) {
   typedef int i8 __attribute__((ext_vector_type(8)));
   const i8 a8 = {a[0], a[1], a[2], a[3], 0, 0, 0, 0}, b8 = {b[0], b[1], b[2], b[3], 0, 0, 0, 0};
   constexpr int kE2M1 = 4;
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a8, b8, c, kE2M1, kE2M1, 0, a_scale, 0, b_scale);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a8, b8, c, kE2M1, kE2M1, HALF, a_scale, HALF, b_scale);
 }
 
-// W waves, F fragments of 16 columns of each right operand, D slices on their way
-template <class Epi, int W, int F, int D>
-__global__ __launch_bounds__(64 * W, 2) void rr_mxfp4_rows_kernel(Product prm, int blocks) {
+template <class Epi, int W, bool STREAMED>
+__global__ __launch_bounds__(64 * W, 3) void rr_mxfp4_rows_kernel(Product prm, int blocks) {
   constexpr int B = Epi::kDual ? 2 : 1;
+  constexpr int F = kWeightRows / 16 / B;  // fragments of 16 columns of each right operand
   constexpr int kCols = 16 * F;
-  __shared__ __align__(16) f4 s_sums[W > 1 ? W / 2 : 1][B * F][64];
+  extern __shared__ __align__(128) char smem[];  // [W][kWaveBytes]
   const int lane = static_cast<int>(threadIdx.x) & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int li = lane & 15, g = lane >> 4;
@@ -53,7 +64,8 @@ __global__ __launch_bounds__(64 * W, 2) void rr_mxfp4_rows_kernel(Product prm, i
   const int e = find_group(prm, static_cast<int>(blockIdx.x / static_cast<unsigned>(blocks)), &first, &count);
   if (e < 0) return;
   const int n0 = block * kCols;
-  const int N = prm.N, row_bytes = prm.lda;
+  const int N = prm.N;
+  const int64_t row_bytes = prm.lda;
   // this wave's slices
   const int slices = (prm.K + 7) / 8;
   const int s0 = static_cast<int>(static_cast<int64_t>(slices) * wave / W);
@@ -61,84 +73,85 @@ __global__ __launch_bounds__(64 * W, 2) void rr_mxfp4_rows_kernel(Product prm, i
 
   const int columns = min(N - n0, kCols);
   const int64_t channel = static_cast<int64_t>(e) * N + n0;
-  const int64_t x_slice = static_cast<int64_t>(prm.rows) * 8, w_slice = static_cast<int64_t>(prm.experts) * N * 8;
-  auto buffer_of = [](const void* base, int64_t at, int bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(base) + at), 0, bytes, kBufferFlags);
-  };
-  // rows past the last and columns past N repeat the last one: their results are not stored
-  const uint32_t x_lane = static_cast<uint32_t>(min(li, count - 1)) * row_bytes + 16 * g;
-  const uint32_t xs_lane = static_cast<uint32_t>(min(li, count - 1)) * 8;
-  uint32_t w_lane[F], ws_lane[F];
-#pragma unroll
-  for (int j = 0; j < F; ++j) {
-    const uint32_t c = min(16 * j + li, columns - 1);
-    w_lane[j] = c * row_bytes + 16 * g;
-    ws_lane[j] = c * 8;
-  }
-  // What a slice multiplies. Of a slice past the wave's last nothing is read (zeros).
-  struct Slice {
-    i4 x[2], w[B][F][2];
-    i2 x_scale, w_scale[B][F];
-  };
-  auto load = [&](Slice& o, int s) {
-    const bool on = s < s1;
-    const int left = prm.K - 8 * s;  // blocks of a row from the slice on
+  const int64_t x_slice = static_cast<int64_t>(prm.rows) * kScaleBytes, w_slice = static_cast<int64_t>(prm.experts) * N * kScaleBytes;
+  // Rows past the last and columns past N are past the buffers' records: zeros. (What lies past
+  // a row's end in its last slice is the next row's: its scales count as 2^-127.)
+  const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((RR_LDS char*)smem)) + wave * kWaveBytes;
+  const uint32_t at_lane = static_cast<uint32_t>((lane >> 3) * prm.lda) + (static_cast<uint32_t>((lane & 7) ^ (lane >> 3)) << 4);
+  auto load = [&](int s) {
+    const int64_t from = static_cast<int64_t>(s) * kSliceBytes;
 #pragma unroll
     for (int b = 0; b < B; ++b) {
-      const auto w = buffer_of(b == 0 ? prm.b : prm.b_up, channel * row_bytes, on ? columns * row_bytes : 0);
+      const char* w = static_cast<const char*>(b == 0 ? prm.b : prm.b_up) + channel * row_bytes + from;
+      const int64_t left = columns * row_bytes - from;
 #pragma unroll
-      for (int j = 0; j < F; ++j) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          o.w[b][j][h] = __builtin_bit_cast(i4, __builtin_amdgcn_raw_buffer_load_b128(w, w_lane[j] + 64 * h + s * kSliceBytes, 0, 0));
+      for (int q = 0; q < 2 * F; ++q) {
+        const i4 buffer = make_buffer(w + 8 * q * row_bytes, left - 8 * q * row_bytes);
+        const uint32_t to = lds + (b * 2 * F + q) * 1024;
+        if constexpr (STREAMED) {
+          stream_to_lds(buffer, at_lane, to);
+        } else {
+          load_to_lds(buffer, at_lane, to);
         }
       }
     }
-    const auto x = buffer_of(prm.a, static_cast<int64_t>(first) * row_bytes, on ? count * row_bytes : 0);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      // (blocks past the last are zeros: what the weights have there, the next channel's, does not count)
-      const uint32_t at = 4 * h + g < left ? x_lane + 64 * h + s * kSliceBytes : kPast;
-      o.x[h] = __builtin_bit_cast(i4, __builtin_amdgcn_raw_buffer_load_b128(x, at, 0, 0));
+    for (int q = 0; q < 2; ++q) {
+      const int64_t skip = (first + 8 * q) * row_bytes + from;
+      load_to_lds(make_buffer(static_cast<const char*>(prm.a) + skip, (count - 8 * q) * row_bytes - from), at_lane, lds + kRows + q * 1024);
     }
-    const auto xs = buffer_of(prm.a2, static_cast<int64_t>(first) * 8 + s * x_slice, on ? count * 8 : 0);
-    o.x_scale = __builtin_bit_cast(i2, __builtin_amdgcn_raw_buffer_load_b64(xs, xs_lane, 0, 0));
 #pragma unroll
     for (int b = 0; b < B; ++b) {
-      const auto ws = buffer_of(b == 0 ? prm.in : prm.in_up, channel * 8 + s * w_slice, on ? columns * 8 : 0);
+      const char* scales = static_cast<const char*>(b == 0 ? prm.in : prm.in_up) + channel * kScaleBytes + s * w_slice;
 #pragma unroll
-      for (int j = 0; j < F; ++j) o.w_scale[b][j] = __builtin_bit_cast(i2, __builtin_amdgcn_raw_buffer_load_b64(ws, ws_lane[j], 0, 0));
+      for (int q = 0; q < F / 2; ++q) {
+        load_words_to_lds(make_buffer(scales + q * 256, columns * kScaleBytes - q * 256), lane * 4,
+                          lds + kWeightScales + (b * F / 2 + q) * 256);
+      }
+    }
+    if (lane < 32) {
+      load_words_to_lds(make_buffer(static_cast<const char*>(prm.a2) + first * static_cast<int64_t>(kScaleBytes) + s * x_slice, count * kScaleBytes),
+                        lane * 4, lds + kRowScales);
     }
   };
+  // block 2 g + h of a row's slice
+  uint32_t at_row[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) at_row[h] = lds + li * kSliceBytes + (static_cast<uint32_t>((2 * g + h) ^ (li & 7)) << 4);
+  const uint32_t at_scale = lds + li * kScaleBytes + 2 * g;
+  auto read_scales = [&](uint32_t at) { return static_cast<int>(*reinterpret_cast<RR_LDS const uint16_t*>(at)); };
+
   f4 acc[B][F] = {};
-  auto multiply_slice = [&](const Slice& o, int s) {
-    const int left = prm.K - 8 * s;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const bool is = 4 * h + g < left;  // (scales past the last block are not looked at)
-      const int x_scale = is ? (o.x_scale[h] >> (8 * g)) & 255 : 0;
-#pragma unroll
-      for (int b = 0; b < B; ++b) {
-#pragma unroll
-        for (int j = 0; j < F; ++j) {
-          acc[b][j] = multiply(o.w[b][j][h], o.x[h], acc[b][j], is ? (o.w_scale[b][j][h] >> (8 * g)) & 255 : 0, x_scale);
-        }
-      }
-    }
-  };
-  Slice set[D];
-#pragma unroll
-  for (int d = 0; d < D; ++d) load(set[d], s0 + d);
+  if (s0 < s1) load(s0);
 #pragma unroll 1
-  for (int s = s0; s < s1; s += D) {
+  for (int s = s0; s < s1; ++s) {
+    wait_loads<0>();
+    i4 w[B * F][2], x[2];
+    int w_scale[B * F];
+    const int left = prm.K - 8 * s - 2 * g;  // blocks of a row from the lane's on; scales past them are not looked at
+    const int mask = left >= 2 ? 0xFFFF : left == 1 ? 0xFF : 0;
 #pragma unroll
-    for (int d = 0; d < D; ++d) {
-      __builtin_amdgcn_sched_barrier(0);  // (loads hoisted over the products would need registers of their own)
-      multiply_slice(set[d], s + d);
-      __builtin_amdgcn_sched_barrier(0);
-      load(set[d], s + d + D);
+    for (int j = 0; j < B * F; ++j) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) w[j][h] = read16(at_row[h] + j * 16 * kSliceBytes);
+      w_scale[j] = read_scales(at_scale + kWeightScales + j * 16 * kScaleBytes);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) x[h] = read16(at_row[h] + kRows);
+    const int x_scale = read_scales(at_scale + kRowScales) & mask;
+    wait_lds();
+    if (s + 1 < s1) load(s + 1);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < B * F; ++j) {
+      acc[j / F][j % F] = multiply<0>(w[j][0], x[0], acc[j / F][j % F], w_scale[j] & mask, x_scale);
+      acc[j / F][j % F] = multiply<1>(w[j][1], x[1], acc[j / F][j % F], w_scale[j] & mask, x_scale);
     }
   }
+  // (the parts of LDS become the sums')
+  f4(*s_sums)[B * F][64] = reinterpret_cast<f4(*)[B * F][64]>(smem);
+  static_assert(W / 2 * B * F * 64 * sizeof(f4) <= W * kWaveBytes);
+  __syncthreads();
 
   // the waves' sums, halved round by round
 #pragma unroll
@@ -175,21 +188,45 @@ __global__ __launch_bounds__(64 * W, 2) void rr_mxfp4_rows_kernel(Product prm, i
   }
 }
 
-template <class Epi, int W, int F, int D>
+template <class Epi, int W, bool STREAMED>
 hipError_t launch(const Product& prm, hipStream_t stream) {
-  const int blocks = (prm.N + 16 * F - 1) / (16 * F);
+  constexpr int kLds = W * kWaveBytes;
+  if constexpr (kLds > 64 * 1024) {
+    static std::atomic<uint64_t> allowed{0};
+    const hipError_t error = allow_lds(reinterpret_cast<const void*>(rr_mxfp4_rows_kernel<Epi, W, STREAMED>), kLds, &allowed);
+    if (error != hipSuccess) return error;
+  }
+  constexpr int kCols = kWeightRows / (Epi::kDual ? 2 : 1);
+  const int blocks = (prm.N + kCols - 1) / kCols;
   const std::size_t grid = most_groups(prm.rows, prm.experts) * blocks;
-  rr_mxfp4_rows_kernel<Epi, W, F, D><<<dim3(static_cast<unsigned>(grid)), 64 * W, 0, stream>>>(prm, blocks);
+  rr_mxfp4_rows_kernel<Epi, W, STREAMED><<<dim3(static_cast<unsigned>(grid)), 64 * W, kLds, stream>>>(prm, blocks);
   return hipGetLastError();
+}
+
+// Few waves that have many slices each, but enough of them in all (two rows, two experts: K =
+// 4096, N = 14336, gated, two waves 23 us, four 24, eight 29; K = 14336, N = 4096 34, 22 and 16).
+template <class Epi, bool STREAMED>
+hipError_t launch_waves(const Product& prm, hipStream_t stream) {
+  const int slices = (prm.K + 7) / 8;
+  constexpr int kCols = kWeightRows / (Epi::kDual ? 2 : 1);
+  const std::size_t workgroups = static_cast<std::size_t>(std::min(prm.experts, prm.rows)) * ((prm.N + kCols - 1) / kCols);
+  if (slices >= 16 && workgroups < 384) return launch<Epi, 8, STREAMED>(prm, stream);
+  if (slices >= 8 && workgroups < 768) return launch<Epi, 4, STREAMED>(prm, stream);
+  return launch<Epi, 2, STREAMED>(prm, stream);
 }
 
 }  // namespace
 
-bool mxfp4_rows_ok(int rows, int experts) { return rows <= 16 || rows <= 3 * std::min(rows, experts); }
+// Twelve rows an expert on average: a tile multiplies 64 rows for every few but reads an expert's
+// weights once, here every 16 rows read them again (E = 128, K = 2048, N = 768, gated: 8 rows
+// an expert 38 us, on tiles 45; 12: 40 and 45; 16: 44 and 46. E = 8, K = 4096, N = 14336: 8 rows 39
+// and 49, 12: 46 and 49, 16: 52 and 50).
+bool mxfp4_rows_ok(int rows, int experts) { return rows <= 16 || rows <= 12L * std::min(rows, experts); }
 
 template <class Epi>
 hipError_t mxfp4_rows(const Product& prm, hipStream_t stream) {
-  return launch<Epi, 4, 4, 1>(prm, stream);
+  const std::size_t bytes = static_cast<std::size_t>(std::min(prm.experts, prm.rows)) * prm.N * prm.lda * (Epi::kDual ? 2 : 1);
+  return bytes > kStreamedBytes ? launch_waves<Epi, true>(prm, stream) : launch_waves<Epi, false>(prm, stream);
 }
 
 template hipError_t mxfp4_rows<EpiStore<float>>(const Product&, hipStream_t);

@@ -52,6 +52,13 @@ __device__ __forceinline__ void load_to_lds(i4 buffer, uint32_t offset, uint32_t
                : "memory", "m0");
 }
 
+// The same past the caches.
+__device__ __forceinline__ void stream_to_lds(i4 buffer, uint32_t offset, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds" ::"s"(
+                   __builtin_amdgcn_readfirstlane(static_cast<int>(to))),
+               "v"(offset), "s"(buffer)
+               : "memory", "m0");
+}
 // The same of 64 lanes x 4 bytes.
 __device__ __forceinline__ void load_words_to_lds(i4 buffer, uint32_t offset, uint32_t to) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(
