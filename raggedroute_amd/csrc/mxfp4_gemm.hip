@@ -16,6 +16,12 @@
 //    that a lane ends with 16 adjacent columns of a row.
 //  - Scales of blocks past the row's last, whatever their bytes are, are replaced by 0 on both
 //    sides: the elements there, the next row's, then add 2^-254 times 36 at most, nothing.
+//
+// What bounds it: large products the power that the instructions draw, LDS, which is read and
+// written as long as they run (264 KB a slice), and the slices' loads (16384 rows of eight experts, K =
+// 4096, N = 14336: 560 us = 3.4 PFLOP/s; without its loads 438, without its LDS reads, too, 379, of
+// which the stores of 470 MB are 70); small ones the prologue and the epilogue of one or two
+// tiles a CU (6002 rows of nine experts, K = 1023, N = 1535, gated: 33 us, at K = 64 21).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -431,7 +437,10 @@ hipError_t product(const Product& prm, hipStream_t stream) {
   constexpr int kMost = (160 * 1024 - MxKind<Epi, 128>::kStages * MxKind<Epi, 128>::kStageBytes) / (3 * static_cast<int>(sizeof(int32_t))) - 1;
   static_assert(kMost >= 512);
   static_assert(MxKind<Epi, 256>::kStages * MxKind<Epi, 256>::kStageBytes + 3 * (RR_MAX_EXPERTS + 1) * sizeof(int32_t) <= 160 * 1024);
-  const bool few = prm.rows <= 96L * prm.experts && prm.experts <= kMost;
+  // Tiles of 128 rows where an expert has 128 rows or fewer on average (E = 128, K = 2048, N = 768,
+  // gated: 16384 rows 75 us, on tiles of 256 rows 82; E = 8, K = N = 4096: 1024 rows 25.8 and 27.8, but N
+  // = 14336 82 and 78; 2048 rows of those 117 and 108).
+  const bool few = prm.rows <= 128L * prm.experts && prm.experts <= kMost;
   return few ? launch<MxKind<Epi, 128>>(prm, stream) : launch<MxKind<Epi, 256>>(prm, stream);
 }
 
@@ -453,7 +462,7 @@ hipError_t typed(const MxGemmParams& f, hipStream_t stream) {
   p.lda = p.ldb = 16 * p.K;
   if (f.w_up != nullptr) {
     p.out_act = f.y;
-    return product<EpiGate<T>>(p, stream);
+    return product<EpiMxGate<T>>(p, stream);
   }
   p.out = f.y;
   return product<EpiStore<T>>(p, stream);

@@ -232,8 +232,8 @@ hipError_t mxfp4_rows(const Product& prm, hipStream_t stream) {
 template hipError_t mxfp4_rows<EpiStore<float>>(const Product&, hipStream_t);
 template hipError_t mxfp4_rows<EpiStore<bf16>>(const Product&, hipStream_t);
 template hipError_t mxfp4_rows<EpiStore<f16>>(const Product&, hipStream_t);
-template hipError_t mxfp4_rows<EpiGate<float>>(const Product&, hipStream_t);
-template hipError_t mxfp4_rows<EpiGate<bf16>>(const Product&, hipStream_t);
-template hipError_t mxfp4_rows<EpiGate<f16>>(const Product&, hipStream_t);
+template hipError_t mxfp4_rows<EpiMxGate<float>>(const Product&, hipStream_t);
+template hipError_t mxfp4_rows<EpiMxGate<bf16>>(const Product&, hipStream_t);
+template hipError_t mxfp4_rows<EpiMxGate<f16>>(const Product&, hipStream_t);
 
 }  // namespace rr::kern
