@@ -465,7 +465,7 @@ hipError_t typed(const MxGemmParams& f, hipStream_t stream) {
     return product<EpiMxGate<T>>(p, stream);
   }
   p.out = f.y;
-  return product<EpiStore<T>>(p, stream);
+  return product<EpiMxStore<T>>(p, stream);
 }
 
 }  // namespace

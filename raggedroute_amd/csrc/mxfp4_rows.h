@@ -7,6 +7,36 @@
 
 namespace rr::kern {
 
+// V columns of a row of 16-bit results. Rows of an odd width start on a word boundary and off it
+// by turns; off it the first and the last column are stored by themselves, so that the others are
+// whole words.
+template <typename T, int V>
+__device__ __forceinline__ void store_columns(T* p, const float (&v)[V], int left) {
+  if constexpr (sizeof(T) == 2) {
+    if (left >= V && (reinterpret_cast<uintptr_t>(p) & 2) != 0) {
+      typedef T inner __attribute__((ext_vector_type(V - 2), aligned(4)));
+      inner o;
+#pragma unroll
+      for (int i = 0; i < V - 2; ++i) o[i] = static_cast<T>(v[i + 1]);
+      p[0] = static_cast<T>(v[0]);
+      *reinterpret_cast<inner*>(p + 1) = o;
+      p[V - 1] = static_cast<T>(v[V - 1]);
+      return;
+    }
+  }
+  Cols<T, V>::store(p, v, left);
+}
+
+// out = sums
+template <typename T>
+struct EpiMxStore {
+  static constexpr bool kDual = false;
+  template <int V>
+  static __device__ __forceinline__ void emit(const Product& p, int, std::size_t row, int n, int left, const float (&v)[V]) {
+    store_columns<T, V>(static_cast<T*>(p.out) + row * p.N + n, v, left);
+  }
+};
+
 // out_act = act(g) u. A tile's 64 results a lane cost as much as a few slices of products, so
 // that the kind is chosen once for all columns and the exponent is one polynomial: act(g) = g
 // / (1 + 2^-z), z = log2(e) g for SiLU and log2(e) g (kGelu + kGelu kGeluCube g^2) for the tanh form
@@ -30,7 +60,7 @@ struct EpiMxGate {
     } else {
       apply([](float v) { return v * __builtin_fmaf(-kLog2e * rr::dev::kGelu * rr::dev::kGeluCube, v * v, -kLog2e * rr::dev::kGelu); });
     }
-    Cols<T, V>::store(static_cast<T*>(p.out_act) + row * p.N + n, a, left);
+    store_columns<T, V>(static_cast<T*>(p.out_act) + row * p.N + n, a, left);
   }
 };
 

@@ -229,9 +229,9 @@ hipError_t mxfp4_rows(const Product& prm, hipStream_t stream) {
   return bytes > kStreamedBytes ? launch_waves<Epi, true>(prm, stream) : launch_waves<Epi, false>(prm, stream);
 }
 
-template hipError_t mxfp4_rows<EpiStore<float>>(const Product&, hipStream_t);
-template hipError_t mxfp4_rows<EpiStore<bf16>>(const Product&, hipStream_t);
-template hipError_t mxfp4_rows<EpiStore<f16>>(const Product&, hipStream_t);
+template hipError_t mxfp4_rows<EpiMxStore<float>>(const Product&, hipStream_t);
+template hipError_t mxfp4_rows<EpiMxStore<bf16>>(const Product&, hipStream_t);
+template hipError_t mxfp4_rows<EpiMxStore<f16>>(const Product&, hipStream_t);
 template hipError_t mxfp4_rows<EpiMxGate<float>>(const Product&, hipStream_t);
 template hipError_t mxfp4_rows<EpiMxGate<bf16>>(const Product&, hipStream_t);
 template hipError_t mxfp4_rows<EpiMxGate<f16>>(const Product&, hipStream_t);
