@@ -432,7 +432,7 @@ hipError_t launch(const Product& prm, hipStream_t stream) {
 
 template <class Epi>
 hipError_t product(const Product& prm, hipStream_t stream) {
-  if (mxfp4_rows_ok(prm.rows, prm.experts)) return mxfp4_rows<Epi>(prm, stream);
+  if (mxfp4_rows_ok(prm, Epi::kDual)) return mxfp4_rows<Epi>(prm, stream);
   // (the LDS that three stages leave holds the bounds of 596 experts)
   constexpr int kMost = (160 * 1024 - MxKind<Epi, 128>::kStages * MxKind<Epi, 128>::kStageBytes) / (3 * static_cast<int>(sizeof(int32_t))) - 1;
   static_assert(kMost >= 512);

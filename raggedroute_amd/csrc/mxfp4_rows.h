@@ -64,9 +64,9 @@ struct EpiMxGate {
   }
 };
 
-// Whether the kernel for few rows takes a product of this many rows.
-bool mxfp4_rows_ok(int rows, int experts);
-// prm as rr_mxfp4_gemm_kernel's.
+// Whether the kernel for few rows takes a product (dual: with two right operands). prm as
+// rr_mxfp4_gemm_kernel's.
+bool mxfp4_rows_ok(const Product& prm, bool dual);
 template <class Epi>
 hipError_t mxfp4_rows(const Product& prm, hipStream_t stream);
 

@@ -188,6 +188,12 @@ __global__ __launch_bounds__(64 * W, 3) void rr_mxfp4_rows_kernel(Product prm, i
   }
 }
 
+// Workgroups that share an expert's columns.
+std::size_t blocks_of(int columns, bool dual) {
+  const int of_one = kWeightRows / (dual ? 2 : 1);
+  return static_cast<std::size_t>((columns + of_one - 1) / of_one);
+}
+
 template <class Epi, int W, bool STREAMED>
 hipError_t launch(const Product& prm, hipStream_t stream) {
   constexpr int kLds = W * kWaveBytes;
@@ -196,23 +202,23 @@ hipError_t launch(const Product& prm, hipStream_t stream) {
     const hipError_t error = allow_lds(reinterpret_cast<const void*>(rr_mxfp4_rows_kernel<Epi, W, STREAMED>), kLds, &allowed);
     if (error != hipSuccess) return error;
   }
-  constexpr int kCols = kWeightRows / (Epi::kDual ? 2 : 1);
-  const int blocks = (prm.N + kCols - 1) / kCols;
+  const std::size_t blocks = blocks_of(prm.N, Epi::kDual);
   const std::size_t grid = most_groups(prm.rows, prm.experts) * blocks;
-  rr_mxfp4_rows_kernel<Epi, W, STREAMED><<<dim3(static_cast<unsigned>(grid)), 64 * W, kLds, stream>>>(prm, blocks);
+  rr_mxfp4_rows_kernel<Epi, W, STREAMED><<<dim3(static_cast<unsigned>(grid)), 64 * W, kLds, stream>>>(prm, static_cast<int>(blocks));
   return hipGetLastError();
 }
 
 // Few waves that have many slices each, but enough of them in all (two rows, two experts: K =
-// 4096, N = 14336, gated, two waves 23 us, four 24, eight 29; K = 14336, N = 4096 34, 22 and 16).
+// 4096, N = 14336, gated, two waves 23 us, four 24, eight 29; K = 14336, N = 4096 34, 22 and 16). One
+// where a row is one slice (1302 rows of 166 experts, K = 64, N = 5280: 36 -> 20 us).
 template <class Epi, bool STREAMED>
 hipError_t launch_waves(const Product& prm, hipStream_t stream) {
   const int slices = (prm.K + 7) / 8;
-  constexpr int kCols = kWeightRows / (Epi::kDual ? 2 : 1);
-  const std::size_t workgroups = static_cast<std::size_t>(std::min(prm.experts, prm.rows)) * ((prm.N + kCols - 1) / kCols);
+  const std::size_t workgroups = most_groups(prm.rows, prm.experts) * blocks_of(prm.N, Epi::kDual);
   if (slices >= 16 && workgroups < 384) return launch<Epi, 8, STREAMED>(prm, stream);
   if (slices >= 8 && workgroups < 768) return launch<Epi, 4, STREAMED>(prm, stream);
-  return launch<Epi, 2, STREAMED>(prm, stream);
+  if (slices >= 2) return launch<Epi, 2, STREAMED>(prm, stream);
+  return launch<Epi, 1, STREAMED>(prm, stream);
 }
 
 }  // namespace
@@ -220,8 +226,14 @@ hipError_t launch_waves(const Product& prm, hipStream_t stream) {
 // Twelve rows an expert on average: a tile multiplies 64 rows for every few but reads an expert's
 // weights once, here every 16 rows read them again (E = 128, K = 2048, N = 768, gated: 8 rows
 // an expert 38 us, on tiles 45; 12: 40 and 45; 16: 44 and 46. E = 8, K = 4096, N = 14336: 8 rows 39
-// and 49, 12: 46 and 49, 16: 52 and 50).
-bool mxfp4_rows_ok(int rows, int experts) { return rows <= 16 || rows <= 12L * std::min(rows, experts); }
+// and 49, 12: 46 and 49, 16: 52 and 50). And with more where there are few tiles, whose slices
+// follow each other while most of the card is idle: K = N = 4096, one expert, 128 rows (512
+// workgroups here) 12 us, on tiles 19; 256 rows 23 and 21; K = 1024, N = 1024, eight experts, 1024 rows
+// (1024 workgroups of few slices) 7.7 and 10; K = 2784, N = 672, one expert, 256 rows 7 and 18.
+bool mxfp4_rows_ok(const Product& prm, bool dual) {
+  if (prm.rows <= 16 || prm.rows <= 12L * std::min(prm.rows, prm.experts)) return true;
+  return most_groups(prm.rows, prm.experts) * blocks_of(prm.N, dual) <= 640;
+}
 
 template <class Epi>
 hipError_t mxfp4_rows(const Product& prm, hipStream_t stream) {

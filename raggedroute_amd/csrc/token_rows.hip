@@ -88,8 +88,9 @@ constexpr int kBatch = 8;  // routes of a token whose positions are loaded toget
 // Every route's position and the offsets, for few routes: every workgroup reads all ids. The
 // first `tokens * chunks` workgroups rank the routes of a token (a wave for each in turn, 64
 // ids at a time by ballots) and copy a chunk of its row; the others count the ids below every
-// expert.
-constexpr int kFewRoutes = 1024;
+// expert. (Rows of 2048 BF16 numbers of 128 experts, top-8: 64 routes 3.4 us, by the kernel for more
+// routes 4.7; 256 routes 5.2 and 4.7, 1024 17 and 4.9.)
+constexpr int kFewRoutes = 128;
 
 template <typename TX, typename T, bool ROWS>
 __global__ __launch_bounds__(kThreads) void rr_sort_few_kernel(SortParams p, int chunks) {
@@ -453,7 +454,8 @@ __device__ __forceinline__ int checked(int32_t pos, int64_t routes) {
   return pos >= 0 && pos < routes ? pos : -1;
 }
 
-// G threads a token: its row read once and stored at the positions of its routes.
+// G threads a token (and as many more as blockIdx.y counts, for wide rows of few tokens): its row
+// read once and stored at the positions of its routes.
 template <typename TX, typename T, int G, int MODE>
 __global__ __launch_bounds__(kThreads) void rr_sort_rows_kernel(SortParams p) {
   constexpr int V = kPiece<T>;
@@ -470,7 +472,7 @@ __global__ __launch_bounds__(kThreads) void rr_sort_rows_kernel(SortParams p) {
       for (int j = 0; j < kBatch; ++j) {
         pos[j] = j0 + j < p.top_k ? checked(p.route_pos[t * p.top_k + j0 + j], routes) : -1;
       }
-      for (int c = lane * V; c < p.hidden; c += G * V) {
+      for (int c = (static_cast<int>(blockIdx.y) * G + lane) * V; c < p.hidden; c += static_cast<int>(gridDim.y) * G * V) {
         Piece<TX, V> piece;
         piece.template load<MODE>(x + t * H + c, p.hidden - c);
         const Piece<T, V> o = converted<T>(piece);
@@ -494,7 +496,7 @@ __global__ __launch_bounds__(kThreads) void rr_combine_kernel(CombineParams p) {
   const std::size_t H = p.hidden;
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * (kThreads / G) + tid / G; t < p.tokens;
        t += static_cast<int64_t>(gridDim.x) * (kThreads / G)) {
-    for (int c = lane * V; c < p.hidden; c += G * V) {
+    for (int c = (static_cast<int>(blockIdx.y) * G + lane) * V; c < p.hidden; c += static_cast<int>(gridDim.y) * G * V) {
       float sum[V] = {};
       for (int j0 = 0; j0 < p.top_k; j0 += kBatch) {
         int pos[kBatch];
@@ -657,6 +659,15 @@ unsigned token_grid(int tokens, int per) {
   return static_cast<unsigned>(std::min<int64_t>((static_cast<int64_t>(tokens) + per - 1) / per, 16384));
 }
 
+// Workgroups that share a token's columns, for few tokens with wide rows (six tokens of 4864 FP32
+// numbers, top-8, combined: 8.3 us by one each, 4.4 by five).
+template <int G>
+dim3 token_grid(int tokens, int hidden, int piece) {
+  const unsigned x = token_grid(tokens, kThreads / G);
+  const int most = (hidden + G * piece - 1) / (G * piece);
+  return dim3(x, static_cast<unsigned>(std::max(1, std::min(most, static_cast<int>(1024 / x)))));
+}
+
 // Threads of a token: as many as its row has pieces, up to a workgroup's (a wave for a row of 256
 // pieces: combining 65536 rows of 2048 BF16 numbers 79 us against 59, its gradients 131 against
 // 115). BACKWARD: a wave up to 128 pieces, whose sums then meet at no barrier (gradients of 6002
@@ -688,7 +699,7 @@ hipError_t sort_rows(const SortParams& p, hipStream_t stream) {
   return with_group<false>(p.hidden, kPiece<T>, bytes, [&](auto g, auto mode) {
     constexpr int G = decltype(g)::value;
     constexpr int M = decltype(mode)::value;
-    rr_sort_rows_kernel<TX, T, G, M><<<token_grid(p.tokens, kThreads / G), kThreads, 0, stream>>>(p);
+    rr_sort_rows_kernel<TX, T, G, M><<<token_grid<G>(p.tokens, p.hidden, kPiece<T>), kThreads, 0, stream>>>(p);
     return hipGetLastError();
   });
 }
@@ -741,7 +752,7 @@ hipError_t combine_typed(const CombineParams& p, hipStream_t stream) {
   return with_group<false>(p.hidden, kPiece<T>, sizeof(TY) * p.tokens * p.hidden, [&](auto g, auto mode) {
     constexpr int G = decltype(g)::value;
     constexpr int M = decltype(mode)::value;
-    rr_combine_kernel<TY, T, G, M><<<token_grid(p.tokens, kThreads / G), kThreads, 0, stream>>>(p);
+    rr_combine_kernel<TY, T, G, M><<<token_grid<G>(p.tokens, p.hidden, kPiece<T>), kThreads, 0, stream>>>(p);
     return hipGetLastError();
   });
 }
