@@ -3,7 +3,9 @@
 // A lane takes eight elements, four lanes a block: the largest magnitude is found on the bits
 // (a NaN is above an infinity, an infinity above the rest), the scale's exponent is that of the
 // magnitude less 2, and the conversion divides by the scale, rounds to even and cuts at 6.
-// 16 lanes put four scales together to a word. What bounds it is HBM.
+// 16 lanes put four scales together to a word. What bounds it is memory: 16384 rows of 4096 BF16
+// numbers gathered from 8192 tokens 28 us, 134 MB read (half of it again, from the caches) and 36
+// written.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

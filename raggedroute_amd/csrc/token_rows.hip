@@ -6,8 +6,9 @@
 //   d sorted[pos[r]] = w[r] dy[t],  dw[r] = <dy[t], sorted[pos[r]]>
 //   dlogits[t, id_j] = w_j sum_i w_i (dw_j - dw_i)
 //
-// Nothing here is arithmetic to speak of: the rows are moved at the rate of HBM and the maps
-// take the latency of a launch or two.
+// Nothing here is arithmetic to speak of: the rows are moved at the rate of HBM (65536 rows of 2048
+// BF16 numbers: sorted in 59 us, 5.1 TB/s; combined in 55, 5.5; both gradients of that 102 to 114, 5.0
+// to 5.6; a plain copy 5.15) and the maps take the latency of a launch or two.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
