@@ -231,8 +231,9 @@ hipError_t launch_waves(const Product& prm, hipStream_t stream) {
 // workgroups here) 12 us, on tiles 19; 256 rows 23 and 21; K = 1024, N = 1024, eight experts, 1024 rows
 // (1024 workgroups of few slices) 7.7 and 10; K = 2784, N = 672, one expert, 256 rows 7 and 18.
 bool mxfp4_rows_ok(const Product& prm, bool dual) {
-  if (prm.rows <= 16 || prm.rows <= 12L * std::min(prm.rows, prm.experts)) return true;
-  return most_groups(prm.rows, prm.experts) * blocks_of(prm.N, dual) <= 640;
+  const std::size_t workgroups = most_groups(prm.rows, prm.experts) * blocks_of(prm.N, dual);
+  if (workgroups >= std::size_t{1} << 23) return false;  // (a launch has less than 2^32 threads)
+  return prm.rows <= 16 || prm.rows <= 12L * std::min(prm.rows, prm.experts) || workgroups <= 640;
 }
 
 template <class Epi>

@@ -709,8 +709,9 @@ template <typename TX, typename T>
 hipError_t sort_typed(const SortParams& p, hipStream_t stream) {
   const int64_t routes = static_cast<int64_t>(p.tokens) * p.top_k;
   if (routes > kFewRoutes && p.experts <= kCountedExperts) {
-    const int owned = static_cast<int>(std::min<int64_t>((p.tokens + kOwners - 1) / kOwners, kOwnedRoutes / p.top_k));
-    const unsigned grid = static_cast<unsigned>((p.tokens + owned - 1) / owned);
+    const int64_t tokens = p.tokens;
+    const int owned = static_cast<int>(std::min<int64_t>((tokens + kOwners - 1) / kOwners, kOwnedRoutes / p.top_k));
+    const unsigned grid = static_cast<unsigned>((tokens + owned - 1) / owned);
     const bool counted = routes > kCountedRoutes;
     if (counted) {
       const int64_t chunk = chunk_routes(routes);
