@@ -223,17 +223,22 @@ hipError_t launch_waves(const Product& prm, hipStream_t stream) {
 
 }  // namespace
 
-// Twelve rows an expert on average: a tile multiplies 64 rows for every few but reads an expert's
-// weights once, here every 16 rows read them again (E = 128, K = 2048, N = 768, gated: 8 rows
-// an expert 38 us, on tiles 45; 12: 40 and 45; 16: 44 and 46. E = 8, K = 4096, N = 14336: 8 rows 39
-// and 49, 12: 46 and 49, 16: 52 and 50). And with more where there are few tiles, whose slices
-// follow each other while most of the card is idle: K = N = 4096, one expert, 128 rows (512
-// workgroups here) 12 us, on tiles 19; 256 rows 23 and 21; K = 1024, N = 1024, eight experts, 1024 rows
-// (1024 workgroups of few slices) 7.7 and 10; K = 2784, N = 672, one expert, 256 rows 7 and 18.
+// Rows an expert on average: a tile multiplies 64 rows for every few but reads an expert's weights
+// once, here every 16 rows read them again. Long sums: twelve (16 slices, E = 8, N = 14336: 8 rows an
+// expert 39 us, on tiles 49; 12: 46 and 49; 16: 52 and 50), 16 for eight slices (E = 128, N = 768,
+// gated: 44 and 46). Of short ones a tile is mostly prologue and epilogue: 40 (four slices, E =
+// 64, N = 1024, gated: 32 rows 22 and 25, 48: 27 and 28, 64: 33 and 28; two, N = 2048: 32 rows 16 and 19, 48: 21
+// and 20; one, E = 167, N = 4816: 32 rows 48 and 52, 48: 62 and 57).
+// And with more where there are few tiles, whose slices follow each other while most of the
+// card is idle: K = N = 4096, one expert, 128 rows (512 workgroups here) 12 us, on tiles 19; 256 rows
+// 23 and 21; K = 1024, N = 1024, eight experts, 1024 rows (1024 workgroups of few slices) 7.7 and 10; K =
+// 2784, N = 672, one expert, 256 rows 7 and 18.
 bool mxfp4_rows_ok(const Product& prm, bool dual) {
   const std::size_t workgroups = most_groups(prm.rows, prm.experts) * blocks_of(prm.N, dual);
   if (workgroups >= std::size_t{1} << 23) return false;  // (a launch has less than 2^32 threads)
-  return prm.rows <= 16 || prm.rows <= 12L * std::min(prm.rows, prm.experts) || workgroups <= 640;
+  const int slices = (prm.K + 7) / 8;
+  const long rows = slices <= 4 ? 40 : slices <= 8 ? 16 : 12;
+  return prm.rows <= 16 || prm.rows <= rows * std::min(prm.rows, prm.experts) || workgroups <= 640;
 }
 
 template <class Epi>
