@@ -82,7 +82,12 @@ __device__ __forceinline__ Piece<T, V> converted(const Piece<TX, V>& x) {
 // Elements of a thread's piece: 16 bytes of the sorted rows' type.
 template <typename T>
 constexpr int kPiece = 16 / sizeof(T);
-constexpr int kBatch = 8;  // routes of a token whose positions are loaded together
+// Routes of a token whose positions, then rows are on their way together. Sums of up to four
+// routes are held for four only, and where a thread has several whole pieces of a row, for two of
+// them: BF16, top-2, the sum and its gradients, 8192 rows of 2048: 15.0, 38.9 us for eight ->
+// 13.9, 27.2 for four; 8192 of 4096: 35.3, 59.5 for eight, 33.1, 52.5 for four, 31.5, 51.9 for
+// four of two pieces. (Pieces of odd rows, 3001 of 4095: gradients 28.3 us by one, 32.1 by two.)
+constexpr int kBatch = 8, kFewTopK = 4;
 
 // ---- the routes' order ----
 
@@ -455,6 +460,25 @@ __device__ __forceinline__ int checked(int32_t pos, int64_t routes) {
   return pos >= 0 && pos < routes ? pos : -1;
 }
 
+// The positions and weights of B routes of a token from route j0 on. Every load is on its way
+// before one of them is looked at; past the last route it is loaded again and counts as none.
+template <int B>
+__device__ __forceinline__ void load_positions(const int32_t* of_token, int j0, int top_k, int64_t routes, int (&pos)[B]) {
+#pragma unroll
+  for (int j = 0; j < B; ++j) pos[j] = of_token[min(j0 + j, top_k - 1)];
+#pragma unroll
+  for (int j = 0; j < B; ++j) pos[j] = j0 + j < top_k ? checked(pos[j], routes) : -1;
+}
+
+template <int B>
+__device__ __forceinline__ void load_weights(const float* weights, int64_t r0, int j0, int top_k, float (&w)[B]) {
+#pragma unroll
+  for (int j = 0; j < B; ++j) w[j] = 1.0F;
+  if (weights == nullptr) return;
+#pragma unroll
+  for (int j = 0; j < B; ++j) w[j] = weights[r0 + min(j0 + j, top_k - 1)];
+}
+
 // G threads a token (and as many more as blockIdx.y counts, for wide rows of few tokens): its row
 // read once and stored at the positions of its routes.
 template <typename TX, typename T, int G, int MODE>
@@ -469,10 +493,7 @@ __global__ __launch_bounds__(kThreads) void rr_sort_rows_kernel(SortParams p) {
        t += static_cast<int64_t>(gridDim.x) * (kThreads / G)) {
     for (int j0 = 0; j0 < p.top_k; j0 += kBatch) {
       int pos[kBatch];
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        pos[j] = j0 + j < p.top_k ? checked(p.route_pos[t * p.top_k + j0 + j], routes) : -1;
-      }
+      load_positions(p.route_pos + t * p.top_k, j0, p.top_k, routes, pos);
       for (int c = (static_cast<int>(blockIdx.y) * G + lane) * V; c < p.hidden; c += static_cast<int>(gridDim.y) * G * V) {
         Piece<TX, V> piece;
         piece.template load<MODE>(x + t * H + c, p.hidden - c);
@@ -486,8 +507,9 @@ __global__ __launch_bounds__(kThreads) void rr_sort_rows_kernel(SortParams p) {
   }
 }
 
-// G threads a token: the sum of its routes' rows.
-template <typename TY, typename T, int G, int MODE>
+// G threads a token (and as many more as blockIdx.y counts, for wide rows of few tokens): the sum of
+// its routes' rows. B routes and C pieces of each are on their way together.
+template <typename TY, typename T, int G, int MODE, int B, int C>
 __global__ __launch_bounds__(kThreads) void rr_combine_kernel(CombineParams p) {
   constexpr int V = kPiece<T>;
   const int tid = static_cast<int>(threadIdx.x), lane = tid & (G - 1);
@@ -495,46 +517,59 @@ __global__ __launch_bounds__(kThreads) void rr_combine_kernel(CombineParams p) {
   const auto* rows = static_cast<const T*>(p.sorted);
   auto* out = static_cast<TY*>(p.out);
   const std::size_t H = p.hidden;
+  const int step = static_cast<int>(gridDim.y) * G * V;  // between a thread's pieces
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * (kThreads / G) + tid / G; t < p.tokens;
        t += static_cast<int64_t>(gridDim.x) * (kThreads / G)) {
-    for (int c = (static_cast<int>(blockIdx.y) * G + lane) * V; c < p.hidden; c += static_cast<int>(gridDim.y) * G * V) {
-      float sum[V] = {};
-      for (int j0 = 0; j0 < p.top_k; j0 += kBatch) {
-        int pos[kBatch];
-        float w[kBatch];
-        Piece<T, V> row[kBatch];
+    for (int c0 = (static_cast<int>(blockIdx.y) * G + lane) * V; c0 < p.hidden; c0 += C * step) {
+      float sum[C][V] = {};
+      for (int j0 = 0; j0 < p.top_k; j0 += B) {
+        int pos[B];
+        float w[B];
+        Piece<T, V> row[B][C];
+        load_positions(p.route_pos + t * p.top_k, j0, p.top_k, routes, pos);
+        load_weights(p.weights, t * p.top_k, j0, p.top_k, w);
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-          const int64_t r = t * p.top_k + j0 + j;
-          pos[j] = j0 + j < p.top_k ? checked(p.route_pos[r], routes) : -1;
-          w[j] = p.weights != nullptr && j0 + j < p.top_k ? p.weights[r] : 1.0F;
+        for (int j = 0; j < B; ++j) {
+#pragma unroll
+          for (int q = 0; q < C; ++q) {
+            const int c = c0 + q * step;
+            if (j0 + j < p.top_k && (q == 0 || c < p.hidden)) {
+              row[j][q].template load<MODE>(rows + max(pos[j], 0) * H + c, p.hidden - c);
+            }
+          }
         }
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-          if (j0 + j < p.top_k) row[j].template load<MODE>(rows + max(pos[j], 0) * H + c, p.hidden - c);
-        }
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
+        for (int j = 0; j < B; ++j) {
           if (j0 + j < p.top_k && pos[j] >= 0) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) sum[i] = __builtin_fmaf(w[j], static_cast<float>(row[j].v[i]), sum[i]);
+            for (int q = 0; q < C; ++q) {
+#pragma unroll
+              for (int i = 0; i < V; ++i) sum[q][i] = __builtin_fmaf(w[j], static_cast<float>(row[j][q].v[i]), sum[q][i]);
+            }
           }
         }
       }
-      Piece<TY, V> o;
+      // (no loop: out of a loop of one step the compiler moves the store and loses that it is nontemporal)
+      auto store = [&](int q, int c) {
+        Piece<TY, V> o;
 #pragma unroll
-      for (int i = 0; i < V; ++i) o.v[i] = static_cast<TY>(sum[i]);
-      o.template store<MODE>(out + t * H + c, p.hidden - c);
+        for (int i = 0; i < V; ++i) o.v[i] = static_cast<TY>(sum[q][i]);
+        o.template store<MODE>(out + t * H + c, p.hidden - c);
+      };
+      store(0, c0);
+      if constexpr (C == 2) {
+        if (c0 + step < p.hidden) store(1, c0 + step);
+      }
     }
   }
 }
 
-// G threads a token: the gradients of its routes' rows and weights. The columns' products are
-// added by lane, then over the lanes in a fixed order.
-template <typename TY, typename T, int G, int MODE>
+// G threads a token: the gradients of its routes' rows and weights, B routes and C pieces of each
+// together. The columns' products are added by lane, then over the lanes in a fixed order.
+template <typename TY, typename T, int G, int MODE, int B, int C>
 __global__ __launch_bounds__(kThreads) void rr_combine_backward_kernel(CombineParams p) {
   constexpr int V = kPiece<T>;
-  __shared__ float s_dot[2][kThreads / 64][kBatch];  // by turns
+  __shared__ float s_dot[2][kThreads / 64][B];  // by turns
   int turn = 0;
   const int tid = static_cast<int>(threadIdx.x), lane = tid & (G - 1);
   const int64_t routes = static_cast<int64_t>(p.tokens) * p.top_k;
@@ -547,58 +582,75 @@ __global__ __launch_bounds__(kThreads) void rr_combine_backward_kernel(CombinePa
   for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * (kThreads / G); t0 < p.tokens; t0 += step) {
     const int64_t t = t0 + tid / G;
     const bool here = t < p.tokens;
-    for (int j0 = 0; j0 < p.top_k; j0 += kBatch) {
-      int pos[kBatch];
-      float w[kBatch], dot[kBatch] = {};
+    for (int j0 = 0; j0 < p.top_k; j0 += B) {
+      int pos[B];
+      float w[B], dot[B] = {};
+      const int64_t r0 = (here ? t : 0) * p.top_k;
+      load_positions(p.route_pos + r0, j0, p.top_k, here ? routes : 0, pos);
+      load_weights(p.weights, r0, j0, p.top_k, w);
+      for (int c0 = lane * V; here && c0 < p.hidden; c0 += C * G * V) {
+        Piece<TY, V> g[C];
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        const int64_t r = t * p.top_k + j0 + j;
-        const bool is = here && j0 + j < p.top_k;
-        pos[j] = is ? checked(p.route_pos[r], routes) : -1;
-        w[j] = is && p.weights != nullptr ? p.weights[r] : 1.0F;
-      }
-      for (int c = lane * V; here && c < p.hidden; c += G * V) {
-        Piece<TY, V> g;
-        g.template load<MODE>(dy + t * H + c, p.hidden - c);
+        for (int q = 0; q < C; ++q) {
+          const int c = c0 + q * G * V;
+          if (q == 0 || c < p.hidden) g[q].template load<MODE>(dy + t * H + c, p.hidden - c);
+        }
         if (p.dweights != nullptr) {
-          Piece<T, V> row[kBatch];
+          Piece<T, V> row[B][C];
 #pragma unroll
-          for (int j = 0; j < kBatch; ++j) {
-            if (pos[j] >= 0) row[j].template load<MODE>(rows + pos[j] * H + c, p.hidden - c);
-          }
-#pragma unroll
-          for (int j = 0; j < kBatch; ++j) {
+          for (int j = 0; j < B; ++j) {
             if (pos[j] < 0) continue;
 #pragma unroll
-            for (int i = 0; i < V; ++i) dot[j] = __builtin_fmaf(static_cast<float>(g.v[i]), static_cast<float>(row[j].v[i]), dot[j]);
+            for (int q = 0; q < C; ++q) {
+              const int c = c0 + q * G * V;
+              if (q == 0 || c < p.hidden) row[j][q].template load<MODE>(rows + pos[j] * H + c, p.hidden - c);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < B; ++j) {
+            if (pos[j] < 0) continue;
+#pragma unroll
+            for (int q = 0; q < C; ++q) {
+              if (q > 0 && c0 + q * G * V >= p.hidden) continue;
+#pragma unroll
+              for (int i = 0; i < V; ++i) {
+                dot[j] = __builtin_fmaf(static_cast<float>(g[q].v[i]), static_cast<float>(row[j][q].v[i]), dot[j]);
+              }
+            }
           }
         }
         if (p.dy_sorted != nullptr) {
-#pragma unroll
-          for (int j = 0; j < kBatch; ++j) {
-            if (pos[j] < 0) continue;
+          auto store = [&](int j, int q, int c) {  // (as in the kernel above)
             Piece<T, V> o;
 #pragma unroll
-            for (int i = 0; i < V; ++i) o.v[i] = static_cast<T>(w[j] * static_cast<float>(g.v[i]));
+            for (int i = 0; i < V; ++i) o.v[i] = static_cast<T>(w[j] * static_cast<float>(g[q].v[i]));
             o.template store<MODE>(back + pos[j] * H + c, p.hidden - c);
+          };
+#pragma unroll
+          for (int j = 0; j < B; ++j) {
+            if (pos[j] < 0) continue;
+            store(j, 0, c0);
+            if constexpr (C == 2) {
+              if (c0 + G * V < p.hidden) store(j, 1, c0 + G * V);
+            }
           }
         }
       }
       if (p.dweights == nullptr) continue;
 #pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
+      for (int j = 0; j < B; ++j) {
 #pragma unroll
         for (int m = 1; m < (G < 64 ? G : 64); m *= 2) dot[j] += __shfl_xor(dot[j], m, 64);
       }
       if constexpr (G > 64) {
         if ((tid & 63) == 0) {
 #pragma unroll
-          for (int j = 0; j < kBatch; ++j) s_dot[turn][tid >> 6][j] = dot[j];
+          for (int j = 0; j < B; ++j) s_dot[turn][tid >> 6][j] = dot[j];
         }
         __syncthreads();  // (the other turn's sums were read before it)
         if (lane == 0) {
 #pragma unroll
-          for (int j = 0; j < kBatch; ++j) {
+          for (int j = 0; j < B; ++j) {
             dot[j] = 0.0F;
             for (int q = 0; q < G / 64; ++q) dot[j] += s_dot[turn][(tid >> 6) + q][j];
           }
@@ -607,7 +659,7 @@ __global__ __launch_bounds__(kThreads) void rr_combine_backward_kernel(CombinePa
       }
       if (here && lane == 0) {
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
+        for (int j = 0; j < B; ++j) {
           if (j0 + j < p.top_k) p.dweights[t * p.top_k + j0 + j] = pos[j] >= 0 ? dot[j] : 0.0F;
         }
       }
@@ -754,7 +806,18 @@ hipError_t combine_typed(const CombineParams& p, hipStream_t stream) {
   return with_group<false>(p.hidden, kPiece<T>, sizeof(TY) * p.tokens * p.hidden, [&](auto g, auto mode) {
     constexpr int G = decltype(g)::value;
     constexpr int M = decltype(mode)::value;
-    rr_combine_kernel<TY, T, G, M><<<token_grid<G>(p.tokens, p.hidden, kPiece<T>), kThreads, 0, stream>>>(p);
+    const dim3 grid = token_grid<G>(p.tokens, p.hidden, kPiece<T>);
+    if constexpr (M != kAny) {
+      if (p.top_k <= kFewTopK && static_cast<std::size_t>(p.hidden) > static_cast<std::size_t>(grid.y) * G * kPiece<T>) {
+        rr_combine_kernel<TY, T, G, M, kFewTopK, 2><<<grid, kThreads, 0, stream>>>(p);
+        return hipGetLastError();
+      }
+    }
+    if (p.top_k <= kFewTopK) {
+      rr_combine_kernel<TY, T, G, M, kFewTopK, 1><<<grid, kThreads, 0, stream>>>(p);
+    } else {
+      rr_combine_kernel<TY, T, G, M, kBatch, 1><<<grid, kThreads, 0, stream>>>(p);
+    }
     return hipGetLastError();
   });
 }
@@ -764,7 +827,18 @@ hipError_t backward_typed(const CombineParams& p, hipStream_t stream) {
   return with_group<true>(p.hidden, kPiece<T>, sizeof(T) * p.tokens * p.top_k * p.hidden, [&](auto g, auto mode) {
     constexpr int G = decltype(g)::value;
     constexpr int M = decltype(mode)::value;
-    rr_combine_backward_kernel<TY, T, G, M><<<token_grid(p.tokens, kThreads / G), kThreads, 0, stream>>>(p);
+    const unsigned grid = token_grid(p.tokens, kThreads / G);
+    if constexpr (M != kAny) {
+      if (p.top_k <= kFewTopK && p.hidden > G * kPiece<T>) {
+        rr_combine_backward_kernel<TY, T, G, M, kFewTopK, 2><<<grid, kThreads, 0, stream>>>(p);
+        return hipGetLastError();
+      }
+    }
+    if (p.top_k <= kFewTopK) {
+      rr_combine_backward_kernel<TY, T, G, M, kFewTopK, 1><<<grid, kThreads, 0, stream>>>(p);
+    } else {
+      rr_combine_backward_kernel<TY, T, G, M, kBatch, 1><<<grid, kThreads, 0, stream>>>(p);
+    }
     return hipGetLastError();
   });
 }
