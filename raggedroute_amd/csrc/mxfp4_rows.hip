@@ -1,8 +1,8 @@
 // 4-bit products for few rows an expert (decoding): the weights are read once from memory,
 // a line at a time.
 //
-// A workgroup of W waves takes 64 weight rows (of one operand, or 32 of each of two) of one
-// expert and 16 of its rows; the waves share the blocks of a row and add up through LDS in a
+// A workgroup of W waves takes R = 64 or 32 weight rows (of one operand, or half of them of each of
+// two) of one expert and 16 of its rows; the waves share the blocks of a row and add up through LDS in a
 // fixed order. A step is a slice of 256 elements: 128 bytes of every row, which eight lanes
 // bring as one line straight into the wave's own part of LDS, and eight scales. It is read
 // from there in operand order, and the next slice is on its way before it is multiplied. What bounds it is memory: two rows
@@ -33,13 +33,16 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 
 // Weights that are larger than the caches keep from one call to the next are loaded past them.
 constexpr std::size_t kStreamedBytes = std::size_t{64} << 20;
-constexpr int kWeightRows = 64;  // of a workgroup
-constexpr int kScaleBytes = 8;   // of a row's slice
-// A wave's part of LDS: weights, rows, their scales.
-constexpr int kRows = kWeightRows * kSliceBytes;
-constexpr int kWeightScales = kRows + 16 * kSliceBytes;
-constexpr int kRowScales = kWeightScales + kWeightRows * kScaleBytes;
-constexpr int kWaveBytes = kRowScales + 16 * kScaleBytes;
+constexpr int kScaleBytes = 8;  // of a row's slice
+
+// A wave's part of LDS for R weight rows: weights, rows, their scales.
+template <int R>
+struct Part {
+  static constexpr int kRows = R * kSliceBytes;
+  static constexpr int kWeightScales = kRows + 16 * kSliceBytes;
+  static constexpr int kRowScales = kWeightScales + R * kScaleBytes;
+  static constexpr int kBytes = kRowScales + 16 * kScaleBytes;
+};
 
 // HALF: which of the scales' two low bytes counts.
 template <int HALF>
@@ -50,12 +53,13 @@ __device__ __forceinline__ f4 multiply(i4 a, i4 b, f4 c, int a_scale, int b_scal
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a8, b8, c, kE2M1, kE2M1, HALF, a_scale, HALF, b_scale);
 }
 
-template <class Epi, int W, bool STREAMED>
+template <class Epi, int W, int R, bool STREAMED>
 __global__ __launch_bounds__(64 * W, 3) void rr_mxfp4_rows_kernel(Product prm, int blocks) {
   constexpr int B = Epi::kDual ? 2 : 1;
-  constexpr int F = kWeightRows / 16 / B;  // fragments of 16 columns of each right operand
+  constexpr int F = R / 16 / B;  // fragments of 16 columns of each right operand
+  using L = Part<R>;
   constexpr int kCols = 16 * F;
-  extern __shared__ __align__(128) char smem[];  // [W][kWaveBytes]
+  extern __shared__ __align__(128) char smem[];  // [W][L::kBytes]
   const int lane = static_cast<int>(threadIdx.x) & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int li = lane & 15, g = lane >> 4;
@@ -76,7 +80,7 @@ __global__ __launch_bounds__(64 * W, 3) void rr_mxfp4_rows_kernel(Product prm, i
   const int64_t x_slice = static_cast<int64_t>(prm.rows) * kScaleBytes, w_slice = static_cast<int64_t>(prm.experts) * N * kScaleBytes;
   // Rows past the last and columns past N are past the buffers' records: zeros. (What lies past
   // a row's end in its last slice is the next row's: its scales count as 2^-127.)
-  const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((RR_LDS char*)smem)) + wave * kWaveBytes;
+  const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((RR_LDS char*)smem)) + wave * L::kBytes;
   const uint32_t at_lane = static_cast<uint32_t>((lane >> 3) * prm.lda) + (static_cast<uint32_t>((lane & 7) ^ (lane >> 3)) << 4);
   auto load = [&](int s) {
     const int64_t from = static_cast<int64_t>(s) * kSliceBytes;
@@ -98,20 +102,22 @@ __global__ __launch_bounds__(64 * W, 3) void rr_mxfp4_rows_kernel(Product prm, i
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       const int64_t skip = (first + 8 * q) * row_bytes + from;
-      load_to_lds(make_buffer(static_cast<const char*>(prm.a) + skip, (count - 8 * q) * row_bytes - from), at_lane, lds + kRows + q * 1024);
+      load_to_lds(make_buffer(static_cast<const char*>(prm.a) + skip, (count - 8 * q) * row_bytes - from), at_lane, lds + L::kRows + q * 1024);
     }
 #pragma unroll
     for (int b = 0; b < B; ++b) {
       const char* scales = static_cast<const char*>(b == 0 ? prm.in : prm.in_up) + channel * kScaleBytes + s * w_slice;
 #pragma unroll
-      for (int q = 0; q < F / 2; ++q) {
-        load_words_to_lds(make_buffer(scales + q * 256, columns * kScaleBytes - q * 256), lane * 4,
-                          lds + kWeightScales + (b * F / 2 + q) * 256);
+      for (int q = 0; q < (F + 1) / 2; ++q) {
+        if (F > 1 || lane < 32) {
+          load_words_to_lds(make_buffer(scales + q * 256, columns * kScaleBytes - q * 256), lane * 4,
+                            lds + L::kWeightScales + b * F * 128 + q * 256);
+        }
       }
     }
     if (lane < 32) {
       load_words_to_lds(make_buffer(static_cast<const char*>(prm.a2) + first * static_cast<int64_t>(kScaleBytes) + s * x_slice, count * kScaleBytes),
-                        lane * 4, lds + kRowScales);
+                        lane * 4, lds + L::kRowScales);
     }
   };
   // block 2 g + h of a row's slice
@@ -134,11 +140,11 @@ __global__ __launch_bounds__(64 * W, 3) void rr_mxfp4_rows_kernel(Product prm, i
     for (int j = 0; j < B * F; ++j) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) w[j][h] = read16(at_row[h] + j * 16 * kSliceBytes);
-      w_scale[j] = read_scales(at_scale + kWeightScales + j * 16 * kScaleBytes);
+      w_scale[j] = read_scales(at_scale + L::kWeightScales + j * 16 * kScaleBytes);
     }
 #pragma unroll
-    for (int h = 0; h < 2; ++h) x[h] = read16(at_row[h] + kRows);
-    const int x_scale = read_scales(at_scale + kRowScales) & mask;
+    for (int h = 0; h < 2; ++h) x[h] = read16(at_row[h] + L::kRows);
+    const int x_scale = read_scales(at_scale + L::kRowScales) & mask;
     wait_lds();
     if (s + 1 < s1) load(s + 1);
     __builtin_amdgcn_sched_barrier(0);
@@ -150,7 +156,7 @@ __global__ __launch_bounds__(64 * W, 3) void rr_mxfp4_rows_kernel(Product prm, i
   }
   // (the parts of LDS become the sums')
   f4(*s_sums)[B * F][64] = reinterpret_cast<f4(*)[B * F][64]>(smem);
-  static_assert(W / 2 * B * F * 64 * sizeof(f4) <= W * kWaveBytes);
+  static_assert(W / 2 * B * F * 64 * sizeof(f4) <= W * L::kBytes);
   __syncthreads();
 
   // the waves' sums, halved round by round
@@ -188,37 +194,45 @@ __global__ __launch_bounds__(64 * W, 3) void rr_mxfp4_rows_kernel(Product prm, i
   }
 }
 
-// Workgroups that share an expert's columns.
-std::size_t blocks_of(int columns, bool dual) {
-  const int of_one = kWeightRows / (dual ? 2 : 1);
+// Workgroups that share an expert's columns, `weight_rows` each.
+std::size_t blocks_of(int columns, bool dual, int weight_rows = 64) {
+  const int of_one = weight_rows / (dual ? 2 : 1);
   return static_cast<std::size_t>((columns + of_one - 1) / of_one);
 }
 
-template <class Epi, int W, bool STREAMED>
+template <class Epi, int W, int R, bool STREAMED>
 hipError_t launch(const Product& prm, hipStream_t stream) {
-  constexpr int kLds = W * kWaveBytes;
+  constexpr int kLds = W * Part<R>::kBytes;
   if constexpr (kLds > 64 * 1024) {
     static std::atomic<uint64_t> allowed{0};
-    const hipError_t error = allow_lds(reinterpret_cast<const void*>(rr_mxfp4_rows_kernel<Epi, W, STREAMED>), kLds, &allowed);
+    const hipError_t error = allow_lds(reinterpret_cast<const void*>(rr_mxfp4_rows_kernel<Epi, W, R, STREAMED>), kLds, &allowed);
     if (error != hipSuccess) return error;
   }
-  const std::size_t blocks = blocks_of(prm.N, Epi::kDual);
+  const std::size_t blocks = blocks_of(prm.N, Epi::kDual, R);
   const std::size_t grid = most_groups(prm.rows, prm.experts) * blocks;
-  rr_mxfp4_rows_kernel<Epi, W, STREAMED><<<dim3(static_cast<unsigned>(grid)), 64 * W, kLds, stream>>>(prm, static_cast<int>(blocks));
+  rr_mxfp4_rows_kernel<Epi, W, R, STREAMED><<<dim3(static_cast<unsigned>(grid)), 64 * W, kLds, stream>>>(prm, static_cast<int>(blocks));
   return hipGetLastError();
 }
 
 // Few waves that have many slices each, but enough of them in all (two rows, two experts: K =
 // 4096, N = 14336, gated, two waves 23 us, four 24, eight 29; K = 14336, N = 4096 34, 22 and 16). One
 // where a row is one slice (1302 rows of 166 experts, K = 64, N = 5280: 36 -> 20 us).
+// Workgroups of half the weight rows where whole ones would leave CUs idle, with eight waves for long
+// sums and four for others (two rows, two experts: K = 14336, N = 4096 15.2 -> 12.6 us, by sixteen waves
+// 12.8; K = N = 4096 6.6 -> 5.9; 128 rows of one expert, K = N = 1024 5.1 -> 4.4, by eight 4.6), but not for
+// sums of a few slices (40 rows of three experts, K = 512, N = 520, gated: 4.3 and 4.8).
+constexpr std::size_t kFewWorkgroups = 256;
+
 template <class Epi, bool STREAMED>
 hipError_t launch_waves(const Product& prm, hipStream_t stream) {
   const int slices = (prm.K + 7) / 8;
   const std::size_t workgroups = most_groups(prm.rows, prm.experts) * blocks_of(prm.N, Epi::kDual);
-  if (slices >= 16 && workgroups < 384) return launch<Epi, 8, STREAMED>(prm, stream);
-  if (slices >= 8 && workgroups < 768) return launch<Epi, 4, STREAMED>(prm, stream);
-  if (slices >= 2) return launch<Epi, 2, STREAMED>(prm, stream);
-  return launch<Epi, 1, STREAMED>(prm, stream);
+  if (workgroups < kFewWorkgroups && slices >= 16) return launch<Epi, 8, 32, STREAMED>(prm, stream);
+  if (workgroups < kFewWorkgroups && slices >= 4) return launch<Epi, 4, 32, STREAMED>(prm, stream);
+  if (slices >= 16 && workgroups < 384) return launch<Epi, 8, 64, STREAMED>(prm, stream);
+  if (slices >= 8 && workgroups < 768) return launch<Epi, 4, 64, STREAMED>(prm, stream);
+  if (slices >= 2) return launch<Epi, 2, 64, STREAMED>(prm, stream);
+  return launch<Epi, 1, 64, STREAMED>(prm, stream);
 }
 
 }  // namespace
@@ -232,7 +246,7 @@ hipError_t launch_waves(const Product& prm, hipStream_t stream) {
 // And with more where there are few tiles, whose slices follow each other while most of the
 // card is idle: K = N = 4096, one expert, 128 rows (512 workgroups here) 12 us, on tiles 19; 256 rows
 // 23 and 21; K = 1024, N = 1024, eight experts, 1024 rows (1024 workgroups of few slices) 7.7 and 10; K =
-// 2784, N = 672, one expert, 256 rows 7 and 18.
+// 2784, N = 672, one expert, 256 rows 6.5 and 18.
 bool mxfp4_rows_ok(const Product& prm, bool dual) {
   const std::size_t workgroups = most_groups(prm.rows, prm.experts) * blocks_of(prm.N, dual);
   if (workgroups >= std::size_t{1} << 23) return false;  // (a launch has less than 2^32 threads)

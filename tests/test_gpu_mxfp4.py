@@ -236,6 +236,26 @@ def test_products(device, counts, k, n, dtype, gated, act, family):
     assert (y[sum(counts):].contiguous().view(torch.uint8) == 0xA5).all()
 
 
+# Sums of many slices by two, four and eight waves, with few workgroups (half the columns each) and with more.
+SHARED = [
+    ([1], 4097, 1),
+    ([1, 1, 0, 6], 4129, 272),
+    ([0, 17, 0], 14337, 63),
+    ([3, 33], 2049, 250),
+    ([20, 3], 1100, 97),
+    ([20, 3], 2050, 5501),
+    ([20, 3], 4100, 5501),
+    ([2, 0, 1], 4100, 4160),
+    ([20, 3], 800, 5501),
+]
+
+
+@pytest.mark.parametrize("dtype,gated,act", [("bf16", False, "silu"), ("f32", True, "gelu")])
+@pytest.mark.parametrize("counts,k,n", SHARED)
+def test_products_of_shared_sums(device, counts, k, n, dtype, gated, act):
+    test_products(device, counts, k, n, dtype, gated, act, "auto")
+
+
 @pytest.mark.parametrize("family", ["auto", "naive"])
 @pytest.mark.parametrize("rows", [5, 300])
 def test_scales_over_the_whole_range(device, rows, family):
