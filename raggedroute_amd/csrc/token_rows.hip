@@ -166,6 +166,10 @@ __global__ __launch_bounds__(kThreads) void rr_sort_few_kernel(SortParams p, int
 // another.
 //  - Up to kCountedRoutes every workgroup counts all ids and copies its tokens' rows, too: one
 //    launch (6002 routes of nine experts, rows of 1023: 10.5 us, in two launches 13.5).
+//    With kApartBytes of tokens or more (two thirds of it where rows are no whole pieces) the rows
+//    are another launch's, too (FP32 to FP16, one launch and two: 8192 rows of 2048 25.1 and
+//    22.6 us, 4096 51 and 43, 3001 of 7168, top-2, 39.8 and 37.3; BF16: 8192 of 2048 16.2 and 18.5,
+//    of 2827 41 and 28.5, 3001 of 2827, top-2, 15.4 and 15.5).
 //  - Above, the rows are another launch's, a workgroup a token in the tokens' order, which
 //    writes a row behind the other in every expert's segment (32768 rows of 4096 BF16 numbers of
 //    eight experts: 80 us; 512 workgroups that copy what they own, spread over the segments, 88).
@@ -174,6 +178,7 @@ __global__ __launch_bounds__(kThreads) void rr_sort_few_kernel(SortParams p, int
 constexpr int kOwnedRoutes = 512;  // of a workgroup at most
 constexpr int kOwners = 512;       // workgroups, or as many as routes make of kOwnedRoutes
 constexpr int kCountedRoutes = 8192;
+constexpr std::size_t kApartBytes = std::size_t{48} << 20;
 constexpr int kCountedExperts = 256;
 constexpr int kChunks = 32;
 
@@ -780,8 +785,13 @@ hipError_t sort_typed(const SortParams& p, hipStream_t stream) {
       rr_sort_owned_kernel<TX, T, decltype(mode)::value, false, decltype(rows)::value><<<grid, kThreads, 0, stream>>>(p, owned);
       return hipGetLastError();
     };
-    if (p.x_sorted == nullptr) return run(std::integral_constant<int, kAny>{}, std::false_type{});
-    if (p.hidden % kPiece<T> != 0) return run(std::integral_constant<int, kAny>{}, std::true_type{});
+    const bool whole = p.hidden % kPiece<T> == 0;
+    const bool apart = sizeof(TX) * tokens * p.hidden >= (whole ? kApartBytes : kApartBytes / 3 * 2);
+    if (p.x_sorted == nullptr || apart) {
+      const hipError_t error = run(std::integral_constant<int, kAny>{}, std::false_type{});
+      return error != hipSuccess || p.x_sorted == nullptr ? error : sort_rows<TX, T>(p, stream);
+    }
+    if (!whole) return run(std::integral_constant<int, kAny>{}, std::true_type{});
     if (sizeof(T) * routes * p.hidden < kStreamedBytes) return run(std::integral_constant<int, kWhole>{}, std::true_type{});
     return run(std::integral_constant<int, kStreamed>{}, std::true_type{});
   }

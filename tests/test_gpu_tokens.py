@@ -106,6 +106,15 @@ def test_sort_types(device, tokens, hidden, dtype, x_dtype):
     check_sort(ids, x, 7, dtype, sort(ids, x, 7, dtype, x_dtype, 3))
 
 
+@pytest.mark.parametrize("dtype,x_dtype", [("f16", "f32"), ("bf16", "bf16")])
+@pytest.mark.parametrize("tokens,top_k,hidden", [(3000, 2, 7000), (2999, 1, 7001), (8192, 1, 4104), (1500, 5, 11000)])
+def test_sort_wide_rows(device, tokens, top_k, hidden, dtype, x_dtype):
+    """Around the size from which the rows are another launch's."""
+    ids = routes(tokens, top_k, 13, tokens)
+    x = torch.randn(tokens, hidden, device="cuda:0").to(TYPES[x_dtype])
+    check_sort(ids, x, 13, dtype, sort(ids, x, 13, dtype, x_dtype, 1))
+
+
 @pytest.mark.parametrize("tokens", [9, 3000])
 def test_sort_maps_alone(device, tokens):
     ids = routes(tokens, 3, 11, tokens)
@@ -205,6 +214,18 @@ def test_combine_backward(device, tokens, top_k, experts, hidden, kind, dtype, y
         else:
             bound = (hidden + 1) * ROUNDING["f32"] * products.abs().sum(1) + LEAST["f32"]
             assert_within(b[5].t, products.sum(1), bound, "droute_weights")
+
+
+# Rows of several pieces a thread, the last of them of some threads only.
+WIDE = [(1030, 2, 5, 4104, "any"), (1030, 4, 6, 2056, "any"), (1100, 3, 3, 6152, "any"), (1025, 1, 2, 8200, "any"),
+        (1030, 2, 5, 4101, "any"), (1030, 5, 6, 4104, "any")]
+
+
+@pytest.mark.parametrize("dtype,y_dtype", [("bf16", "f32"), ("f16", "f16"), ("f32", "f32")])
+@pytest.mark.parametrize("tokens,top_k,experts,hidden,kind", WIDE)
+def test_combine_wide_rows(device, tokens, top_k, experts, hidden, kind, dtype, y_dtype):
+    test_combine(device, tokens, top_k, experts, hidden, kind, dtype, y_dtype)
+    test_combine_backward(device, tokens, top_k, experts, hidden, kind, dtype, y_dtype)
 
 
 def test_rows_that_no_route_names_do_not_enter(device):
