@@ -179,7 +179,6 @@ constexpr int kOwnedRoutes = 512;  // of a workgroup at most
 constexpr int kOwners = 512;       // workgroups, or as many as routes make of kOwnedRoutes
 constexpr int kCountedRoutes = 8192;
 constexpr std::size_t kApartBytes = std::size_t{48} << 20;
-constexpr int kCountedExperts = 256;
 constexpr int kChunks = 32;
 
 // Routes of a chunk: a multiple of 256, as few as make kChunks chunks or fewer.
@@ -204,7 +203,8 @@ __device__ __forceinline__ void count_ids(int32_t* counts, const int32_t* ids, i
 }
 
 __global__ __launch_bounds__(1024) void rr_sort_count_kernel(SortParams p) {
-  __shared__ int32_t s_counts[kCountedExperts];
+  __shared__ int32_t s_counts[RR_MAX_EXPERTS];
+  static_assert(RR_MAX_EXPERTS <= 1024, "a thread an expert");
   const int tid = static_cast<int>(threadIdx.x);
   const int64_t routes = static_cast<int64_t>(p.tokens) * p.top_k, chunk = chunk_routes(routes);
   const int64_t begin = static_cast<int64_t>(blockIdx.x) * chunk;
@@ -215,10 +215,10 @@ __global__ __launch_bounds__(1024) void rr_sort_count_kernel(SortParams p) {
   if (tid < p.experts) p.counts[static_cast<int>(blockIdx.x) * p.experts + tid] = s_counts[tid];
 }
 
-template <typename TX, typename T, int MODE, bool COUNTED, bool ROWS>
+// P experts a thread.
+template <typename TX, typename T, int MODE, bool COUNTED, bool ROWS, int P>
 __global__ __launch_bounds__(kThreads) void rr_sort_owned_kernel(SortParams p, int owned) {
-  static_assert(kCountedExperts <= kThreads, "a thread an expert");
-  __shared__ int32_t s_before[kCountedExperts], s_from[kCountedExperts];  // ids before the workgroup's own; from there on
+  __shared__ int32_t s_before[P * kThreads], s_from[P * kThreads];  // ids before the workgroup's own; from there on
   __shared__ int32_t s_wave[kThreads / 64];
   __shared__ int32_t s_pos[kOwnedRoutes];
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
@@ -227,15 +227,15 @@ __global__ __launch_bounds__(kThreads) void rr_sort_owned_kernel(SortParams p, i
   const int tokens = static_cast<int>(p.tokens - t0 < owned ? p.tokens - t0 : owned);
   const int64_t r0 = t0 * p.top_k;
   const int count = tokens * p.top_k;
-  if (tid < p.experts) s_before[tid] = s_from[tid] = 0;
+  for (int e = tid; e < p.experts; e += kThreads) s_before[e] = s_from[e] = 0;
   __syncthreads();
   if constexpr (COUNTED) {
     const int64_t chunk = chunk_routes(routes);
     const int mine = static_cast<int>(r0 / chunk), chunks = static_cast<int>((routes + chunk - 1) / chunk);
     // every expert's chunks shared among as many threads as there are for it
-    const int shares = kThreads / p.experts;
-    const int e = tid % p.experts, share = tid / p.experts;
-    if (share < shares) {
+    const int shares = max(kThreads / p.experts, 1);
+    for (int i = tid; i < shares * p.experts; i += kThreads) {
+      const int e = i % p.experts, share = i / p.experts;
       int32_t before = 0, from = 0;
 #pragma unroll 8
       for (int c = share; c < chunks; c += shares) {
@@ -262,21 +262,31 @@ __global__ __launch_bounds__(kThreads) void rr_sort_owned_kernel(SortParams p, i
   __syncthreads();
   // where every expert begins, and this workgroup's first route of it
   {
-    const int32_t all = tid < p.experts ? s_before[tid] + s_from[tid] : 0;
-    const int32_t through = rr::dev::wave_inclusive_scan(all);
+    int32_t all[P], sum = 0;  // of experts P tid + 0..
+#pragma unroll
+    for (int q = 0; q < P; ++q) {
+      const int e = P * tid + q;
+      all[q] = e < p.experts ? s_before[e] + s_from[e] : 0;
+      sum += all[q];
+    }
+    const int32_t through = rr::dev::wave_inclusive_scan(sum);
     if (lane == 63) s_wave[tid >> 6] = through;
     __syncthreads();
-    int32_t start = through - all;
+    int32_t start = through - sum;
     int32_t placed = 0;
     for (int w = 0; w < kThreads / 64; ++w) {
       start += w < tid >> 6 ? s_wave[w] : 0;
       placed += s_wave[w];
     }
-    if (tid < p.experts) s_before[tid] += start;
-    if (blockIdx.x == 0) {
-      if (tid < p.experts) p.offsets[tid] = start;
-      if (tid == 0) p.offsets[p.experts] = placed;
+#pragma unroll
+    for (int q = 0; q < P; ++q) {
+      const int e = P * tid + q;
+      if (e >= p.experts) continue;
+      s_before[e] += start;
+      if (blockIdx.x == 0) p.offsets[e] = start;
+      start += all[q];
     }
+    if (blockIdx.x == 0 && tid == 0) p.offsets[p.experts] = placed;
     if (p.sorted_route != nullptr) {  // (the last entries, spread over the workgroups)
       for (int64_t i = placed + static_cast<int64_t>(blockIdx.x) * kThreads + tid; i < routes; i += static_cast<int64_t>(gridDim.x) * kThreads) {
         p.sorted_route[i] = -1;
@@ -339,119 +349,6 @@ __global__ __launch_bounds__(kThreads) void rr_sort_owned_kernel(SortParams p, i
         for (int j = 0; j < p.top_k; ++j) {
           const int pos = s_pos[token[k] * p.top_k + j];
           if (pos >= 0) o.template store<MODE>(out + pos * H + column[k], p.hidden - column[k]);
-        }
-      }
-    }
-  }
-}
-
-// Many experts: a workgroup owns G of them and reads all ids twice, its 16 waves a contiguous
-// share each, four ids a lane and load, eight loads at a time. The first pass counts the ids below the workgroup's experts
-// and those of each; the second gives the routes of its experts their positions. No workgroup
-// waits for another and nothing is added atomically.
-constexpr int kRankWaves = 16;
-constexpr int kRankLoads = 8;
-constexpr int kRankExperts = 4;  // of a workgroup
-
-__global__ __launch_bounds__(64 * kRankWaves) void rr_sort_rank_kernel(SortParams p) {
-  constexpr int G = kRankExperts;
-  __shared__ int32_t s_count[G + 1][kRankWaves];  // of a wave's ids: [0] below, [1 + g] of expert e0 + g
-  typedef int quad __attribute__((ext_vector_type(4), aligned(4)));
-  constexpr int kStep = 256 * kRankLoads;  // ids of a wave's step
-  const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int e0 = static_cast<int>(blockIdx.x) * G;
-  const int64_t routes = static_cast<int64_t>(p.tokens) * p.top_k;
-  const int64_t share = ((routes + kRankWaves * 256 - 1) / (kRankWaves * 256)) * 256;
-  const int64_t begin = share * wave, end = begin + share < routes ? begin + share : routes;
-  // (as unsigned numbers, ids below 0 are above all; so is what stands for those past the end)
-  quad v[kRankLoads];
-  auto load = [&](int64_t from) {
-#pragma unroll
-    for (int q = 0; q < kRankLoads; ++q) {
-      const int64_t at = from + 256 * q + 4 * lane;
-      v[q] = quad{-1, -1, -1, -1};
-      if (at + 4 <= end) {
-        v[q] = *reinterpret_cast<const quad*>(p.ids + at);
-      } else if (at < end) {
-        for (int i = 0; at + i < end; ++i) {
-          const int id = p.ids[at + i];
-          v[q][0] = i == 0 ? id : v[q][0];
-          v[q][1] = i == 1 ? id : v[q][1];
-          v[q][2] = i == 2 ? id : v[q][2];
-        }
-      }
-    }
-  };
-  int32_t below = 0, mine[G] = {};
-  for (int64_t from = begin; from < end; from += kStep) {
-    load(from);
-#pragma unroll
-    for (int q = 0; q < kRankLoads; ++q) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        below += __popcll(__ballot(static_cast<unsigned>(v[q][i]) < static_cast<unsigned>(e0)));
-#pragma unroll
-        for (int g = 0; g < G; ++g) mine[g] += __popcll(__ballot(v[q][i] == e0 + g));
-      }
-    }
-  }
-  if (lane == 0) {
-    s_count[0][wave] = below;
-#pragma unroll
-    for (int g = 0; g < G; ++g) s_count[1 + g][wave] = e0 + g < p.experts ? mine[g] : 0;
-  }
-  __syncthreads();
-  // where expert e0 + g begins, and this wave's first route of it
-  int32_t start = 0, at_wave[G];
-  for (int w = 0; w < kRankWaves; ++w) start += s_count[0][w];
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-    at_wave[g] = start;
-    int32_t all = 0;
-    for (int w = 0; w < kRankWaves; ++w) {
-      if (w < wave) at_wave[g] += s_count[1 + g][w];
-      all += s_count[1 + g][w];
-    }
-    if (tid == 0 && e0 + g < p.experts) p.offsets[e0 + g] = start;
-    start += all;
-  }
-  if (e0 + G >= p.experts) {  // the last workgroup: start is the number of placed routes
-    if (tid == 0) p.offsets[p.experts] = start;
-    if (p.sorted_route != nullptr) {
-      for (int64_t i = start + tid; i < routes; i += 64 * kRankWaves) p.sorted_route[i] = -1;
-    }
-  }
-  const uint64_t lower = rr::dev::lanemask_lt();
-  for (int64_t from = begin; from < end; from += kStep) {
-    if (share > kStep) load(from);  // (a share of one step is still there)
-#pragma unroll
-    for (int q = 0; q < kRankLoads; ++q) {
-      const int64_t at = from + 256 * q + 4 * lane;
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-        if (e0 + g >= p.experts) continue;
-        uint64_t m[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) m[i] = __ballot(v[q][i] == e0 + g);
-        if ((m[0] | m[1] | m[2] | m[3]) == 0) continue;
-        int32_t pos = at_wave[g];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) pos += __popcll(m[i] & lower);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (v[q][i] == e0 + g) {
-            p.route_pos[at + i] = pos;
-            if (p.sorted_route != nullptr) p.sorted_route[pos] = static_cast<int32_t>(at + i);
-            ++pos;
-          }
-          at_wave[g] += __popcll(m[i]);
-        }
-      }
-      if (blockIdx.x == 0) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (static_cast<unsigned>(v[q][i]) >= static_cast<unsigned>(p.experts) && at + i < end) p.route_pos[at + i] = -1;
         }
       }
     }
@@ -762,53 +659,51 @@ hipError_t sort_rows(const SortParams& p, hipStream_t stream) {
   });
 }
 
-template <typename TX, typename T>
-hipError_t sort_typed(const SortParams& p, hipStream_t stream) {
-  const int64_t routes = static_cast<int64_t>(p.tokens) * p.top_k;
-  if (routes > kFewRoutes && p.experts <= kCountedExperts) {
-    const int64_t tokens = p.tokens;
-    const int owned = static_cast<int>(std::min<int64_t>((tokens + kOwners - 1) / kOwners, kOwnedRoutes / p.top_k));
-    const unsigned grid = static_cast<unsigned>((tokens + owned - 1) / owned);
-    const bool counted = routes > kCountedRoutes;
+template <typename TX, typename T, int P>
+hipError_t sort_owned(const SortParams& p, hipStream_t stream) {
+  const int64_t tokens = p.tokens, routes = tokens * p.top_k;
+  const int owned = static_cast<int>(std::min<int64_t>((tokens + kOwners - 1) / kOwners, kOwnedRoutes / p.top_k));
+  const unsigned grid = static_cast<unsigned>((tokens + owned - 1) / owned);
+  const bool counted = routes > kCountedRoutes;
+  const bool whole = p.hidden % kPiece<T> == 0;
+  const bool apart = counted || sizeof(TX) * tokens * p.hidden >= (whole ? kApartBytes : kApartBytes / 3 * 2);
+  if (p.x_sorted == nullptr || apart) {
     if (counted) {
       const int64_t chunk = chunk_routes(routes);
       rr_sort_count_kernel<<<static_cast<unsigned>((routes + chunk - 1) / chunk), 1024, 0, stream>>>(p);
       const hipError_t error = hipGetLastError();
       if (error != hipSuccess) return error;
-    }
-    if (counted) {
-      rr_sort_owned_kernel<TX, T, kAny, true, false><<<grid, kThreads, 0, stream>>>(p, owned);
-      const hipError_t error = hipGetLastError();
-      return error != hipSuccess || p.x_sorted == nullptr ? error : sort_rows<TX, T>(p, stream);
-    }
-    auto run = [&](auto mode, auto rows) {
-      rr_sort_owned_kernel<TX, T, decltype(mode)::value, false, decltype(rows)::value><<<grid, kThreads, 0, stream>>>(p, owned);
-      return hipGetLastError();
-    };
-    const bool whole = p.hidden % kPiece<T> == 0;
-    const bool apart = sizeof(TX) * tokens * p.hidden >= (whole ? kApartBytes : kApartBytes / 3 * 2);
-    if (p.x_sorted == nullptr || apart) {
-      const hipError_t error = run(std::integral_constant<int, kAny>{}, std::false_type{});
-      return error != hipSuccess || p.x_sorted == nullptr ? error : sort_rows<TX, T>(p, stream);
-    }
-    if (!whole) return run(std::integral_constant<int, kAny>{}, std::true_type{});
-    if (sizeof(T) * routes * p.hidden < kStreamedBytes) return run(std::integral_constant<int, kWhole>{}, std::true_type{});
-    return run(std::integral_constant<int, kStreamed>{}, std::true_type{});
-  }
-  if (routes <= kFewRoutes) {
-    const int counters = (p.experts + 1 + kThreads - 1) / kThreads;
-    if (p.x_sorted == nullptr) {
-      rr_sort_few_kernel<TX, T, false><<<p.tokens + counters, kThreads, 0, stream>>>(p, 1);
+      rr_sort_owned_kernel<TX, T, kAny, true, false, P><<<grid, kThreads, 0, stream>>>(p, owned);
     } else {
-      const int chunks = (p.hidden + kThreads * kPiece<T> - 1) / (kThreads * kPiece<T>);
-      rr_sort_few_kernel<TX, T, true><<<p.tokens * chunks + counters, kThreads, 0, stream>>>(p, chunks);
+      rr_sort_owned_kernel<TX, T, kAny, false, false, P><<<grid, kThreads, 0, stream>>>(p, owned);
     }
-    return hipGetLastError();
+    const hipError_t error = hipGetLastError();
+    return error != hipSuccess || p.x_sorted == nullptr ? error : sort_rows<TX, T>(p, stream);
   }
-  rr_sort_rank_kernel<<<(p.experts + kRankExperts - 1) / kRankExperts, 64 * kRankWaves, 0, stream>>>(p);
-  const hipError_t error = hipGetLastError();
-  if (error != hipSuccess || p.x_sorted == nullptr) return error;
-  return sort_rows<TX, T>(p, stream);
+  if (!whole) {
+    rr_sort_owned_kernel<TX, T, kAny, false, true, P><<<grid, kThreads, 0, stream>>>(p, owned);
+  } else if (sizeof(T) * routes * p.hidden < kStreamedBytes) {
+    rr_sort_owned_kernel<TX, T, kWhole, false, true, P><<<grid, kThreads, 0, stream>>>(p, owned);
+  } else {
+    rr_sort_owned_kernel<TX, T, kStreamed, false, true, P><<<grid, kThreads, 0, stream>>>(p, owned);
+  }
+  return hipGetLastError();
+}
+
+template <typename TX, typename T>
+hipError_t sort_typed(const SortParams& p, hipStream_t stream) {
+  if (static_cast<int64_t>(p.tokens) * p.top_k > kFewRoutes) {
+    static_assert(RR_MAX_EXPERTS <= 4 * kThreads);
+    return p.experts <= kThreads ? sort_owned<TX, T, 1>(p, stream) : sort_owned<TX, T, 4>(p, stream);
+  }
+  const int counters = (p.experts + 1 + kThreads - 1) / kThreads;
+  if (p.x_sorted == nullptr) {
+    rr_sort_few_kernel<TX, T, false><<<p.tokens + counters, kThreads, 0, stream>>>(p, 1);
+  } else {
+    const int chunks = (p.hidden + kThreads * kPiece<T> - 1) / (kThreads * kPiece<T>);
+    rr_sort_few_kernel<TX, T, true><<<p.tokens * chunks + counters, kThreads, 0, stream>>>(p, chunks);
+  }
+  return hipGetLastError();
 }
 
 template <typename TY, typename T>
@@ -856,7 +751,7 @@ hipError_t backward_typed(const CombineParams& p, hipStream_t stream) {
 }  // namespace
 
 std::size_t sort_tokens_counts(int64_t routes, int experts) {
-  return routes > kCountedRoutes && experts <= kCountedExperts ? static_cast<std::size_t>(kChunks) * experts : 0;
+  return routes > kCountedRoutes ? static_cast<std::size_t>(kChunks) * experts : 0;
 }
 
 hipError_t sort_tokens(const SortParams& p, hipStream_t stream) {

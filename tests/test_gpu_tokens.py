@@ -125,6 +125,15 @@ def test_sort_maps_alone(device, tokens):
     assert b["route"].untouched(slice(None)) and b["out"].untouched(slice(None))
 
 
+@pytest.mark.parametrize("kind", ["any", "one", "none"])
+@pytest.mark.parametrize("tokens,top_k,experts", [(129, 1, 1024), (2000, 4, 257), (2731, 3, 512), (9000, 1, 1023), (20000, 8, 768),
+                                                  (8193, 1, 256), (300, 64, 1024)])
+def test_sort_many_experts(device, tokens, top_k, experts, kind):
+    ids = routes(tokens, top_k, experts, tokens, kind)
+    x = torch.randn(tokens, 24, device="cuda:0").half()
+    check_sort(ids, x, experts, "f16", sort(ids, x, experts, "f16", "f16"))
+
+
 def test_sort_no_tokens(device):
     offsets = Buf(shape=(301,), dtype=torch.int32)
     run(rr.sort_tokens, rr.SortTokensArgs(offsets=offsets.ptr, tokens=0, experts=300, hidden=8))

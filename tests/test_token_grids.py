@@ -58,8 +58,8 @@ def test_grids(tmp_path):
     assert out.returncode == 0, out.stderr
     most = 2 ** 31 - 1
     want = [
-        # workgroups of 512 routes; of 64 routes a token eight tokens; of four experts; of one token; one a token and one for the offsets
-        f"maps {most} 1 256 {-(-most // 512)}", f"maps {most // 64} 64 8 {-(-(most // 64) // 8)}", f"maps {most} 1 1024 256",
+        # workgroups of 512 routes; of 64 routes a token eight tokens; of one token; one a token and one for the offsets
+        f"maps {most} 1 256 {-(-most // 512)}", f"maps {most // 64} 64 8 {-(-(most // 64) // 8)}", f"maps {most} 1 1024 {-(-most // 512)}",
         "maps 129 1 8 129", "maps 1 64 8 2",
         "combine 16384", "backward 16384", "gate 16384", "quantize 16384",
         # more workgroups than a launch of the kernel for few rows has, one a compute unit; groups of 16 rows times 64 columns

@@ -125,12 +125,12 @@ def test_workspaces():
 
 
 def test_workspace_of_many_routes():
-    """The counts of 32 parts of the routes, for up to 256 experts."""
+    """The counts of 32 parts of the routes."""
     def args(**change):
         return rr.SortTokensArgs(**(ENTRIES["sort_tokens"][1] | change))
 
     for tokens, top_k, experts, need in ((4096, 2, 256, 0), (8193, 1, 256, 32 * 256 * 4), (2 ** 30, 1, 9, 32 * 9 * 4),
-                                         (2 ** 30, 1, 257, 0), (2 ** 30, 2, 9, 0), (-1, 2, 9, 0)):
+                                         (2 ** 30, 1, 1024, 32 * 1024 * 4), (2 ** 30, 2, 9, 0), (-1, 2, 9, 0)):
         assert rr.get_sort_tokens_workspace_size(args(tokens=tokens, top_k=top_k, experts=experts)) == need
     many = dict(tokens=8193, top_k=1, experts=9)
     size = 32 * 9 * 4
