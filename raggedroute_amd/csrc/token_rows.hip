@@ -165,19 +165,21 @@ __global__ __launch_bounds__(kThreads) void rr_sort_few_kernel(SortParams p, int
 // ranks the workgroup's routes by ballots, 64 at a time in their order. No workgroup waits for
 // another.
 //  - Up to kCountedRoutes every workgroup counts all ids and copies its tokens' rows, too: one
-//    launch (6002 routes of nine experts, rows of 1023: 10.5 us, in two launches 13.5).
-//    With kApartBytes of tokens or more (two thirds of it where rows are no whole pieces) the rows
-//    are another launch's, too (FP32 to FP16, one launch and two: 8192 rows of 2048 25.1 and
+//    launch (6002 routes of nine experts, rows of 1023: 10.5 us, in two launches 13.5; 12000 routes, rows of
+//    1024 BF16 numbers: of eight experts 13.2, in three launches 14.3, of 512 13.5 and 17.5). With
+//    kApartBytes of tokens or more (two thirds of it where rows are no whole pieces) the rows
+//    are another launch's (FP32 to FP16, one launch and two: 8192 rows of 2048 25.1 and
 //    22.6 us, 4096 51 and 43, 3001 of 7168, top-2, 39.8 and 37.3; BF16: 8192 of 2048 16.2 and 18.5,
-//    of 2827 41 and 28.5, 3001 of 2827, top-2, 15.4 and 15.5).
-//  - Above, the rows are another launch's, a workgroup a token in the tokens' order, which
-//    writes a row behind the other in every expert's segment (32768 rows of 4096 BF16 numbers of
-//    eight experts: 80 us; 512 workgroups that copy what they own, spread over the segments, 88).
-//    Maps of 65536 routes of 128 experts 8.3 us; by workgroups that own an expert and read all
-//    ids 15.
+//    of 2827 41 and 28.5, 3001 of 2827, top-2, 15.4 and 15.5), and with more than kCountedApart routes the
+//    chunks' counts are, too (16384 rows of 4096 of eight experts 54.8, without 59.6).
+//  - Above, the counts and the rows are other launches', the rows' a workgroup a token in the tokens'
+//    order, which writes a row behind the other in every expert's segment (32768 rows of 4096 BF16
+//    numbers of eight experts: 80 us; 512 workgroups that copy what they own, spread over the
+//    segments, 88). Maps of 65536 routes of 128 experts 8.3 us; by workgroups that own an expert and read
+//    all ids 15.
 constexpr int kOwnedRoutes = 512;  // of a workgroup at most
 constexpr int kOwners = 512;       // workgroups, or as many as routes make of kOwnedRoutes
-constexpr int kCountedRoutes = 8192;
+constexpr int kCountedRoutes = 16384, kCountedApart = 8192;
 constexpr std::size_t kApartBytes = std::size_t{48} << 20;
 constexpr int kChunks = 32;
 
@@ -664,9 +666,10 @@ hipError_t sort_owned(const SortParams& p, hipStream_t stream) {
   const int64_t tokens = p.tokens, routes = tokens * p.top_k;
   const int owned = static_cast<int>(std::min<int64_t>((tokens + kOwners - 1) / kOwners, kOwnedRoutes / p.top_k));
   const unsigned grid = static_cast<unsigned>((tokens + owned - 1) / owned);
-  const bool counted = routes > kCountedRoutes;
   const bool whole = p.hidden % kPiece<T> == 0;
-  const bool apart = counted || sizeof(TX) * tokens * p.hidden >= (whole ? kApartBytes : kApartBytes / 3 * 2);
+  const bool large = p.x_sorted != nullptr && sizeof(TX) * tokens * p.hidden >= (whole ? kApartBytes : kApartBytes / 3 * 2);
+  const bool counted = routes > (large ? kCountedApart : kCountedRoutes);
+  const bool apart = counted || large;
   if (p.x_sorted == nullptr || apart) {
     if (counted) {
       const int64_t chunk = chunk_routes(routes);
@@ -751,7 +754,7 @@ hipError_t backward_typed(const CombineParams& p, hipStream_t stream) {
 }  // namespace
 
 std::size_t sort_tokens_counts(int64_t routes, int experts) {
-  return routes > kCountedRoutes ? static_cast<std::size_t>(kChunks) * experts : 0;
+  return routes > kCountedApart ? static_cast<std::size_t>(kChunks) * experts : 0;
 }
 
 hipError_t sort_tokens(const SortParams& p, hipStream_t stream) {
