@@ -39,3 +39,19 @@ TILES = [
 # Rows of a tile: rows an expert and columns of the products with scales far apart and with offsets that do not
 # rise (K = 320, three experts and more).
 TILE_SIZES = {128: (100, 2050), 256: (300, 2050)}
+
+# The kernel for few rows: (rows of every expert, K, N of plain and of gated products, [waves, weight rows of a
+# workgroup, 1 where the weights are loaded past the caches]).
+FEW_ROWS = [
+    ([20, 3], 4100, 500, 251, [8, 32, 0]),
+    ([20, 3], 1100, 300, 149, [4, 32, 0]),
+    ([20, 3], 4100, 5501, 2751, [8, 64, 0]),
+    ([20, 3], 2100, 6001, 3001, [4, 64, 0]),
+    ([20, 3], 600, 101, 130, [2, 64, 0]),
+    ([7, 0, 33], 200, 97, 64, [1, 64, 0]),
+    ([7], 20000, 8001, 4001, [8, 32, 1]),
+    ([7, 8], 9000, 8201, 4101, [8, 64, 1]),
+    ([7, 8, 6, 5], 4200, 8201, 4101, [4, 64, 1]),
+    ([3] * 31 + [1], 600, 7001, 3501, [2, 64, 1]),
+    ([2] * 63 + [1], 200, 9401, 4701, [1, 64, 1]),
+]
