@@ -228,7 +228,9 @@ hipError_t launch_waves(const Product& prm, hipStream_t stream) {
   const int slices = (prm.K + 7) / 8;
   const std::size_t workgroups = most_groups(prm.rows, prm.experts) * blocks_of(prm.N, Epi::kDual);
   if (workgroups < kFewWorkgroups && slices >= 16) return launch<Epi, 8, 32, STREAMED>(prm, stream);
-  if (workgroups < kFewWorkgroups && slices >= 4) return launch<Epi, 4, 32, STREAMED>(prm, stream);
+  // (the weights of so few workgroups' columns of less than 16 slices are 31 MB at most)
+  static_assert(kFewWorkgroups * 64 * 15 * kSliceBytes < kStreamedBytes);
+  if (workgroups < kFewWorkgroups && slices >= 4) return launch<Epi, 4, 32, false>(prm, stream);
   if (slices >= 16 && workgroups < 384) return launch<Epi, 8, 64, STREAMED>(prm, stream);
   if (slices >= 8 && workgroups < 768) return launch<Epi, 4, 64, STREAMED>(prm, stream);
   if (slices >= 2) return launch<Epi, 2, 64, STREAMED>(prm, stream);

@@ -671,7 +671,10 @@ hipError_t sort_rows(const SortParams& p, hipStream_t stream) {
   const std::size_t bytes = sizeof(T) * p.tokens * p.top_k * p.hidden;
   return with_group<false>(p.hidden, kPiece<T>, bytes, [&](auto g, auto mode) {
     constexpr int G = decltype(g)::value;
-    constexpr int M = decltype(mode)::value;
+    // (whole rows of more than 64 pieces that have this launch are more than kStreamedBytes: they are
+    // more than kCountedRoutes, or kApartBytes of tokens, which 16 bits halve)
+    static_assert((kCountedRoutes + 1) * std::size_t{65 * 16} >= kStreamedBytes && kApartBytes / 2 >= kStreamedBytes);
+    constexpr int M = G > 64 && decltype(mode)::value == kWhole ? kStreamed : decltype(mode)::value;
     rr_sort_rows_kernel<TX, T, G, M><<<token_grid<G>(p.tokens, p.hidden, kPiece<T>), kThreads, 0, stream>>>(p);
     return hipGetLastError();
   });
@@ -731,7 +734,7 @@ hipError_t combine_typed(const CombineParams& p, hipStream_t stream) {
     constexpr int G = decltype(g)::value;
     constexpr int M = decltype(mode)::value;
     const dim3 grid = token_grid<G>(p.tokens, p.hidden, kPiece<T>);
-    if constexpr (M != kAny) {
+    if constexpr (M != kAny && G == kThreads) {  // (of fewer threads each has one piece)
       if (p.top_k <= kFewTopK && static_cast<std::size_t>(p.hidden) > static_cast<std::size_t>(grid.y) * G * kPiece<T>) {
         rr_combine_kernel<TY, T, G, M, kFewTopK, 2><<<grid, kThreads, 0, stream>>>(p);
         return hipGetLastError();
@@ -752,7 +755,7 @@ hipError_t backward_typed(const CombineParams& p, hipStream_t stream) {
     constexpr int G = decltype(g)::value;
     constexpr int M = decltype(mode)::value;
     const unsigned grid = token_grid(p.tokens, kThreads / G);
-    if constexpr (M != kAny) {
+    if constexpr (M != kAny && G >= 64) {  // (of fewer threads each has one piece)
       if (p.top_k <= kFewTopK && p.hidden > G * kPiece<T>) {
         rr_combine_backward_kernel<TY, T, G, M, kFewTopK, 2><<<grid, kThreads, 0, stream>>>(p);
         return hipGetLastError();
