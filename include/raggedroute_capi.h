@@ -655,7 +655,8 @@ rr_status rr_int8_grouped_gemm(const rr_int8_grouped_gemm_args* args,
  *   x_sorted[route_pos[r]] = x[r / top_k].
  * A route whose id is none of 0..experts-1 (padding) is not placed: its route_pos is -1, and
  * the last entries of sorted_route are -1. Rows of x_sorted past offsets[experts] are left
- * alone. x_sorted NULL: the maps alone (x is not read). Without tokens offsets is zeros.
+ * alone. x_sorted NULL: the maps alone (x is not read, hidden may be anything). Without tokens
+ * offsets is zeros.
  * Workspace: rr_sort_tokens_workspace_size (0 for few routes), 16-byte aligned.
  */
 typedef struct rr_sort_tokens_args {

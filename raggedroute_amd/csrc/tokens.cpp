@@ -41,10 +41,11 @@ rr_status rr_sort_tokens(const rr_sort_tokens_args* args, const rr_runtime_conte
   if (args == nullptr) return rr::invalid_argument("sort_tokens: no argument struct was given");
   if (context == nullptr) return rr::invalid_argument("sort_tokens: no runtime context was given");
   const rr_sort_tokens_args& a = *args;
-  if (!rr::routes_ok(a.tokens, a.top_k) || !rr::experts_ok(a.experts) || !rr::width_ok(a.hidden)) {
+  // (the maps alone have no rows)
+  if (!rr::routes_ok(a.tokens, a.top_k) || !rr::experts_ok(a.experts) || (a.x_sorted != nullptr && !rr::width_ok(a.hidden))) {
     return rr::invalid_argument(
-        "sort_tokens: needs tokens >= 0, top_k in 1..64, tokens * top_k within 31 bits, 1 <= experts <= 1024 and "
-        "hidden in 1..1048576");
+        "sort_tokens: needs tokens >= 0, top_k in 1..64, tokens * top_k within 31 bits, 1 <= experts <= 1024 and, with "
+        "x_sorted, hidden in 1..1048576");
   }
   if (!rr::types_ok(a.dtype, a.x_dtype)) {
     return rr::make_status(RR_STATUS_UNSUPPORTED_DATA_TYPE,
