@@ -1,4 +1,4 @@
-// Argument checks that the wrappers of the expert block's operators share.
+// Argument checks that the wrappers of the expert block's, the token and the 4-bit operators share.
 #pragma once
 
 #include <cstddef>
@@ -42,14 +42,14 @@ inline rr_status choose_family(rr_kernel_selection kernel, int32_t architecture,
   const rr_status status = rr_resolve_device_architecture(architecture, &resolved);
   if (status.code != RR_STATUS_SUCCESS) return status;
   if (resolved != RR_ARCH_GFX950) {
-    return make_status(RR_STATUS_UNSUPPORTED_ARCHITECTURE, "expert block: kernels exist for gfx950 (MI355X) only");
+    return make_status(RR_STATUS_UNSUPPORTED_ARCHITECTURE, "this operator has kernels for gfx950 (MI355X) only");
   }
   const bool native = (kernel.family == RR_FAMILY_AUTO && kernel.implementation_id == 0) ||
                       (kernel.family == RR_FAMILY_OPTIMIZED && kernel.implementation_id == RR_IMPL_GFX950_NATIVE);
   const bool plain = naive != nullptr && kernel.family == RR_FAMILY_NAIVE && kernel.implementation_id == 0;
   if (!native && !plain) {
     return make_status(RR_STATUS_UNSUPPORTED_KERNEL_VARIANT,
-                       "expert block: no kernel has that family and implementation id");
+                       "no kernel of this operator has that family and implementation id");
   }
   if (naive != nullptr) *naive = plain;
   return ok_status();
@@ -61,7 +61,7 @@ inline rr_status check_workspace(const rr_runtime_context* context, std::size_t 
     return make_status(RR_STATUS_INSUFFICIENT_WORKSPACE, message);
   }
   if (!is_aligned(context->workspace, kWorkspaceAlignment)) {
-    return invalid_argument("expert block: the workspace must start on a 16-byte boundary");
+    return invalid_argument("the workspace of this operator must start on a 16-byte boundary");
   }
   return ok_status();
 }
