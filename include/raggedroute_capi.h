@@ -656,8 +656,8 @@ rr_status rr_int8_grouped_gemm(const rr_int8_grouped_gemm_args* args,
  * A route whose id is none of 0..experts-1 (padding) is not placed: its route_pos is -1, and
  * the last entries of sorted_route are -1. Rows of x_sorted past offsets[experts] are left
  * alone. x_sorted NULL: the maps alone (x is not read, hidden may be anything). Without tokens
- * offsets is zeros.
- * Workspace: rr_sort_tokens_workspace_size (0 for few routes), 16-byte aligned.
+ * offsets is zeros. The time of the maps grows with the square of the routes from some hundred
+ * thousand on. Workspace: rr_sort_tokens_workspace_size (0 for few routes), 16-byte aligned.
  */
 typedef struct rr_sort_tokens_args {
   const void* x;             /* [tokens, hidden] of x_dtype */
