@@ -19,9 +19,9 @@
 //
 // What bounds it: large products the power that the instructions draw, LDS, which is read and
 // written as long as they run (264 KB a slice), and the slices' loads (16384 rows of eight experts, K =
-// 4096, N = 14336: 560 us = 3.4 PFLOP/s; without its loads 438, without its LDS reads, too, 379, of
+// 4096, N = 14336: 555 us = 3.5 PFLOP/s; without its loads 438, without its LDS reads, too, 379, of
 // which the stores of 470 MB are 70); small ones the prologue and the epilogue of one or two
-// tiles a CU (6002 rows of nine experts, K = 1023, N = 1535, gated: 33 us, at K = 64 21).
+// tiles a CU (6002 rows of nine experts, K = 1023, N = 1535, gated: 30 us, at K = 64 21).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

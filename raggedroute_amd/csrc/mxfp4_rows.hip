@@ -246,9 +246,11 @@ hipError_t launch_waves(const Product& prm, hipStream_t stream) {
 // 64, N = 1024, gated: 32 rows 22 and 25, 48: 27 and 28, 64: 33 and 28; two, N = 2048: 32 rows 16 and 19, 48: 21
 // and 20; one, E = 167, N = 4816: 32 rows 48 and 52, 48: 62 and 57).
 // And with more where there are few tiles, whose slices follow each other while most of the
-// card is idle: K = N = 4096, one expert, 128 rows (512 workgroups here) 12 us, on tiles 19; 256 rows
-// 23 and 21; K = 1024, N = 1024, eight experts, 1024 rows (1024 workgroups of few slices) 7.7 and 10; K =
-// 2784, N = 672, one expert, 256 rows 6.5 and 18.
+// card is idle: K = N = 4096, one expert, 128 rows (512 workgroups here) 9.3 us, on tiles 18.8; K =
+// 2784, N = 672, one expert, 256 rows (176) 6.3 and 17.9. The limit of 640 workgroups leaves to tiles what is
+// faster on them from some 2000 on (K = 4096, N = 14336, one expert, 160 rows, 2240: 31 and 25.5; K = 2048,
+// N = 4096, eight experts, 512 rows, 2496: 19.4 and 14.2), and some that is not below that (K = N = 4096,
+// one expert, 256 rows, 1024: 13.9 and 21; K = N = 1024, eight experts, 1024 rows, 1136: 7.4 and 10.4).
 bool mxfp4_rows_ok(const Product& prm, bool dual) {
   const std::size_t workgroups = most_groups(prm.rows, prm.experts) * blocks_of(prm.N, dual);
   if (workgroups >= std::size_t{1} << 23) return false;  // (a launch has less than 2^32 threads)

@@ -7,8 +7,9 @@
 //   dlogits[t, id_j] = w_j sum_i w_i (dw_j - dw_i)
 //
 // Nothing here is arithmetic to speak of: the rows are moved at the rate of HBM (65536 rows of 2048
-// BF16 numbers: sorted in 59 us, 5.1 TB/s; combined in 55, 5.5; both gradients of that 102 to 114, 5.0
-// to 5.6; a plain copy 5.15) and the maps take the latency of a launch or two.
+// BF16 numbers: sorted in 59 us, 5.1 TB/s; combined in 55, 5.5; both gradients of that 99 to 114, 5.0
+// to 5.8; a plain copy 5.15) and the maps take the latency of a launch or two, up to some hundred
+// thousand routes.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -176,7 +177,9 @@ __global__ __launch_bounds__(kThreads) void rr_sort_few_kernel(SortParams p, int
 //    order, which writes a row behind the other in every expert's segment (32768 rows of 4096 BF16
 //    numbers of eight experts: 80 us; 512 workgroups that copy what they own, spread over the
 //    segments, 88). Maps of 65536 routes of 128 experts 8.3 us; by workgroups that own an expert and read
-//    all ids 15.
+//    all ids 15. A chunk is a 32nd of the routes, and a workgroup counts the ids of its own chunk up to
+//    its own: past some hundred thousand routes the time grows with their square (of 1, 8, 128 and 1024
+//    experts: 262144 routes 35, 15, 16 and 24 us; 2^20 407, 107, 77 and 91; 2^22 4300, 948, 512 and 538).
 constexpr int kOwnedRoutes = 512;  // of a workgroup at most
 constexpr int kOwners = 512;       // workgroups, or as many as routes make of kOwnedRoutes
 constexpr int kCountedRoutes = 16384, kCountedApart = 8192;
@@ -243,7 +246,7 @@ __global__ __launch_bounds__(kThreads) void rr_sort_owned_kernel(SortParams p, i
   const int tokens = static_cast<int>(p.tokens - t0 < owned ? p.tokens - t0 : owned);
   const int64_t r0 = t0 * p.top_k;
   const int count = tokens * p.top_k;
-  const int shift = COUNTED ? 0 : copies_shift(p.experts);  // (few ids are left to count)
+  const int shift = COUNTED ? 0 : copies_shift(p.experts);  // (COUNTED: no copies, a chunk's ids alone are counted)
   for (int i = tid; i < p.experts << shift; i += kThreads) s_before[i] = s_from[i] = 0;
   __syncthreads();
   if constexpr (COUNTED) {
