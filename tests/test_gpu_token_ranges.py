@@ -2,6 +2,7 @@
 whose calls are several launches."""
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
 
@@ -118,3 +119,45 @@ def test_captured(device, tokens, top_k, experts, hidden):
             assert torch.equal(t[name], other[name]), (seed, name)
     offsets, pos, route = base.maps(t["ids"].cpu(), experts)
     assert torch.equal(t["offsets"].cpu(), offsets) and torch.equal(t["pos"].cpu(), pos) and torch.equal(t["route"].cpu(), route)
+
+
+# around the sizes from which another kernel ranks the routes, and numbers of experts from which others count them
+@pytest.mark.parametrize("experts", [1, 2, 31, 32, 33, 255, 256, 257, 1023, 1024])
+@pytest.mark.parametrize("tokens,top_k", [(127, 1), (64, 2), (43, 3), (8191, 1), (2731, 3), (16384, 1), (8192, 2), (2341, 7), (257, 64),
+                                          (262144, 1), (131073, 2), (100001, 3), (4099, 64), (2 ** 20 + 1, 1)])
+def test_maps_at_borders(device, tokens, top_k, experts):
+    gen = torch.Generator(device="cuda:0")
+    gen.manual_seed(tokens + experts)
+    routes = tokens * top_k
+    for low, high in ((-1, experts + 1), (0, experts), (experts - 1, experts)):
+        ids = torch.randint(low, high, (routes,), device="cuda:0", generator=gen, dtype=torch.int32)
+        b = dict(ids=Buf(ids), offsets=Buf(shape=(experts + 1,), dtype=torch.int32), pos=Buf(shape=(routes,), dtype=torch.int32),
+                 route=Buf(shape=(routes,), dtype=torch.int32))
+        base.run(rr.sort_tokens, rr.SortTokensArgs(
+            expert_ids=b["ids"].ptr, offsets=b["offsets"].ptr, route_pos=b["pos"].ptr, sorted_route=b["route"].ptr, tokens=tokens,
+            experts=experts, top_k=top_k), rr.get_sort_tokens_workspace_size)
+        assert all(buf.intact() for buf in b.values())
+        key = torch.where((ids >= 0) & (ids < experts), ids, experts).long()
+        counts = torch.bincount(key, minlength=experts + 1)[:experts]
+        placed = int(counts.sum())
+        order = torch.sort(key, stable=True).indices[:placed].int()
+        offsets = torch.cat([torch.zeros(1, dtype=torch.long, device="cuda:0"), counts.cumsum(0)]).int()
+        pos = torch.full((routes,), -1, dtype=torch.int32, device="cuda:0")
+        pos[order.long()] = torch.arange(placed, dtype=torch.int32, device="cuda:0")
+        assert torch.equal(b["offsets"].t, offsets) and torch.equal(b["pos"].t, pos)
+        assert torch.equal(b["route"].t[:placed], order) and (b["route"].t[placed:] == -1).all()
+
+
+@pytest.mark.parametrize("dtype,least", [("f16", -24), ("bf16", -133), ("f32", -149)])
+def test_quantised_subnormal_numbers(device, dtype, least):
+    """Rows of multiples of the type's least number, alone and beside ordinary ones."""
+    x = torch.zeros(40, 64, dtype=torch.float64)
+    x[:, :32] = torch.arange(40 * 32, dtype=torch.float64).view(40, 32) % 67 - 33
+    x = torch.ldexp(x, torch.tensor(least))
+    x[20:, 40] = 1.5
+    x = x.to(TYPES[dtype])
+    assert x[:, :32].any(1).all()
+    code, scale = test_gpu_mxfp4.encode(x.double().numpy())
+    q, s = test_gpu_mxfp4.quantize(x.cuda(), dtype)
+    assert np.array_equal(s, test_gpu_mxfp4.layout(scale))
+    test_gpu_mxfp4.same_codes(q, test_gpu_mxfp4.pack(code))
